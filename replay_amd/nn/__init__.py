@@ -1,6 +1,6 @@
 from replay_amd.utils import TORCH_AVAILABLE
 from .agg import ConcatAggregator, SumAggregator
-from .attention import MultiheadAttention, MultiHeadDifferentialAttention
+from .attention import MultiheadAttention, MultiHeadDifferentialAttention, MultiheadLinearAttention
 from .embedding import (
     CategoricalEmbedding,
     CategoricalListEmbedding,
@@ -18,6 +18,7 @@ __all__ = [
     "SumAggregator",
     "MultiheadAttention",
     "MultiHeadDifferentialAttention",
+    "MultiheadLinearAttention",
     "CategoricalEmbedding",
     "CategoricalListEmbedding",
     "IdentityEmbedding",

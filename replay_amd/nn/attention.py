@@ -7,6 +7,9 @@ scores + additive mask + softmax + PV + out projection.  It is written so the
 scores->softmax->PV middle runs through replay_amd.ops (HIP flash-style
 fused attention on GPU, K1/K2 in SURVEY §2.12).
 
+``MultiheadLinearAttention`` is linear attention with a decay for each head, for
+long histories and for serving by single events.
+
 ``MultiHeadDifferentialAttention`` gives parity with reference
 replay/nn/attention.py:7 (dual softmax attentions subtracted with a learned
 lambda, per-head RMSNorm, reference :67-157).
@@ -135,6 +138,95 @@ class RMSNormPerHead(torch.nn.Module):
     def forward(self, x: torch.Tensor) -> torch.Tensor:
         norm = x * torch.rsqrt(x.pow(2).mean(-1, keepdim=True) + self.eps)
         return norm * self.weight
+
+
+class MultiheadLinearAttention(torch.nn.Module):
+    """Multi-head linear attention with a decay for each head: one product for
+    q, k, v, the decayed recurrence (``replay_amd.ops.linear_attention``), an
+    RMSNorm for each head in the place of softmax's normalization, and the
+    output product with the residual in its epilogue.
+
+    The decays start spread from a horizon of some ten to one of some hundred
+    positions, ``log_decay = logsigmoid(decay_logit)``; ``learn_decay`` trains
+    them.  Causal by construction; time and memory linear in the length.
+    """
+
+    def __init__(self, embed_dim: int, num_heads: int, bias: bool = True, learn_decay: bool = False) -> None:
+        super().__init__()
+        if embed_dim % num_heads != 0:
+            raise ValueError("embed_dim must divide num_heads")
+        from replay_amd.ops.fast_linear import ChunkedWgradLinear
+        from replay_amd.ops.linear_attention import MAX_HEAD_DIM
+
+        self.embed_dim = embed_dim
+        self.num_heads = num_heads
+        self.head_dim = embed_dim // num_heads
+        if self.head_dim > MAX_HEAD_DIM:
+            raise ValueError(f"embed_dim / num_heads must be at most {MAX_HEAD_DIM}, got {self.head_dim}")
+        self.in_proj = ChunkedWgradLinear(embed_dim, 3 * embed_dim, bias=bias)
+        self.out_proj = ChunkedWgradLinear(embed_dim, embed_dim, bias=bias)
+        # eps 1: the norm only shrinks.  A history's first outputs are single
+        # products q.k, some of them near zero, whose gradients a norm with a
+        # tiny eps would magnify without bound
+        self.head_norm = RMSNormPerHead(self.head_dim, eps=1.0)
+        horizon = 2.0 ** torch.linspace(3.0, 9.0, num_heads) if num_heads > 1 else torch.tensor([32.0])
+        # decay 1 - 1/horizon, as a logit
+        self.decay_logit = torch.nn.Parameter(torch.log(horizon - 1.0), requires_grad=learn_decay)
+
+    def log_decay(self) -> torch.Tensor:
+        return torch.nn.functional.logsigmoid(self.decay_logit.float())
+
+    def new_state(self, batch_size: int) -> torch.Tensor:
+        """The state before the first position: [B, H, Dh, Dh] float32 zeros."""
+        return torch.zeros(
+            batch_size, self.num_heads, self.head_dim, self.head_dim, device=self.decay_logit.device
+        )
+
+    def _heads(self, x: torch.Tensor):
+        from replay_amd.ops.fused_linear import fused_linear
+
+        qkv = fused_linear(x, self.in_proj.weight, self.in_proj.bias)
+        return (t.unflatten(-1, (self.num_heads, self.head_dim)) for t in qkv.chunk(3, dim=-1))
+
+    def _project(self, out: torch.Tensor, residual: Optional[torch.Tensor]) -> torch.Tensor:
+        from replay_amd.ops.fused_linear import fused_linear
+
+        out = self.head_norm(out.float()).to(out.dtype).flatten(-2)
+        return fused_linear(out, self.out_proj.weight, self.out_proj.bias, residual=residual)
+
+    def forward(
+        self,
+        x: torch.Tensor,
+        padding_mask: Optional[torch.Tensor] = None,
+        residual: Optional[torch.Tensor] = None,
+        state: Optional[torch.Tensor] = None,
+        return_state: bool = False,
+    ):
+        """x: [B, L, E]; padding_mask: [B, L] bool, True = VALID; residual:
+        [B, L, E], added to the output; state: what an earlier part of the same
+        histories left.  Returns [B, L, E], and the new state if asked for."""
+        from replay_amd.ops.linear_attention import linear_attention
+
+        q, k, v = (t.transpose(1, 2) for t in self._heads(x))
+        out = linear_attention(q, k, v, self.log_decay(), padding_mask, state, return_state=return_state)
+        out, state = out if return_state else (out, None)
+        out = self._project(out.transpose(1, 2), residual)
+        return (out, state) if return_state else out
+
+    @torch.no_grad()
+    def step(
+        self,
+        x: torch.Tensor,
+        state: torch.Tensor,
+        active: Optional[torch.Tensor] = None,
+        residual: Optional[torch.Tensor] = None,
+    ) -> torch.Tensor:
+        """One new position for each row, x: [B, E]; the state is updated in
+        place, except for the rows that ``active`` [B] leaves out."""
+        from replay_amd.ops.linear_attention import linear_attention_step
+
+        q, k, v = self._heads(x)
+        return self._project(linear_attention_step(q, k, v, self.log_decay(), state, active), residual)
 
 
 class MultiHeadDifferentialAttention(torch.nn.Module):

@@ -5,8 +5,9 @@ conv1d(k=1) -> activation -> conv1d(k=1) + residual + dropout; SwiGLU:60;
 SwiGLUEncoder:102).
 
 MI355X note: a conv1d with kernel 1 IS a GEMM; both matmuls here map to MFMA
-through hipBLASLt, and the activation+residual epilogue is fused by the HIP
-fused-FFN kernel (K4/K5 in SURVEY §2.12) on the GPU path.
+through hipBLASLt, or with ``PointWiseFeedForward(fused=True)`` through the
+framework's own product with bias, activation and residual in its epilogue
+(``replay_amd.ops.fused_linear``).
 """
 
 from __future__ import annotations
@@ -21,6 +22,7 @@ class PointWiseFeedForward(torch.nn.Module):
         dropout: float = 0.0,
         activation: str = "relu",
         hidden_dim: int = None,
+        fused: bool = False,
     ) -> None:
         super().__init__()
         hidden = hidden_dim or embedding_dim
@@ -33,8 +35,22 @@ class PointWiseFeedForward(torch.nn.Module):
         self.dropout1 = torch.nn.Dropout(dropout)
         self.dropout2 = torch.nn.Dropout(dropout)
         self.activation = torch.nn.ReLU() if activation == "relu" else torch.nn.GELU()
+        # fused=True: bias, activation and residual in the products' epilogue
+        # (replay_amd.ops.fused_linear); the same parameters either way
+        self.fused = activation if fused else None
+
+    def _forward_fused(self, x: torch.Tensor) -> torch.Tensor:
+        from replay_amd.ops.fused_linear import fused_linear
+
+        h = self.dropout1(fused_linear(x, self.w1.weight, self.w1.bias, activation=self.fused))
+        if self.training and self.dropout2.p > 0.0:
+            # the dropout stands between the product and the residual
+            return self.dropout2(fused_linear(h, self.w2.weight, self.w2.bias)) + x
+        return fused_linear(h, self.w2.weight, self.w2.bias, residual=x)
 
     def forward(self, x: torch.Tensor) -> torch.Tensor:
+        if self.fused is not None:
+            return self._forward_fused(x)
         out = self.dropout2(self.w2(self.dropout1(self.activation(self.w1(x)))))
         return out + x
 

@@ -2,6 +2,8 @@ from .bert4rec import Bert4Rec, Bert4RecBody
 from .sasrec import (
     DiffTransformerBlock,
     DiffTransformerLayer,
+    LinearTransformerBlock,
+    LinearTransformerLayer,
     PositionAwareAggregator,
     SasRec,
     SasRecBody,
@@ -15,6 +17,8 @@ __all__ = [
     "Bert4RecBody",
     "DiffTransformerBlock",
     "DiffTransformerLayer",
+    "LinearTransformerBlock",
+    "LinearTransformerLayer",
     "PositionAwareAggregator",
     "SasRec",
     "SasRecBody",

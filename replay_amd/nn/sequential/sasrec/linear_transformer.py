@@ -1,0 +1,139 @@
+"""Linear-attention encoder blocks for SASRec.
+
+The place of ``SasRecTransformerLayer`` (same call signature) for long
+histories and for serving by events: time and memory are linear in the
+history's length, and what a history leaves behind is one state for each
+block, so a new interaction costs one ``step`` instead of a new pass over the
+history.  The blocks keep the pre-LN order of the SASRec encoder
+(reference replay/nn/sequential/sasrec/transformer.py:93-110); position enters
+through the decays, so the aggregator needs no positional embedding.
+"""
+
+from __future__ import annotations
+
+from typing import List, Optional, Tuple
+
+import torch
+
+from replay_amd.nn.attention import MultiheadLinearAttention
+from replay_amd.nn.ffn import PointWiseFeedForward
+from replay_amd.nn.mask import MaskSpec
+from replay_amd.ops.layer_norm import LayerNorm
+
+
+class LinearTransformerBlock(torch.nn.Module):
+    def __init__(
+        self,
+        embedding_dim: int,
+        num_heads: int,
+        dropout: float = 0.0,
+        activation: str = "relu",
+        learn_decay: bool = False,
+    ) -> None:
+        super().__init__()
+        self.attn_norm = LayerNorm(embedding_dim, eps=1e-8)
+        self.attention = MultiheadLinearAttention(embedding_dim, num_heads, learn_decay=learn_decay)
+        self.ffn_norm = LayerNorm(embedding_dim, eps=1e-8)
+        self.ffn = PointWiseFeedForward(embedding_dim, dropout, activation, fused=True)
+
+    def forward(
+        self,
+        x: torch.Tensor,
+        padding_mask: Optional[torch.Tensor] = None,
+        state: Optional[torch.Tensor] = None,
+        return_state: bool = False,
+    ):
+        out = self.attention(
+            self.attn_norm(x), padding_mask, residual=x, state=state, return_state=return_state
+        )
+        x, state = out if return_state else (out, None)
+        x = self.ffn(self.ffn_norm(x))
+        return (x, state) if return_state else x
+
+    def step(self, x: torch.Tensor, state: torch.Tensor, active: Optional[torch.Tensor] = None) -> torch.Tensor:
+        x = self.attention.step(self.attn_norm(x), state, active, residual=x)
+        return self.ffn(self.ffn_norm(x))
+
+
+class LinearTransformerLayer(torch.nn.Module):
+    """Drop-in encoder for SasRecBody, with ``prefill`` and ``step`` beside
+    ``forward`` for serving."""
+
+    def __init__(
+        self,
+        embedding_dim: int,
+        num_heads: int,
+        num_blocks: int,
+        dropout: float = 0.0,
+        activation: str = "relu",
+        learn_decay: bool = False,
+    ) -> None:
+        super().__init__()
+        self.blocks = torch.nn.ModuleList(
+            [
+                LinearTransformerBlock(embedding_dim, num_heads, dropout, activation, learn_decay)
+                for _ in range(num_blocks)
+            ]
+        )
+
+    @staticmethod
+    def _check_mask(attn_mask) -> None:
+        if attn_mask is None:
+            return
+        if not isinstance(attn_mask, MaskSpec):
+            raise ValueError("linear attention takes no additive attention mask: pass a MaskSpec or None")
+        if not attn_mask.causal:
+            raise ValueError("linear attention is causal: the attention mask must be too")
+
+    @staticmethod
+    def _blank(x: torch.Tensor, valid: Optional[torch.Tensor]) -> torch.Tensor:
+        return x if valid is None else x * valid.unsqueeze(-1).to(x.dtype)
+
+    def forward(
+        self,
+        x: torch.Tensor,
+        attn_mask=None,
+        padding_mask: Optional[torch.Tensor] = None,
+    ) -> torch.Tensor:
+        """x: [B, L, E]; padding_mask: [B, L] bool, True = VALID.  attn_mask
+        (DefaultAttentionMask's MaskSpec) must be causal; without a
+        padding_mask its own is used."""
+        self._check_mask(attn_mask)
+        if padding_mask is None and attn_mask is not None:
+            padding_mask = attn_mask.padding_mask
+        for block in self.blocks:
+            x = self._blank(block(x, padding_mask), padding_mask)
+        return x
+
+    def prefill(
+        self,
+        x: torch.Tensor,
+        padding_mask: Optional[torch.Tensor] = None,
+        states: Optional[List[torch.Tensor]] = None,
+    ) -> Tuple[torch.Tensor, List[torch.Tensor]]:
+        """``forward`` that also returns the blocks' states after the last
+        position, and starts from ``states`` if given (which it leaves as they
+        were)."""
+        if states is not None and len(states) != len(self.blocks):
+            raise ValueError(f"expected {len(self.blocks)} states, got {len(states)}")
+        new = []
+        for i, block in enumerate(self.blocks):
+            x, state = block(x, padding_mask, None if states is None else states[i], return_state=True)
+            x = self._blank(x, padding_mask)
+            new.append(state)
+        return x, new
+
+    @torch.no_grad()
+    def step(
+        self,
+        x: torch.Tensor,
+        states: List[torch.Tensor],
+        active: Optional[torch.Tensor] = None,
+    ) -> torch.Tensor:
+        """One new position for each row, x: [B, E]; ``states`` are updated in
+        place.  Rows that ``active`` [B] leaves out keep theirs and give zeros."""
+        if len(states) != len(self.blocks):
+            raise ValueError(f"expected {len(self.blocks)} states, got {len(states)}")
+        for block, state in zip(self.blocks, states):
+            x = self._blank(block.step(x, state, active), active)
+        return x

@@ -49,7 +49,12 @@ def build_extension(verbose: bool = True):
         name=EXT_NAME,
         sources=sources,
         extra_cflags=["-O3"],
-        extra_cuda_cflags=["-O3", "--offload-arch=gfx950", "-std=c++17"],
+        # no packed fp32 arithmetic: hipcc forms it from ordinary float code, and
+        # some of its forms have given wrong results on this hardware
+        extra_cuda_cflags=[
+            "-O3", "--offload-arch=gfx950", "-std=c++17",
+            "-Xclang", "-target-feature", "-Xclang", "-packed-fp32-ops",
+        ],
         build_directory=str(build_dir),
         verbose=verbose,
     )

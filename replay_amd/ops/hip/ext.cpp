@@ -48,6 +48,26 @@ torch::Tensor metrics_reduce(torch::Tensor preds, torch::Tensor gt,
                              c10::optional<torch::Tensor> train, torch::Tensor ks);
 std::vector<torch::Tensor> scored_topk_gemm_fp8(torch::Tensor q, torch::Tensor w,
                                                 torch::Tensor thresholds, int64_t capacity);
+std::vector<torch::Tensor> linear_attention_fwd(torch::Tensor q, torch::Tensor k, torch::Tensor v,
+                                                torch::Tensor log_decay,
+                                                c10::optional<torch::Tensor> mask,
+                                                c10::optional<torch::Tensor> state, double scale,
+                                                bool want_state);
+std::vector<torch::Tensor> linear_attention_bwd(
+    torch::Tensor q, torch::Tensor k, torch::Tensor v, torch::Tensor log_decay,
+    c10::optional<torch::Tensor> mask, c10::optional<torch::Tensor> state, torch::Tensor dout,
+    c10::optional<torch::Tensor> dstate, torch::Tensor seg, double scale, bool need_decay,
+    bool need_state);
+torch::Tensor linear_attention_step(torch::Tensor q, torch::Tensor k, torch::Tensor v,
+                                    torch::Tensor log_decay, torch::Tensor state,
+                                    c10::optional<torch::Tensor> active, double scale);
+std::vector<torch::Tensor> fused_linear_fwd(torch::Tensor x, torch::Tensor weight,
+                                            c10::optional<torch::Tensor> bias,
+                                            c10::optional<torch::Tensor> residual, int64_t act,
+                                            bool want_z);
+std::vector<torch::Tensor> fused_linear_bwd(torch::Tensor dy, torch::Tensor x, torch::Tensor weight,
+                                            torch::Tensor z, int64_t act, bool need_x, bool need_w,
+                                            bool need_b);
 
 PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
   m.def("layer_norm_fwd", &layer_norm_fwd, "fused LayerNorm forward (gfx950)");
@@ -75,4 +95,13 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
         "fused e4m3 MFMA score-GEMM + top-k candidate selection (gfx950)");
   m.def("metrics_reduce", &metrics_reduce,
         "fused ranking-metric sums: hits + all cutoffs in one launch (gfx950)");
+  m.def("linear_attention_fwd", &linear_attention_fwd,
+        "linear attention with a decay per head: outputs and states (gfx950)");
+  m.def("linear_attention_bwd", &linear_attention_bwd,
+        "linear attention backward: dq, dk, dv, dlog_decay, dstate (gfx950)");
+  m.def("linear_attention_step", &linear_attention_step,
+        "linear attention for one position, the state updated in place (gfx950)");
+  m.def("fused_linear_fwd", &fused_linear_fwd,
+        "linear + bias + activation + residual in one product (gfx950)");
+  m.def("fused_linear_bwd", &fused_linear_bwd, "its gradients dx, dW, db (gfx950)");
 }

@@ -1,0 +1,664 @@
+// Linear attention with a decay for each head (gfx950).
+//
+// For the valid positions t of one (batch, head), with l = exp(log_decay):
+//
+//   S_t = l S_{t-1} + k_t v_t^T          o_t = scale q_t^T S_t
+//
+// A masked position takes no part: it neither decays nor writes the state,
+// and its output is zero.  Over a chunk of C positions with the start state S
+// and n_i = the number of valid positions among the chunk's first i+1,
+//
+//   o_i = scale [ l^{n_i} q_i^T S + sum_{j<=i} l^{n_i-n_j} (q_i.k_j) v_j ]
+//   S  <- l^N S + sum_j l^{N-n_j} k_j v_j^T                    (N = n_last)
+//
+// Every gradient but the decay's is another linear attention, so ONE pass
+// kernel serves all of them (dO = the output's gradient):
+//
+//   dq = forward pass over (q, k, v) := (dO, v, k), state transposed
+//   dk = REVERSED pass over (v, dO, q), dv = reversed pass over (k, q, dO):
+//        position j sees the later ones i >= j; the state is dL/dS, the
+//        query-side weight is l^{N-n_j} and the update's is scale l^{n_i}
+//
+// The decay's gradient is taken forward: S' = dS/dlog l obeys
+//   S' <- l^N (S' + N S) + sum_j (N-n_j) l^{N-n_j} k_j v_j^T
+// and rides on the dq pass as sum_i q_i . dq'_i.  (The shorter formula
+// sum_t t (q_t.dq_t - k_t.dk_t) cancels nearly everything on long histories.)
+//
+// Where batch x heads alone cannot fill the card, the history is cut into
+// segments: a state-only pass gives each segment's own contribution, a scan
+// over the segments turns these into start states, and the full pass then
+// runs all segments at once.
+
+#include <torch/extension.h>
+#include <ATen/hip/HIPContext.h>
+#include <ATen/hip/impl/HIPGuardImplMasqueradingAsCUDA.h>
+#include "common.h"
+
+namespace {
+
+typedef __attribute__((ext_vector_type(4))) float f32x4;
+
+struct Rows {  // [B, H, L, D] with unit stride in D
+  const void* p;
+  int64_t b, h, l;
+};
+
+struct PassArgs {
+  Rows q, k, v, x;       // x: the query whose product with dq' is the decay's gradient
+  void* out;
+  int64_t out_b, out_h, out_l;
+  const float* log_decay;            // [H]
+  const bool* mask;                  // [B, L] or nullptr, true = valid
+  int64_t mask_b, mask_l;
+  const float* state_in;             // [B, H, Dk, Dv] or nullptr
+  float* state_out;                  // same or nullptr: the state after the last chunk
+  const float* state_end_grad;       // same or nullptr: for <S'_end, dS_end>
+  float* seg;                        // [B, H, G, Dk, Dv]: contributions, then start states
+  float* seg_d;                      // the same for S'
+  int* seg_count;                    // [B, H, G] valid positions
+  float* decay_part;                 // [B, H, G] partial sums of the decay's gradient
+  int64_t st_c, st_e;                // strides of a state's (contraction, value) axes
+  int B, H, L, Dc, De, G, seg_chunks;
+  bool vec_c, vec_e, vec_x;          // 16-byte loads are aligned (contraction / value side, x)
+  float c_pair, c_inter, c_update;   // where the scale goes
+};
+
+// One 16-byte piece of a row, widened to float; beyond D it reads as zero.
+template <typename T>
+__device__ __forceinline__ void load_piece(const T* row, int d0, int D, bool vec, float* o) {
+  constexpr int V = 16 / sizeof(T);
+  if (vec) {
+    if (d0 < D) {
+      alignas(16) T t[V];
+      *reinterpret_cast<float4*>(t) = *reinterpret_cast<const float4*>(row + d0);
+#pragma unroll
+      for (int i = 0; i < V; ++i) o[i] = to_f32<T>(t[i]);
+    } else {
+#pragma unroll
+      for (int i = 0; i < V; ++i) o[i] = 0.f;
+    }
+  } else {
+#pragma unroll
+    for (int i = 0; i < V; ++i) o[i] = (d0 + i < D) ? to_f32<T>(row[d0 + i]) : 0.f;
+  }
+}
+
+// Positions [l0, l0+C) of one head into LDS as float [C][DP+4]; rows that the
+// mask or the length leaves out are zero whatever they hold.
+template <typename T, int DP, int C>
+__device__ __forceinline__ void stage(float* dst, const Rows& r, int b, int h, int l0, int D,
+                                      bool vec, unsigned bits) {
+  constexpr int V = 16 / sizeof(T), PR = DP / V, LD = DP + 4;
+  const T* base = reinterpret_cast<const T*>(r.p) + b * r.b + h * r.h;
+  for (int i = threadIdx.x; i < C * PR; i += DP * 4) {
+    const int row = i / PR, d0 = (i % PR) * V;
+    float o[V];
+    if ((bits >> row) & 1u) {
+      load_piece<T>(base + (int64_t)(l0 + row) * r.l, d0, D, vec, o);
+    } else {
+#pragma unroll
+      for (int j = 0; j < V; ++j) o[j] = 0.f;
+    }
+#pragma unroll
+    for (int j = 0; j < V; j += 4)
+      *reinterpret_cast<f32x4*>(dst + row * LD + d0 + j) = f32x4{o[j], o[j + 1], o[j + 2], o[j + 3]};
+  }
+}
+
+__device__ __forceinline__ f32x4 mfma4(float a, float b, f32x4 c) {
+  return __builtin_amdgcn_mfma_f32_16x16x4f32(a, b, c, 0, 0, 0);
+}
+
+// One segment of one (batch, head).  DP/16 waves; each owns 16 value columns
+// and the whole contraction axis of the state, in the accumulator layout
+// (column = lane & 15, row = 4 (lane >> 4) + r), which is also the layout of
+// an operand whose contraction index is visited in that order: neither the
+// state nor the pair weights leave the registers between products.
+template <typename T, int DP, bool REV, bool STATE_ONLY, bool DERIV>
+__global__ __launch_bounds__(DP * 4) void la_pass_f32(PassArgs a) {
+  constexpr int C = 16, LD = DP + 4, NT = DP / 16;
+  __shared__ __attribute__((aligned(16))) float q_s[STATE_ONLY ? 4 : C * LD];
+  __shared__ __attribute__((aligned(16))) float k_s[C * LD];
+  __shared__ __attribute__((aligned(16))) float v_s[C * LD];
+  __shared__ __attribute__((aligned(16))) float x_s[(DERIV && !STATE_ONLY) ? C * LD : 4];
+  __shared__ float lam[C + 1];
+  __shared__ float red[DP / 16];
+
+  const int seg = blockIdx.x % a.G;
+  const int64_t bh = blockIdx.x / a.G;
+  const int b = bh / a.H, h = bh % a.H;
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  const int lo = lane & 15, g = lane >> 4;
+  const int e0 = wave * 16, e = e0 + lo;
+  const int64_t state_size = (int64_t)a.Dc * a.De;
+  const float ld = a.log_decay[h];
+  // a decay of zero (log -inf) keeps l^0 = 1
+  if (threadIdx.x <= C) lam[threadIdx.x] = threadIdx.x ? expf(ld * threadIdx.x) : 1.f;
+
+  f32x4 S[NT], Sd[DERIV ? NT : 1];
+  {
+    const float* src = nullptr;
+    const float* src_d = nullptr;
+    if (!STATE_ONLY) {
+      if (a.G > 1) {
+        src = a.seg + (bh * a.G + seg) * state_size;
+        if (DERIV) src_d = a.seg_d + (bh * a.G + seg) * state_size;
+      } else if (a.state_in) {
+        src = a.state_in + bh * state_size;
+      }
+    }
+#pragma unroll
+    for (int t = 0; t < NT; ++t) {
+#pragma unroll
+      for (int r = 0; r < 4; ++r) {
+        const int c = 16 * t + 4 * g + r;
+        const bool in = c < a.Dc && e < a.De;
+        S[t][r] = (src && in) ? src[c * a.st_c + e * a.st_e] : 0.f;
+        if (DERIV) Sd[t][r] = (src_d && in) ? src_d[c * a.st_c + e * a.st_e] : 0.f;
+      }
+    }
+  }
+
+  const int n_chunks = (a.L + C - 1) / C;
+  const int first = seg * a.seg_chunks, last = min(n_chunks, first + a.seg_chunks);
+  int total = 0;
+  float d_decay = 0.f;
+  for (int step = first; step < last; ++step) {
+    const int l0 = (REV ? first + last - 1 - step : step) * C;
+    const int pos = l0 + lo;
+    const bool ok = lane < C && pos < a.L &&
+                    (!a.mask || a.mask[b * a.mask_b + pos * a.mask_l]);
+    const unsigned bits = (unsigned)__ballot(ok);
+    const int N = __popc(bits);
+    total += N;
+    __syncthreads();  // the previous chunk's reads, and lam
+    if (!STATE_ONLY) stage<T, DP, C>(q_s, a.q, b, h, l0, a.Dc, a.vec_c, bits);
+    stage<T, DP, C>(k_s, a.k, b, h, l0, a.Dc, a.vec_c, bits);
+    stage<T, DP, C>(v_s, a.v, b, h, l0, a.De, a.vec_e, bits);
+    if (DERIV && !STATE_ONLY) stage<T, DP, C>(x_s, a.x, b, h, l0, a.De, a.vec_x, bits);
+    __syncthreads();
+    if (e0 >= a.De) continue;
+
+    const int n_i = __popc(bits & ((2u << lo) - 1u));
+    int n_j[4];
+    float vr[4];
+#pragma unroll
+    for (int r = 0; r < 4; ++r) {
+      n_j[r] = __popc(bits & ((2u << (4 * g + r)) - 1u));
+      vr[r] = v_s[(4 * g + r) * LD + e];
+    }
+    if (!STATE_ONLY) {
+      // pair products, transposed: rows j (keys), columns i (queries)
+      f32x4 pt = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+      for (int s = 0; s < DP / 4; ++s)
+        pt = mfma4(k_s[lo * LD + 4 * s + g], q_s[lo * LD + 4 * s + g], pt);
+      f32x4 o = {0.f, 0.f, 0.f, 0.f}, od = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+      for (int t = 0; t < NT; ++t) {
+        const f32x4 qv = *reinterpret_cast<const f32x4*>(q_s + lo * LD + 16 * t + 4 * g);
+#pragma unroll
+        for (int r = 0; r < 4; ++r) {
+          o = mfma4(S[t][r], qv[r], o);
+          if (DERIV) od = mfma4(Sd[t][r], qv[r], od);
+        }
+      }
+      const float w_i = a.c_inter * lam[REV ? N - n_i : n_i];
+      if (DERIV) od = w_i * (od + (float)n_i * o);
+      o = w_i * o;
+#pragma unroll
+      for (int r = 0; r < 4; ++r) {
+        const int j = 4 * g + r;
+        const bool seen = REV ? j >= lo : j <= lo;
+        const int gap = REV ? n_j[r] - n_i : n_i - n_j[r];
+        const float p = seen ? pt[r] * (a.c_pair * lam[seen ? gap : 0]) : 0.f;
+        o = mfma4(vr[r], p, o);
+        if (DERIV) od = mfma4(vr[r], p * (float)(seen ? gap : 0), od);
+      }
+      if (DERIV) {
+        const f32x4 xv = *reinterpret_cast<const f32x4*>(x_s + lo * LD + e0 + 4 * g);
+#pragma unroll
+        for (int r = 0; r < 4; ++r) d_decay += xv[r] * od[r];
+      }
+      if (pos < a.L) {
+        T* row = reinterpret_cast<T*>(a.out) + b * a.out_b + h * a.out_h + (int64_t)pos * a.out_l;
+#pragma unroll
+        for (int r = 0; r < 4; ++r)
+          if (e0 + 4 * g + r < a.De) row[e0 + 4 * g + r] = from_f32<T>(o[r]);
+      }
+    }
+    const float lN = lam[N];
+#pragma unroll
+    for (int t = 0; t < NT; ++t) {
+      if (DERIV) Sd[t] = lN * (Sd[t] + (float)N * S[t]);
+      S[t] = lN * S[t];
+    }
+#pragma unroll
+    for (int r = 0; r < 4; ++r) {
+      const int left = REV ? n_j[r] : N - n_j[r];
+      const float w = vr[r] * (a.c_update * lam[left]);
+#pragma unroll
+      for (int t = 0; t < NT; ++t) {
+        const float kv = k_s[(4 * g + r) * LD + 16 * t + lo];
+        S[t] = mfma4(kv, w, S[t]);
+        if (DERIV) Sd[t] = mfma4(kv, w * (float)left, Sd[t]);
+      }
+    }
+  }
+
+  float* dst = nullptr;
+  float* dst_d = nullptr;
+  const bool at_end = REV ? seg == 0 : seg == a.G - 1;
+  if (STATE_ONLY) {
+    dst = a.seg + (bh * a.G + seg) * state_size;
+    if (DERIV) dst_d = a.seg_d + (bh * a.G + seg) * state_size;
+    if (threadIdx.x == 0) a.seg_count[bh * a.G + seg] = total;
+  } else if (at_end && a.state_out) {
+    dst = a.state_out + bh * state_size;
+  }
+  const float* end_grad = (DERIV && !STATE_ONLY && at_end && a.state_end_grad)
+                              ? a.state_end_grad + bh * state_size : nullptr;
+#pragma unroll
+  for (int t = 0; t < NT; ++t) {
+#pragma unroll
+    for (int r = 0; r < 4; ++r) {
+      const int c = 16 * t + 4 * g + r;
+      if (c < a.Dc && e < a.De) {
+        const int64_t at = c * a.st_c + e * a.st_e;
+        if (dst) dst[at] = S[t][r];
+        if (DERIV && dst_d) dst_d[at] = Sd[t][r];
+        if (DERIV && end_grad) d_decay += Sd[t][r] * end_grad[at];
+      }
+    }
+  }
+  if (DERIV && !STATE_ONLY) {
+    d_decay = wave_reduce_sum(d_decay);
+    if (lane == 0) red[wave] = d_decay;
+    __syncthreads();
+    if (threadIdx.x == 0) {
+      float sum = 0.f;
+      for (int w = 0; w < DP / 16; ++w) sum += red[w];
+      a.decay_part[bh * a.G + seg] = sum;
+    }
+  }
+}
+
+// Contributions of the segments -> start states, in place, one thread for
+// each element of a state.
+template <bool REV, bool DERIV>
+__global__ void la_scan(float* seg, float* seg_d, const int* count, const float* state_in,
+                        const float* log_decay, int H, int G, int64_t state_size) {
+  const int64_t bh = blockIdx.x;
+  const float ld = log_decay[bh % H];
+  for (int64_t at = threadIdx.x + (int64_t)blockIdx.y * blockDim.x; at < state_size;
+       at += (int64_t)gridDim.y * blockDim.x) {
+    float run = state_in ? state_in[bh * state_size + at] : 0.f, run_d = 0.f;
+    for (int s = 0; s < G; ++s) {
+      const int64_t i = bh * G + (REV ? G - 1 - s : s);
+      const int N = count[i];
+      const float lN = N ? expf(ld * N) : 1.f;
+      const float own = seg[i * state_size + at];
+      seg[i * state_size + at] = run;
+      if (DERIV) {
+        const float own_d = seg_d[i * state_size + at];
+        seg_d[i * state_size + at] = run_d;
+        run_d = lN * (run_d + (float)N * run) + own_d;
+      }
+      run = lN * run + own;
+    }
+  }
+}
+
+// decay_part [B, H, G] -> [H]; a fixed order, in 64 bits (the parts may cancel).
+__global__ void la_decay_sum(const float* part, float* out, int B, int H, int G) {
+  __shared__ double red[4];
+  const int h = blockIdx.x;
+  double sum = 0.0;
+  for (int64_t i = threadIdx.x; i < (int64_t)B * G; i += blockDim.x)
+    sum += part[((i / G) * H + h) * G + i % G];
+#pragma unroll
+  for (int off = 32; off > 0; off >>= 1) sum += __shfl_xor(sum, off, WAVE);
+  if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = sum;
+  __syncthreads();
+  if (threadIdx.x == 0) out[h] = (float)(red[0] + red[1] + red[2] + red[3]);
+}
+
+// One position for each row: the state is read, updated and written once.
+template <typename T>
+__global__ void la_step_kernel(Rows q, Rows k, Rows v, const float* log_decay, float* state,
+                               int64_t st_b, int64_t st_h, const bool* active, int64_t act_b,
+                               T* out, int H, int Dk, int Dv, float scale) {
+  const int64_t bh = blockIdx.x;
+  const int b = bh / H, h = bh % H;
+  T* o = out + bh * Dv;
+  if (active && !active[b * act_b]) {
+    for (int e = threadIdx.x; e < Dv; e += blockDim.x) o[e] = from_f32<T>(0.f);
+    return;
+  }
+  const float l = expf(log_decay[h]);
+  const T* qr = reinterpret_cast<const T*>(q.p) + b * q.b + h * q.h;
+  const T* kr = reinterpret_cast<const T*>(k.p) + b * k.b + h * k.h;
+  const T* vr = reinterpret_cast<const T*>(v.p) + b * v.b + h * v.h;
+  float* S = state + b * st_b + h * st_h;
+  for (int e = threadIdx.x; e < Dv; e += blockDim.x) {
+    const float ve = to_f32<T>(vr[e]);
+    float sum = 0.f;
+    for (int c = 0; c < Dk; ++c) {
+      const float s = l * S[(int64_t)c * Dv + e] + to_f32<T>(kr[c]) * ve;
+      S[(int64_t)c * Dv + e] = s;
+      sum += to_f32<T>(qr[c]) * s;
+    }
+    o[e] = from_f32<T>(scale * sum);
+  }
+}
+
+// ---------------------------------------------------------------------------
+
+Rows rows_of(const torch::Tensor& t) {
+  return {t.data_ptr(), t.stride(0), t.stride(1), t.dim() == 4 ? t.stride(2) : 0};
+}
+
+bool vec16(const torch::Tensor& t) {
+  const int64_t v = 16 / t.element_size();
+  if (reinterpret_cast<uintptr_t>(t.data_ptr()) % 16 || t.size(3) % v) return false;
+  for (int i = 0; i < 3; ++i)
+    if (t.size(i) > 1 && t.stride(i) % v) return false;
+  return true;
+}
+
+int padded(int64_t d) { return d <= 32 ? 32 : d <= 64 ? 64 : 128; }
+
+struct Split {
+  int G, seg_chunks;
+};
+
+// One workgroup for each (batch, head) where these alone give every CU two;
+// else the history is cut until there are about that many, in segments of at
+// least 8 chunks so that the state-only pass and the scan stay small beside
+// the work they split.
+Split split_of(int64_t BH, int64_t L, int C) {
+  const int64_t chunks = (L + C - 1) / C;
+  int64_t G = BH ? std::min<int64_t>((512 + BH - 1) / BH, chunks / 8) : 1;
+  G = std::max<int64_t>(G, 1);
+  const int64_t per = std::max<int64_t>((chunks + G - 1) / G, 1);
+  return {(int)std::max<int64_t>((chunks + per - 1) / per, 1), (int)per};
+}
+
+template <typename T, bool REV, bool STATE_ONLY, bool DERIV>
+void launch_pass_t(const PassArgs& a, hipStream_t stream) {
+  const int64_t blocks = (int64_t)a.B * a.H * a.G;
+  TORCH_CHECK(blocks < (int64_t(1) << 31), "linear attention: too many (batch, head, segment)s");
+  const int dp = padded(std::max(a.Dc, a.De));
+#define LA_PASS(DP)                                                                          \
+  hipLaunchKernelGGL((la_pass_f32<T, DP, REV, STATE_ONLY, DERIV>), dim3((unsigned)blocks),   \
+                     dim3(DP * 4), 0, stream, a)
+  if (dp == 32) LA_PASS(32);
+  else if (dp == 64) LA_PASS(64);
+  else LA_PASS(128);
+#undef LA_PASS
+  HIP_CHECK(hipGetLastError());
+}
+
+template <bool REV, bool STATE_ONLY, bool DERIV>
+void launch_pass(torch::ScalarType dt, const PassArgs& a, hipStream_t stream) {
+  if (dt == torch::kBFloat16) launch_pass_t<__hip_bfloat16, REV, STATE_ONLY, DERIV>(a, stream);
+  else if (dt == torch::kHalf) launch_pass_t<__half, REV, STATE_ONLY, DERIV>(a, stream);
+  else launch_pass_t<float, REV, STATE_ONLY, DERIV>(a, stream);
+}
+
+template <bool REV, bool DERIV>
+void launch_scan(const PassArgs& a, const float* state_in, hipStream_t stream) {
+  const int64_t size = (int64_t)a.Dc * a.De;
+  const unsigned y = (unsigned)((size + 255) / 256);
+  hipLaunchKernelGGL((la_scan<REV, DERIV>), dim3((unsigned)(a.B * a.H), y), dim3(256), 0, stream,
+                     a.seg, a.seg_d, a.seg_count, state_in, a.log_decay, a.H, a.G, size);
+  HIP_CHECK(hipGetLastError());
+}
+
+void check_inputs(const torch::Tensor& q, const torch::Tensor& k, const torch::Tensor& v,
+                  const torch::Tensor& log_decay, const c10::optional<torch::Tensor>& mask,
+                  const c10::optional<torch::Tensor>& state, int dim) {
+  const auto dt = q.scalar_type();
+  TORCH_CHECK(q.is_cuda(), "linear attention: q must be on the GPU");
+  TORCH_CHECK(dt == torch::kBFloat16 || dt == torch::kHalf || dt == torch::kFloat32,
+              "linear attention: q, k, v must be bfloat16, float16 or float32");
+  TORCH_CHECK(q.dim() == dim && k.dim() == dim && v.dim() == dim, "linear attention: q, k, v need ",
+              dim, " dimensions");
+  for (const auto& t : {q, k, v}) {
+    TORCH_CHECK(t.scalar_type() == dt && t.device() == q.device(),
+                "linear attention: q, k, v must share type and device");
+    TORCH_CHECK(t.size(-1) <= 1 || t.stride(-1) == 1,
+                "linear attention: the last dimension must be contiguous");
+    for (int i = 0; i < dim - 1; ++i)
+      TORCH_CHECK(t.size(i) == q.size(i), "linear attention: q, k, v differ in dimension ", i);
+  }
+  TORCH_CHECK(k.size(-1) == q.size(-1), "linear attention: q and k differ in head size");
+  TORCH_CHECK(q.size(-1) >= 1 && q.size(-1) <= 128 && v.size(-1) >= 1 && v.size(-1) <= 128,
+              "linear attention: head sizes from 1 to 128");
+  for (int i = 0; i < dim - 1; ++i)
+    TORCH_CHECK(q.size(i) < (int64_t(1) << 31) - 256, "linear attention: dimension ", i, " is too large");
+  TORCH_CHECK(log_decay.dim() == 1 && log_decay.size(0) == q.size(1) && log_decay.is_contiguous() &&
+                  log_decay.scalar_type() == torch::kFloat32 && log_decay.device() == q.device(),
+              "linear attention: log_decay must be float32 [H] on the same device");
+  if (mask.has_value()) {
+    TORCH_CHECK(mask->scalar_type() == torch::kBool && mask->device() == q.device() &&
+                    mask->size(0) == q.size(0) && mask->dim() == dim - 2 &&
+                    (dim == 3 || mask->size(1) == q.size(2)),
+                "linear attention: the mask must be bool over the positions, on the same device");
+  }
+  if (state.has_value()) {
+    TORCH_CHECK(state->scalar_type() == torch::kFloat32 && state->device() == q.device() &&
+                    state->dim() == 4 && state->size(0) == q.size(0) && state->size(1) == q.size(1) &&
+                    state->size(2) == q.size(-1) && state->size(3) == v.size(-1),
+                "linear attention: the state must be float32 [B, H, Dk, Dv] on the same device");
+  }
+}
+
+// [B, L, H, D] memory behind a [B, H, L, D] view: what the next projection
+// reads needs no copy.
+torch::Tensor heads_last(const torch::Tensor& q, int64_t D) {
+  return torch::empty({q.size(0), q.size(2), q.size(1), D}, q.options()).transpose(1, 2);
+}
+
+PassArgs args_of(const torch::Tensor& q, const torch::Tensor& k, const torch::Tensor& v,
+                 const torch::Tensor& log_decay, const c10::optional<torch::Tensor>& mask, bool flip) {
+  PassArgs a = {};
+  a.q = rows_of(q);
+  a.k = rows_of(k);
+  a.v = rows_of(v);
+  a.log_decay = log_decay.data_ptr<float>();
+  if (mask.has_value()) {
+    a.mask = mask->data_ptr<bool>();
+    a.mask_b = mask->stride(0);
+    a.mask_l = mask->stride(1);
+  }
+  a.B = q.size(0);
+  a.H = q.size(1);
+  a.L = q.size(2);
+  a.Dc = q.size(3);
+  a.De = v.size(3);
+  a.vec_c = vec16(q) && vec16(k);
+  a.vec_e = vec16(v);
+  // a state lies in memory as [Dk, Dv]; flipped passes contract over Dv
+  a.st_c = flip ? 1 : a.De;
+  a.st_e = flip ? a.Dc : 1;
+  a.G = 1;
+  return a;
+}
+
+void set_out(PassArgs& a, const torch::Tensor& out) {
+  a.out = out.data_ptr();
+  a.out_b = out.stride(0);
+  a.out_h = out.stride(1);
+  a.out_l = out.stride(2);
+}
+
+}  // namespace
+
+// -> {out, state or empty, start states of the segments or empty}
+std::vector<torch::Tensor> linear_attention_fwd(torch::Tensor q, torch::Tensor k, torch::Tensor v,
+                                                torch::Tensor log_decay,
+                                                c10::optional<torch::Tensor> mask,
+                                                c10::optional<torch::Tensor> state, double scale,
+                                                bool want_state) {
+  check_inputs(q, k, v, log_decay, mask, state, 4);
+  TORCH_CHECK(!state.has_value() || state->is_contiguous(), "linear attention: state not contiguous");
+  const c10::hip::HIPGuardMasqueradingAsCUDA guard(q.device());
+  auto stream = at::cuda::getCurrentHIPStream();
+  const int64_t B = q.size(0), H = q.size(1), L = q.size(2), Dk = q.size(3), Dv = v.size(3);
+  auto f32 = q.options().dtype(torch::kFloat32);
+  auto out = heads_last(q, Dv);
+  auto end = want_state ? torch::empty({B, H, Dk, Dv}, f32) : torch::empty({0}, f32);
+  auto seg = torch::empty({0}, f32);
+  if (B * H == 0) return {out, end, seg};
+
+  PassArgs a = args_of(q, k, v, log_decay, mask, false);
+  set_out(a, out);
+  const Split s = split_of(B * H, L, 16);
+  a.G = s.G;
+  a.seg_chunks = s.seg_chunks;
+  a.state_in = state.has_value() ? state->data_ptr<float>() : nullptr;
+  a.state_out = want_state ? end.data_ptr<float>() : nullptr;
+  a.c_pair = a.c_inter = (float)scale;
+  a.c_update = 1.f;
+  torch::Tensor count;
+  if (a.G > 1) {
+    seg = torch::empty({B, H, a.G, Dk, Dv}, f32);
+    count = torch::empty({B, H, a.G}, q.options().dtype(torch::kInt32));
+    a.seg = seg.data_ptr<float>();
+    a.seg_count = count.data_ptr<int>();
+    launch_pass<false, true, false>(q.scalar_type(), a, stream);
+    launch_scan<false, false>(a, a.state_in, stream);
+  }
+  launch_pass<false, false, false>(q.scalar_type(), a, stream);
+  return {out, end, seg};
+}
+
+// -> {dq, dk, dv, dlog_decay or empty, dstate0 or empty}; seg: what the
+// forward pass returned (start states of the segments), or empty
+std::vector<torch::Tensor> linear_attention_bwd(
+    torch::Tensor q, torch::Tensor k, torch::Tensor v, torch::Tensor log_decay,
+    c10::optional<torch::Tensor> mask, c10::optional<torch::Tensor> state, torch::Tensor dout,
+    c10::optional<torch::Tensor> dstate, torch::Tensor seg, double scale, bool need_decay,
+    bool need_state) {
+  check_inputs(q, k, v, log_decay, mask, state, 4);
+  check_inputs(q, k, dout, log_decay, mask, dstate, 4);
+  TORCH_CHECK(dout.size(3) == v.size(3), "linear attention: dout differs from v in head size");
+  TORCH_CHECK((!state.has_value() || state->is_contiguous()) &&
+                  (!dstate.has_value() || dstate->is_contiguous()),
+              "linear attention: state not contiguous");
+  const c10::hip::HIPGuardMasqueradingAsCUDA guard(q.device());
+  auto stream = at::cuda::getCurrentHIPStream();
+  const int64_t B = q.size(0), H = q.size(1), L = q.size(2), Dk = q.size(3), Dv = v.size(3);
+  const auto dt = q.scalar_type();
+  auto f32 = q.options().dtype(torch::kFloat32);
+  auto dq = heads_last(q, Dk), dk = heads_last(q, Dk), dv = heads_last(q, Dv);
+  auto ddecay = need_decay ? torch::empty({H}, f32) : torch::empty({0}, f32);
+  auto ds0 = need_state ? torch::empty({B, H, Dk, Dv}, f32) : torch::empty({0}, f32);
+  if (B * H == 0) {
+    if (need_decay) ddecay.zero_();
+    return {dq, dk, dv, ddecay, ds0};
+  }
+  const Split s = split_of(B * H, L, 16);
+  const bool split = s.G > 1;
+  TORCH_CHECK(!split || (seg.dim() == 5 && seg.size(2) == s.G && seg.is_contiguous()),
+              "linear attention: the forward pass's segment states are missing");
+  const float* state_in = state.has_value() ? state->data_ptr<float>() : nullptr;
+  const float* dstate_in = dstate.has_value() ? dstate->data_ptr<float>() : nullptr;
+  torch::Tensor count, part, seg_d, seg_r;
+  if (split) count = torch::empty({B, H, s.G}, q.options().dtype(torch::kInt32));
+
+  {  // dq, and the decay's gradient
+    PassArgs a = args_of(dout, v, k, log_decay, mask, true);
+    set_out(a, dq);
+    a.G = s.G;
+    a.seg_chunks = s.seg_chunks;
+    a.state_in = state_in;
+    a.state_end_grad = dstate_in;
+    a.c_pair = a.c_inter = (float)scale;
+    a.c_update = 1.f;
+    a.x = rows_of(q);
+    a.vec_x = vec16(q);
+    if (split) {
+      a.seg = seg.data_ptr<float>();
+      a.seg_count = count.data_ptr<int>();
+    }
+    if (need_decay) {
+      part = torch::empty({B, H, s.G}, f32);
+      a.decay_part = part.data_ptr<float>();
+      if (split) {
+        // S' is linear in what the segments add, so it needs these again;
+        // the start states come out as the forward pass left them
+        auto seg2 = torch::empty_like(seg);
+        seg_d = torch::empty_like(seg);
+        a.seg = seg2.data_ptr<float>();
+        a.seg_d = seg_d.data_ptr<float>();
+        launch_pass<false, true, true>(dt, a, stream);
+        launch_scan<false, true>(a, state_in, stream);
+        launch_pass<false, false, true>(dt, a, stream);
+      } else {
+        launch_pass<false, false, true>(dt, a, stream);
+      }
+      hipLaunchKernelGGL(la_decay_sum, dim3((unsigned)H), dim3(256), 0, stream,
+                         part.data_ptr<float>(), ddecay.data_ptr<float>(), (int)B, (int)H, s.G);
+      HIP_CHECK(hipGetLastError());
+    } else {
+      launch_pass<false, false, false>(dt, a, stream);
+    }
+  }
+  {  // dv, with the state's gradient, then dk
+    PassArgs a = args_of(k, q, dout, log_decay, mask, false);
+    set_out(a, dv);
+    a.G = s.G;
+    a.seg_chunks = s.seg_chunks;
+    a.state_in = dstate_in;
+    a.state_out = need_state ? ds0.data_ptr<float>() : nullptr;
+    a.c_pair = a.c_update = (float)scale;
+    a.c_inter = 1.f;
+    if (split) {
+      seg_r = torch::empty_like(seg);
+      a.seg = seg_r.data_ptr<float>();
+      a.seg_count = count.data_ptr<int>();
+      launch_pass<true, true, false>(dt, a, stream);
+      launch_scan<true, false>(a, dstate_in, stream);
+    }
+    launch_pass<true, false, false>(dt, a, stream);
+    PassArgs c = args_of(v, dout, q, log_decay, mask, true);
+    set_out(c, dk);
+    c.G = s.G;
+    c.seg_chunks = s.seg_chunks;
+    c.state_in = dstate_in;
+    c.seg = a.seg;
+    c.c_pair = c.c_update = (float)scale;
+    c.c_inter = 1.f;
+    launch_pass<true, false, false>(dt, c, stream);
+  }
+  return {dq, dk, dv, ddecay, ds0};
+}
+
+torch::Tensor linear_attention_step(torch::Tensor q, torch::Tensor k, torch::Tensor v,
+                                    torch::Tensor log_decay, torch::Tensor state,
+                                    c10::optional<torch::Tensor> active, double scale) {
+  check_inputs(q, k, v, log_decay, active, state, 3);
+  const int64_t B = q.size(0), H = q.size(1), Dk = q.size(2), Dv = v.size(2);
+  TORCH_CHECK(state.stride(3) == 1 && state.stride(2) == Dv,
+              "linear attention: each head's state must be contiguous");
+  TORCH_CHECK(B * H < (int64_t(1) << 31), "linear attention: too many (batch, head)s");
+  const c10::hip::HIPGuardMasqueradingAsCUDA guard(q.device());
+  auto stream = at::cuda::getCurrentHIPStream();
+  auto out = torch::empty({B, H, Dv}, q.options());
+  if (B * H == 0) return out;
+  const bool* act = active.has_value() ? active->data_ptr<bool>() : nullptr;
+  const int64_t act_b = active.has_value() ? active->stride(0) : 0;
+#define LA_STEP(T)                                                                              \
+  hipLaunchKernelGGL((la_step_kernel<T>), dim3((unsigned)(B * H)), dim3(128), 0, stream,        \
+                     rows_of(q), rows_of(k), rows_of(v), log_decay.data_ptr<float>(),           \
+                     state.data_ptr<float>(), state.stride(0), state.stride(1), act, act_b,     \
+                     reinterpret_cast<T*>(out.data_ptr()), (int)H, (int)Dk, (int)Dv, (float)scale)
+  if (q.scalar_type() == torch::kBFloat16) LA_STEP(__hip_bfloat16);
+  else if (q.scalar_type() == torch::kHalf) LA_STEP(__half);
+  else LA_STEP(float);
+#undef LA_STEP
+  HIP_CHECK(hipGetLastError());
+  return out;
+}
