@@ -283,6 +283,417 @@ __global__ __launch_bounds__(DP * 4) void la_pass_f32(PassArgs a) {
   }
 }
 
+// ---------------------------------------------------------------------------
+// The same pass for bfloat16 on the 16-bit matrix instructions, 64 positions a
+// chunk.  Every contraction of 32 is visited in the order that two accumulator
+// tiles have it, {4g .. 4g+3, 16+4g .. 16+4g+3} for lane group g, so that the
+// pair weights and the state go from one product's result into the next one's
+// operand without leaving the registers.  q, k and the value operand come from
+// row-major LDS tiles, the transposed ones by transposing LDS reads.
+//
+// Each wave computes all pair products for itself: 20 of its 58 matrix
+// instructions a chunk at head size 64, which costs less than sharing them
+// through LDS would, since the card's memory is the bound (64 positions of one
+// head are 32 KB, some 2500 cycles of a CU's share, against 930 of products).
+//
+// Roundings to bfloat16: the pair weights, once (half a step of each term).
+// The state, and the values weighted into it, go in as the sum of two bfloat16
+// (2^-17): what reaches the float32 states is no coarser than their sums.
+
+typedef __attribute__((ext_vector_type(8))) __bf16 bf16x8;
+typedef __attribute__((ext_vector_type(4))) __bf16 bf16x4;
+typedef __attribute__((ext_vector_type(4))) short s16x4;
+
+__device__ __forceinline__ f32x4 mfma32(bf16x8 a, bf16x8 b, f32x4 c) {
+  return __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, b, c, 0, 0, 0);
+}
+
+__device__ __forceinline__ bf16x8 join8(uint2 a, uint2 b) {
+  return __builtin_bit_cast(bf16x8, uint4{a.x, a.y, b.x, b.y});
+}
+
+__device__ __forceinline__ bf16x8 pack8(f32x4 a, f32x4 b) {
+  const bf16x4 x = __builtin_convertvector(a, bf16x4), y = __builtin_convertvector(b, bf16x4);
+  return join8(__builtin_bit_cast(uint2, x), __builtin_bit_cast(uint2, y));
+}
+
+__device__ __forceinline__ f32x4 widen(bf16x4 a) { return __builtin_convertvector(a, f32x4); }
+
+// v = hi + lo to 2^-17
+__device__ __forceinline__ void split8(f32x4 a, f32x4 b, bf16x8& hi, bf16x8& lo) {
+  const bf16x4 x = __builtin_convertvector(a, bf16x4), y = __builtin_convertvector(b, bf16x4);
+  hi = join8(__builtin_bit_cast(uint2, x), __builtin_bit_cast(uint2, y));
+  lo = pack8(a - widen(x), b - widen(y));
+}
+
+// 8 neighbours of a row, of which n exist (all of them unless EDGE); no
+// alignment is asked for
+template <bool EDGE>
+__device__ __forceinline__ uint4 load8(const __hip_bfloat16* p, int n) {
+  alignas(16) __hip_bfloat16 t[8];
+  if (!EDGE || n >= 8) {
+    __builtin_memcpy(t, p, 16);
+  } else {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) t[i] = i < n ? p[i] : __hip_bfloat16(0.f);
+  }
+  return *reinterpret_cast<const uint4*>(t);
+}
+
+template <bool EDGE>
+__device__ __forceinline__ void store8(__hip_bfloat16* p, int n, uint4 v) {
+  if (!EDGE || n >= 8) {
+    __builtin_memcpy(p, &v, 16);
+  } else {
+    alignas(16) __hip_bfloat16 t[8];
+    *reinterpret_cast<uint4*>(t) = v;
+#pragma unroll
+    for (int i = 0; i < 8; ++i)
+      if (i < n) p[i] = t[i];
+  }
+}
+
+// One operand's 64 positions on their way from memory to LDS, two 16-byte
+// pieces a thread: rows row and row + 32 of the chunk, columns d .. d + 7.
+template <int DP, bool EDGE>
+struct Chunk {
+  static constexpr int C = 64, NT = DP * 4;
+  // rows 16 bytes apart from a power of two: the fragment reads of 16 rows
+  // then start in banks 4 words apart
+  static constexpr int LD = DP * 2 + 16, BYTES = C * LD;
+
+  const __hip_bfloat16* at;  // this thread's first piece of position 0
+  int64_t l;
+  int left;                  // columns from d on that exist
+  uint4 r[2];
+
+  __device__ __forceinline__ Chunk(const Rows& src, int b, int h, int D) {
+    const int d = (threadIdx.x % (DP / 8)) * 8;
+    l = src.l;
+    left = D - d;
+    at = reinterpret_cast<const __hip_bfloat16*>(src.p) + b * src.b + h * src.h +
+         (threadIdx.x / (DP / 8)) * l + d;
+  }
+  __device__ __forceinline__ void fetch(int l0, uint64_t bits) {
+    const uint64_t mine = bits >> (threadIdx.x / (DP / 8));
+    r[0] = r[1] = uint4{0, 0, 0, 0};
+    if ((mine & 1) && left > 0) r[0] = load8<EDGE>(at + l0 * l, left);
+    if (((mine >> 32) & 1) && left > 0) r[1] = load8<EDGE>(at + (l0 + 32) * l, left);
+  }
+  __device__ __forceinline__ void put(char* dst) const {
+    dst += (threadIdx.x / (DP / 8)) * LD + (threadIdx.x % (DP / 8)) * 16;
+    *reinterpret_cast<uint4*>(dst) = r[0];
+    *reinterpret_cast<uint4*>(dst + 32 * LD) = r[1];
+  }
+  // operand rows row0 + (lane & 15), contraction block s of the head size
+  static __device__ __forceinline__ bf16x8 rows(const char* t, int row0, int s, int lo, int g) {
+    const char* p = t + (row0 + lo) * LD + s * 64 + g * 8;
+    return join8(*reinterpret_cast<const uint2*>(p), *reinterpret_cast<const uint2*>(p + 32));
+  }
+  // operand columns col0 + (lane & 15), contraction block s of the positions
+  static __device__ __forceinline__ bf16x8 columns(const char* t, int col0, int s, int lo, int g) {
+    uint2 half[2];
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      const char* p = t + (32 * s + 16 * i + 4 * g + (lo >> 2)) * LD + col0 * 2 + (lo & 3) * 8;
+      auto v = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s16x4*)p);
+      half[i] = __builtin_bit_cast(uint2, v);
+    }
+    return join8(half[0], half[1]);
+  }
+};
+
+template <int DP, bool REV, bool STATE_ONLY, bool DERIV, bool EDGE>
+__global__ __launch_bounds__(DP * 4, 2) void la_pass_bf16(PassArgs a) {
+  using Ch = Chunk<DP, EDGE>;
+  constexpr int C = 64, NS = DP / 32, NT = DP / 16, LD = Ch::LD;
+  constexpr int WAVES = DP / 16;
+  constexpr bool FULL = !STATE_ONLY, X = DERIV && FULL;
+  __shared__ __attribute__((aligned(16))) char q_s[FULL ? Ch::BYTES : 16];
+  __shared__ __attribute__((aligned(16))) char k_s[Ch::BYTES];
+  __shared__ __attribute__((aligned(16))) char v_s[Ch::BYTES];
+  __shared__ __attribute__((aligned(16))) char o_s[FULL ? Ch::BYTES : 16];
+  __shared__ __attribute__((aligned(16))) char x_s[X ? Ch::BYTES : 16];
+  __shared__ __attribute__((aligned(16))) float n_s[C];  // valid positions up to each
+  __shared__ float lam[C + 1];
+  __shared__ float red[WAVES];
+
+  const int seg = blockIdx.x % a.G;
+  const int64_t bh = blockIdx.x / a.G;
+  const int b = bh / a.H, h = bh % a.H;
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  const int lo = lane & 15, g = lane >> 4;
+  const int e0 = wave * 16, e = e0 + lo;
+  const bool busy = e0 < a.De;
+  const int64_t state_size = (int64_t)a.Dc * a.De;
+  const float ld = a.log_decay[h];
+  // a decay of zero (log -inf) keeps l^0 = 1
+  for (int i = threadIdx.x; i <= C; i += Ch::NT) lam[i] = i ? expf(ld * i) : 1.f;
+
+  f32x4 S[NT], Sd[DERIV ? NT : 1];
+  {
+    const float* src = nullptr;
+    const float* src_d = nullptr;
+    if (FULL) {
+      if (a.G > 1) {
+        src = a.seg + (bh * a.G + seg) * state_size;
+        if (DERIV) src_d = a.seg_d + (bh * a.G + seg) * state_size;
+      } else if (a.state_in) {
+        src = a.state_in + bh * state_size;
+      }
+    }
+#pragma unroll
+    for (int t = 0; t < NT; ++t) {
+#pragma unroll
+      for (int r = 0; r < 4; ++r) {
+        const int c = 16 * t + 4 * g + r;
+        const bool in = c < a.Dc && e < a.De;
+        S[t][r] = (src && in) ? src[c * a.st_c + e * a.st_e] : 0.f;
+        if (DERIV) Sd[t][r] = (src_d && in) ? src_d[c * a.st_c + e * a.st_e] : 0.f;
+      }
+    }
+  }
+  __syncthreads();  // lam
+
+  // The pair weights of a chunk without gaps: on the diagonal tiles, on the
+  // next ones, and what each further tile multiplies these by.
+  f32x4 on_diagonal, off_diagonal;
+  const float lam16 = lam[16];
+  if (FULL) {
+#pragma unroll
+    for (int r = 0; r < 4; ++r) {
+      const int gap = REV ? 4 * g + r - lo : lo - 4 * g - r;
+      on_diagonal[r] = gap >= 0 ? a.c_pair * lam[max(gap, 0)] : 0.f;
+      off_diagonal[r] = a.c_pair * lam[gap + 16];
+    }
+  }
+
+  const int n_chunks = (a.L + C - 1) / C;
+  const int first = seg * a.seg_chunks, last = min(n_chunks, first + a.seg_chunks);
+  auto start_of = [&](int step) { return (REV ? first + last - 1 - step : step) * C; };
+  int total = 0;
+  float d_decay = 0.f;
+  Ch q_r(a.q, b, h, a.Dc), k_r(a.k, b, h, a.Dc), v_r(a.v, b, h, a.De), x_r(a.x, b, h, a.De);
+  // The mask is read a chunk ahead of the rows that it says to read.
+  const bool* mask = a.mask ? a.mask + b * a.mask_b : nullptr;
+  auto look = [&](int step) {
+    const int pos = start_of(step) + lane;
+    return step < last && pos < a.L && (!mask || mask[pos * a.mask_l]);
+  };
+  auto fetch = [&](int step, uint64_t bits) {
+    const int l0 = start_of(step);
+    if (FULL) q_r.fetch(l0, bits);
+    k_r.fetch(l0, bits);
+    v_r.fetch(l0, bits);
+    if (X) x_r.fetch(l0, bits);
+  };
+  __hip_bfloat16* out = nullptr;
+  if (FULL)
+    out = reinterpret_cast<__hip_bfloat16*>(a.out) + b * a.out_b + h * a.out_h +
+          (threadIdx.x / (DP / 8)) * a.out_l + (threadIdx.x % (DP / 8)) * 8;
+  // outputs of the chunk at l0 in whole rows, from LDS or zeros
+  auto store = [&](int l0, bool zero) {
+    const int row = threadIdx.x / (DP / 8), left = v_r.left;
+    const char* from = o_s + row * LD + (threadIdx.x % (DP / 8)) * 16;
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      if (l0 + row + 32 * i >= a.L || left <= 0) continue;
+      uint4 v = {0, 0, 0, 0};
+      if (!zero) v = *reinterpret_cast<const uint4*>(from + 32 * i * LD);
+      store8<EDGE>(out + (l0 + 32 * i) * a.out_l, left, v);
+    }
+  };
+
+  uint64_t bits = __ballot(look(first));
+  fetch(first, bits);
+  bool ahead = look(first + 1);
+#pragma unroll 1
+  for (int step = first; step < last; ++step) {
+    const int l0 = start_of(step);
+    const uint64_t now = bits;
+    const int N = __popcll(now);
+    total += N;
+    if (N == 0) {  // nothing is seen, added or forgotten
+      if (FULL) store(l0, true);
+      bits = __ballot(ahead);
+      fetch(step + 1, bits);
+      ahead = look(step + 2);
+      continue;
+    }
+    if (FULL) q_r.put(q_s);
+    k_r.put(k_s);
+    v_r.put(v_s);
+    if (X) x_r.put(x_s);
+    if (wave == 0) n_s[lane] = (float)__popcll(now & ((2ull << lane) - 1));
+    __syncthreads();
+    bits = __ballot(ahead);
+    fetch(step + 1, bits);
+    ahead = look(step + 2);
+
+    if (busy) {
+      bf16x8 vf[2];
+#pragma unroll
+      for (int s = 0; s < 2; ++s) vf[s] = Ch::columns(v_s, e0, s, lo, g);
+      const float all = (float)N;
+
+      if (FULL) {
+        const bool whole = now == ~0ull;
+        bf16x8 s_hi[NS], s_lo[NS], d_hi[DERIV ? NS : 1], d_lo[DERIV ? NS : 1];
+#pragma unroll
+        for (int s = 0; s < NS; ++s) {
+          split8(S[2 * s], S[2 * s + 1], s_hi[s], s_lo[s]);
+          if (DERIV) split8(Sd[2 * s], Sd[2 * s + 1], d_hi[s], d_lo[s]);
+        }
+#pragma unroll 1
+        for (int it = 0; it < 4; ++it) {
+          bf16x8 qf[NS];
+#pragma unroll
+          for (int s = 0; s < NS; ++s) qf[s] = Ch::rows(q_s, 16 * it, s, lo, g);
+          f32x4 o = {0.f, 0.f, 0.f, 0.f}, od = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+          for (int s = 0; s < NS; ++s) {
+            o = mfma32(s_lo[s], qf[s], o);
+            o = mfma32(s_hi[s], qf[s], o);
+            if (DERIV) {
+              od = mfma32(d_lo[s], qf[s], od);
+              od = mfma32(d_hi[s], qf[s], od);
+            }
+          }
+          const int i = 16 * it + lo;
+          const float n_i = n_s[i];
+          const float w_i = a.c_inter * lam[(int)(REV ? all - n_i : n_i)];
+          if (DERIV) {
+            od = w_i * (od + n_i * o);
+            const f32x4 xv = widen(*reinterpret_cast<const bf16x4*>(x_s + i * LD + (e0 + 4 * g) * 2));
+#pragma unroll
+            for (int r = 0; r < 4; ++r) d_decay += xv[r] * od[r];
+          }
+          o = w_i * o;
+          // pairs with the keys of tiles 2 s and 2 s + 1
+#pragma unroll 1
+          for (int s = REV ? it >> 1 : 0; s <= (REV ? 1 : it >> 1); ++s) {
+            f32x4 p[2];
+#pragma unroll
+            for (int u = 0; u < 2; ++u) {
+              const int jt = 2 * s + u, apart = REV ? jt - it : it - jt;
+              p[u] = f32x4{0.f, 0.f, 0.f, 0.f};
+              if (apart < 0) continue;
+              f32x4 acc = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+              for (int c = 0; c < NS; ++c) acc = mfma32(Ch::rows(k_s, 16 * jt, c, lo, g), qf[c], acc);
+              f32x4 gaps;
+              if (DERIV || !whole) {
+                const f32x4 n_j = *reinterpret_cast<const f32x4*>(n_s + 16 * jt + 4 * g);
+                gaps = REV ? n_j - n_i : n_i - n_j;
+              }
+              if (whole) {
+                f32x4 w = on_diagonal;
+                if (apart > 0) w = off_diagonal;
+                if (apart > 1) w = w * lam16;
+                if (apart > 2) w = w * lam16;
+                p[u] = acc * w;
+              } else {
+#pragma unroll
+                for (int r = 0; r < 4; ++r) {
+                  const int j = 16 * jt + 4 * g + r;
+                  const bool seen = REV ? j >= i : j <= i;
+                  p[u][r] = seen ? acc[r] * (a.c_pair * lam[seen ? (int)gaps[r] : 0]) : 0.f;
+                }
+              }
+              if (DERIV) {
+                // sum of gap weight (q_i.k_j) (x_i.v_j): each tile by one wave
+                if ((4 * it + jt) % ((a.De + 15) / 16) == wave) {
+                  f32x4 other = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+                  for (int c = 0; c < NS; ++c)
+                    other = mfma32(Ch::rows(v_s, 16 * jt, c, lo, g), Ch::rows(x_s, 16 * it, c, lo, g), other);
+#pragma unroll
+                  for (int r = 0; r < 4; ++r) d_decay += p[u][r] * gaps[r] * other[r];
+                }
+              }
+            }
+            o = mfma32(s ? vf[1] : vf[0], pack8(p[0], p[1]), o);
+          }
+          *reinterpret_cast<bf16x4*>(o_s + i * LD + (e0 + 4 * g) * 2) = __builtin_convertvector(o, bf16x4);
+        }
+      }
+
+      const float lN = lam[N];
+#pragma unroll
+      for (int t = 0; t < NT; ++t) {
+        if (DERIV) Sd[t] = lN * (Sd[t] + all * S[t]);
+        S[t] = lN * S[t];
+      }
+#pragma unroll
+      for (int s = 0; s < 2; ++s) {
+        f32x4 w[2], wd[2];
+        const uint4 raw = __builtin_bit_cast(uint4, vf[s]);
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+          const f32x4 val = widen(__builtin_bit_cast(bf16x4, i ? uint2{raw.z, raw.w} : uint2{raw.x, raw.y}));
+          const f32x4 n_j = *reinterpret_cast<const f32x4*>(n_s + 32 * s + 16 * i + 4 * g);
+#pragma unroll
+          for (int r = 0; r < 4; ++r) {
+            const float left = REV ? n_j[r] : all - n_j[r];
+            w[i][r] = val[r] * (a.c_update * lam[(int)left]);
+            if (DERIV) wd[i][r] = w[i][r] * left;
+          }
+        }
+        bf16x8 w_hi, w_lo, wd_hi, wd_lo;
+        split8(w[0], w[1], w_hi, w_lo);
+        if (DERIV) split8(wd[0], wd[1], wd_hi, wd_lo);
+#pragma unroll
+        for (int t = 0; t < NT; ++t) {
+          const bf16x8 kf = Ch::columns(k_s, 16 * t, s, lo, g);
+          S[t] = mfma32(kf, w_lo, S[t]);
+          S[t] = mfma32(kf, w_hi, S[t]);
+          if (DERIV) {
+            Sd[t] = mfma32(kf, wd_lo, Sd[t]);
+            Sd[t] = mfma32(kf, wd_hi, Sd[t]);
+          }
+        }
+      }
+    }
+    __syncthreads();  // the chunk is read and its outputs are in LDS
+    if (FULL) store(l0, false);
+  }
+
+  float* dst = nullptr;
+  float* dst_d = nullptr;
+  const bool at_end = REV ? seg == 0 : seg == a.G - 1;
+  if (STATE_ONLY) {
+    dst = a.seg + (bh * a.G + seg) * state_size;
+    if (DERIV) dst_d = a.seg_d + (bh * a.G + seg) * state_size;
+    if (threadIdx.x == 0) a.seg_count[bh * a.G + seg] = total;
+  } else if (at_end && a.state_out) {
+    dst = a.state_out + bh * state_size;
+  }
+  const float* end_grad = (X && at_end && a.state_end_grad) ? a.state_end_grad + bh * state_size : nullptr;
+#pragma unroll
+  for (int t = 0; t < NT; ++t) {
+#pragma unroll
+    for (int r = 0; r < 4; ++r) {
+      const int c = 16 * t + 4 * g + r;
+      if (c < a.Dc && e < a.De) {
+        const int64_t at = c * a.st_c + e * a.st_e;
+        if (dst) dst[at] = S[t][r];
+        if (DERIV && dst_d) dst_d[at] = Sd[t][r];
+        if (DERIV && end_grad) d_decay += Sd[t][r] * end_grad[at];
+      }
+    }
+  }
+  if (X) {
+    d_decay = wave_reduce_sum(d_decay);
+    if (lane == 0) red[wave] = d_decay;
+    __syncthreads();
+    if (threadIdx.x == 0) {
+      float sum = 0.f;
+      for (int w = 0; w < WAVES; ++w) sum += red[w];
+      a.decay_part[bh * a.G + seg] = sum;
+    }
+  }
+}
+
 // Contributions of the segments -> start states, in place, one thread for
 // each element of a state.
 template <bool REV, bool DERIV>
@@ -372,38 +783,43 @@ struct Split {
   int G, seg_chunks;
 };
 
+// Positions of a chunk: bfloat16's pass takes 64; float16 shares float32's (its
+// range does not hold a state that long histories add up to).
+int chunk_of(torch::ScalarType dt) { return dt == torch::kBFloat16 ? 64 : 16; }
+
 // One workgroup for each (batch, head) where these alone give every CU two;
 // else the history is cut until there are about that many, in segments of at
-// least 8 chunks so that the state-only pass and the scan stay small beside
-// the work they split.
+// least 256 positions so that the state-only pass and the scan stay small
+// beside the work they split.
 Split split_of(int64_t BH, int64_t L, int C) {
   const int64_t chunks = (L + C - 1) / C;
-  int64_t G = BH ? std::min<int64_t>((512 + BH - 1) / BH, chunks / 8) : 1;
+  int64_t G = BH ? std::min<int64_t>((512 + BH - 1) / BH, chunks * C / 256) : 1;
   G = std::max<int64_t>(G, 1);
   const int64_t per = std::max<int64_t>((chunks + G - 1) / G, 1);
   return {(int)std::max<int64_t>((chunks + per - 1) / per, 1), (int)per};
 }
 
-template <typename T, bool REV, bool STATE_ONLY, bool DERIV>
-void launch_pass_t(const PassArgs& a, hipStream_t stream) {
+template <bool REV, bool STATE_ONLY, bool DERIV>
+void launch_pass(torch::ScalarType dt, const PassArgs& a, hipStream_t stream) {
   const int64_t blocks = (int64_t)a.B * a.H * a.G;
   TORCH_CHECK(blocks < (int64_t(1) << 31), "linear attention: too many (batch, head, segment)s");
   const int dp = padded(std::max(a.Dc, a.De));
+  const bool edge = a.Dc % 8 || a.De % 8;
+#define LA_LAUNCH(DP, ...)                                                                   \
+  hipLaunchKernelGGL((__VA_ARGS__), dim3((unsigned)blocks), dim3(DP * 4), 0, stream, a)
 #define LA_PASS(DP)                                                                          \
-  hipLaunchKernelGGL((la_pass_f32<T, DP, REV, STATE_ONLY, DERIV>), dim3((unsigned)blocks),   \
-                     dim3(DP * 4), 0, stream, a)
+  do {                                                                                       \
+    if (dt == torch::kBFloat16 && edge) LA_LAUNCH(DP, la_pass_bf16<DP, REV, STATE_ONLY, DERIV, true>); \
+    else if (dt == torch::kBFloat16) LA_LAUNCH(DP, la_pass_bf16<DP, REV, STATE_ONLY, DERIV, false>); \
+    else if (dt == torch::kHalf) LA_LAUNCH(DP, la_pass_f32<__half, DP, REV, STATE_ONLY, DERIV>); \
+    else LA_LAUNCH(DP, la_pass_f32<float, DP, REV, STATE_ONLY, DERIV>);                      \
+  } while (0)
   if (dp == 32) LA_PASS(32);
   else if (dp == 64) LA_PASS(64);
   else LA_PASS(128);
 #undef LA_PASS
+#undef LA_LAUNCH
   HIP_CHECK(hipGetLastError());
-}
-
-template <bool REV, bool STATE_ONLY, bool DERIV>
-void launch_pass(torch::ScalarType dt, const PassArgs& a, hipStream_t stream) {
-  if (dt == torch::kBFloat16) launch_pass_t<__hip_bfloat16, REV, STATE_ONLY, DERIV>(a, stream);
-  else if (dt == torch::kHalf) launch_pass_t<__half, REV, STATE_ONLY, DERIV>(a, stream);
-  else launch_pass_t<float, REV, STATE_ONLY, DERIV>(a, stream);
 }
 
 template <bool REV, bool DERIV>
@@ -514,7 +930,7 @@ std::vector<torch::Tensor> linear_attention_fwd(torch::Tensor q, torch::Tensor k
 
   PassArgs a = args_of(q, k, v, log_decay, mask, false);
   set_out(a, out);
-  const Split s = split_of(B * H, L, 16);
+  const Split s = split_of(B * H, L, chunk_of(q.scalar_type()));
   a.G = s.G;
   a.seg_chunks = s.seg_chunks;
   a.state_in = state.has_value() ? state->data_ptr<float>() : nullptr;
@@ -559,7 +975,7 @@ std::vector<torch::Tensor> linear_attention_bwd(
     if (need_decay) ddecay.zero_();
     return {dq, dk, dv, ddecay, ds0};
   }
-  const Split s = split_of(B * H, L, 16);
+  const Split s = split_of(B * H, L, chunk_of(q.scalar_type()));
   const bool split = s.G > 1;
   TORCH_CHECK(!split || (seg.dim() == 5 && seg.size(2) == s.G && seg.is_contiguous()),
               "linear attention: the forward pass's segment states are missing");
