@@ -285,11 +285,12 @@ __global__ __launch_bounds__(DP * 4) void la_pass_f32(PassArgs a) {
 
 // ---------------------------------------------------------------------------
 // The same pass for bfloat16 on the 16-bit matrix instructions, 64 positions a
-// chunk.  Every contraction of 32 is visited in the order that two accumulator
-// tiles have it, {4g .. 4g+3, 16+4g .. 16+4g+3} for lane group g, so that the
-// pair weights and the state go from one product's result into the next one's
-// operand without leaving the registers.  q, k and the value operand come from
-// row-major LDS tiles, the transposed ones by transposing LDS reads.
+// chunk.  Pair weights and states go from one product's result into the next
+// one's operand without leaving the registers: a contraction over positions is
+// visited in the order that two accumulator tiles have it, {4g .. 4g+3,
+// 16+4g .. 16+4g+3} for lane group g; one over the head size in memory's order,
+// 8g .. 8g+7, to which the rows of the state's tiles are permuted.  Everything
+// comes from row-major LDS tiles, the transposed operands by transposing reads.
 //
 // Each wave computes all pair products for itself: 20 of its 58 matrix
 // instructions a chunk at head size 64, which costs less than sharing them
@@ -387,15 +388,15 @@ struct Chunk {
   }
   // operand rows row0 + (lane & 15), contraction block s of the head size
   static __device__ __forceinline__ bf16x8 rows(const char* t, int row0, int s, int lo, int g) {
-    const char* p = t + (row0 + lo) * LD + s * 64 + g * 8;
-    return join8(*reinterpret_cast<const uint2*>(p), *reinterpret_cast<const uint2*>(p + 32));
+    return *reinterpret_cast<const bf16x8*>(t + (row0 + lo) * LD + s * 64 + g * 16);
   }
-  // operand columns col0 + (lane & 15), contraction block s of the positions
-  static __device__ __forceinline__ bf16x8 columns(const char* t, int col0, int s, int lo, int g) {
+  // operand columns, contraction block s of the positions: col0 + (lane & 15),
+  // or, for tile t of the state, state_row(t, .) of it
+  static __device__ __forceinline__ bf16x8 columns(const char* t, int col0, int apart, int s, int lo, int g) {
     uint2 half[2];
 #pragma unroll
     for (int i = 0; i < 2; ++i) {
-      const char* p = t + (32 * s + 16 * i + 4 * g + (lo >> 2)) * LD + col0 * 2 + (lo & 3) * 8;
+      const char* p = t + (32 * s + 16 * i + 4 * g + (lo >> 2)) * LD + col0 * 2 + (lo & 3) * apart * 2;
       auto v = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s16x4*)p);
       half[i] = __builtin_bit_cast(uint2, v);
     }
@@ -403,8 +404,13 @@ struct Chunk {
   }
 };
 
+// The contraction index of row 4 g + r of the state's tile t.
+__device__ __forceinline__ int state_row(int t, int g, int r) {
+  return 32 * (t >> 1) + 8 * g + 4 * (t & 1) + r;
+}
+
 template <int DP, bool REV, bool STATE_ONLY, bool DERIV, bool EDGE>
-__global__ __launch_bounds__(DP * 4, 2) void la_pass_bf16(PassArgs a) {
+__global__ __launch_bounds__(DP * 4, DP == 128 || DERIV ? 2 : 3) void la_pass_bf16(PassArgs a) {
   using Ch = Chunk<DP, EDGE>;
   constexpr int C = 64, NS = DP / 32, NT = DP / 16, LD = Ch::LD;
   constexpr int WAVES = DP / 16;
@@ -414,7 +420,9 @@ __global__ __launch_bounds__(DP * 4, 2) void la_pass_bf16(PassArgs a) {
   __shared__ __attribute__((aligned(16))) char v_s[Ch::BYTES];
   __shared__ __attribute__((aligned(16))) char o_s[FULL ? Ch::BYTES : 16];
   __shared__ __attribute__((aligned(16))) char x_s[X ? Ch::BYTES : 16];
-  __shared__ __attribute__((aligned(16))) float n_s[C];  // valid positions up to each
+  // of each position: the valid ones up to it, and its weights in the product
+  // with the start state and in the state's update
+  __shared__ __attribute__((aligned(16))) float n_s[C], inter_s[C], update_s[C];
   __shared__ float lam[C + 1];
   __shared__ float red[WAVES];
 
@@ -446,7 +454,7 @@ __global__ __launch_bounds__(DP * 4, 2) void la_pass_bf16(PassArgs a) {
     for (int t = 0; t < NT; ++t) {
 #pragma unroll
       for (int r = 0; r < 4; ++r) {
-        const int c = 16 * t + 4 * g + r;
+        const int c = state_row(t, g, r);
         const bool in = c < a.Dc && e < a.De;
         S[t][r] = (src && in) ? src[c * a.st_c + e * a.st_e] : 0.f;
         if (DERIV) Sd[t][r] = (src_d && in) ? src_d[c * a.st_c + e * a.st_e] : 0.f;
@@ -455,16 +463,16 @@ __global__ __launch_bounds__(DP * 4, 2) void la_pass_bf16(PassArgs a) {
   }
   __syncthreads();  // lam
 
-  // The pair weights of a chunk without gaps: on the diagonal tiles, on the
-  // next ones, and what each further tile multiplies these by.
-  f32x4 on_diagonal, off_diagonal;
-  const float lam16 = lam[16];
+  // The pair weights of a chunk without gaps, by the distance of the tiles.
+  f32x4 full[FULL ? 4 : 1];
   if (FULL) {
 #pragma unroll
-    for (int r = 0; r < 4; ++r) {
-      const int gap = REV ? 4 * g + r - lo : lo - 4 * g - r;
-      on_diagonal[r] = gap >= 0 ? a.c_pair * lam[max(gap, 0)] : 0.f;
-      off_diagonal[r] = a.c_pair * lam[gap + 16];
+    for (int d = 0; d < 4; ++d) {
+#pragma unroll
+      for (int r = 0; r < 4; ++r) {
+        const int gap = 16 * d + (REV ? 4 * g + r - lo : lo - 4 * g - r);
+        full[d][r] = gap >= 0 ? a.c_pair * lam[max(gap, 0)] : 0.f;
+      }
     }
   }
 
@@ -524,7 +532,12 @@ __global__ __launch_bounds__(DP * 4, 2) void la_pass_bf16(PassArgs a) {
     k_r.put(k_s);
     v_r.put(v_s);
     if (X) x_r.put(x_s);
-    if (wave == 0) n_s[lane] = (float)__popcll(now & ((2ull << lane) - 1));
+    if (wave == 0) {
+      const int n = __popcll(now & ((2ull << lane) - 1));
+      n_s[lane] = (float)n;
+      inter_s[lane] = a.c_inter * lam[REV ? N - n : n];
+      update_s[lane] = a.c_update * lam[REV ? n : N - n];
+    }
     __syncthreads();
     bits = __ballot(ahead);
     fetch(step + 1, bits);
@@ -533,35 +546,43 @@ __global__ __launch_bounds__(DP * 4, 2) void la_pass_bf16(PassArgs a) {
     if (busy) {
       bf16x8 vf[2];
 #pragma unroll
-      for (int s = 0; s < 2; ++s) vf[s] = Ch::columns(v_s, e0, s, lo, g);
+      for (int s = 0; s < 2; ++s) vf[s] = Ch::columns(v_s, e0, 4, s, lo, g);
       const float all = (float)N;
 
       if (FULL) {
         const bool whole = now == ~0ull;
-        bf16x8 s_hi[NS], s_lo[NS], d_hi[DERIV ? NS : 1], d_lo[DERIV ? NS : 1];
+        // the start state's part, a block of the contraction at a time: so the
+        // split state needs registers for one block only
+        f32x4 os[4] = {}, ods[DERIV ? 4 : 1] = {};
 #pragma unroll
         for (int s = 0; s < NS; ++s) {
-          split8(S[2 * s], S[2 * s + 1], s_hi[s], s_lo[s]);
-          if (DERIV) split8(Sd[2 * s], Sd[2 * s + 1], d_hi[s], d_lo[s]);
+          asm volatile("" ::: "memory");
+          bf16x8 s_hi, s_lo, d_hi, d_lo;
+          split8(S[2 * s], S[2 * s + 1], s_hi, s_lo);
+          if (DERIV) split8(Sd[2 * s], Sd[2 * s + 1], d_hi, d_lo);
+#pragma unroll
+          for (int it = 0; it < 4; ++it) {
+            const bf16x8 qf = Ch::rows(q_s, 16 * it, s, lo, g);
+            os[it] = mfma32(s_lo, qf, os[it]);
+            os[it] = mfma32(s_hi, qf, os[it]);
+            if (DERIV) {
+              ods[it] = mfma32(d_lo, qf, ods[it]);
+              ods[it] = mfma32(d_hi, qf, ods[it]);
+            }
+          }
         }
-#pragma unroll 1
+#pragma unroll
         for (int it = 0; it < 4; ++it) {
+          // one tile row at a time: overlapped, they need more registers than
+          // leaves three workgroups a CU
+          asm volatile("" ::: "memory");
           bf16x8 qf[NS];
 #pragma unroll
           for (int s = 0; s < NS; ++s) qf[s] = Ch::rows(q_s, 16 * it, s, lo, g);
-          f32x4 o = {0.f, 0.f, 0.f, 0.f}, od = {0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-          for (int s = 0; s < NS; ++s) {
-            o = mfma32(s_lo[s], qf[s], o);
-            o = mfma32(s_hi[s], qf[s], o);
-            if (DERIV) {
-              od = mfma32(d_lo[s], qf[s], od);
-              od = mfma32(d_hi[s], qf[s], od);
-            }
-          }
+          f32x4 o = os[it], od;
+          if (DERIV) od = ods[it];
           const int i = 16 * it + lo;
-          const float n_i = n_s[i];
-          const float w_i = a.c_inter * lam[(int)(REV ? all - n_i : n_i)];
+          const float n_i = n_s[i], w_i = inter_s[i];
           if (DERIV) {
             od = w_i * (od + n_i * o);
             const f32x4 xv = widen(*reinterpret_cast<const bf16x4*>(x_s + i * LD + (e0 + 4 * g) * 2));
@@ -570,8 +591,9 @@ __global__ __launch_bounds__(DP * 4, 2) void la_pass_bf16(PassArgs a) {
           }
           o = w_i * o;
           // pairs with the keys of tiles 2 s and 2 s + 1
-#pragma unroll 1
-          for (int s = REV ? it >> 1 : 0; s <= (REV ? 1 : it >> 1); ++s) {
+#pragma unroll
+          for (int s = 0; s < 2; ++s) {
+            if (REV ? 2 * s + 1 < it : 2 * s > it) continue;
             f32x4 p[2];
 #pragma unroll
             for (int u = 0; u < 2; ++u) {
@@ -587,17 +609,16 @@ __global__ __launch_bounds__(DP * 4, 2) void la_pass_bf16(PassArgs a) {
                 gaps = REV ? n_j - n_i : n_i - n_j;
               }
               if (whole) {
-                f32x4 w = on_diagonal;
-                if (apart > 0) w = off_diagonal;
-                if (apart > 1) w = w * lam16;
-                if (apart > 2) w = w * lam16;
-                p[u] = acc * w;
+                p[u] = acc * full[apart < 0 ? 0 : apart];
               } else {
+                f32x4 w;
+#pragma unroll
+                for (int r = 0; r < 4; ++r) w[r] = lam[max((int)gaps[r], 0)];
 #pragma unroll
                 for (int r = 0; r < 4; ++r) {
-                  const int j = 16 * jt + 4 * g + r;
-                  const bool seen = REV ? j >= i : j <= i;
-                  p[u][r] = seen ? acc[r] * (a.c_pair * lam[seen ? (int)gaps[r] : 0]) : 0.f;
+                  const int j = 4 * g + r;
+                  const bool seen = apart > 0 || (REV ? j >= lo : j <= lo);
+                  p[u][r] = seen ? acc[r] * (a.c_pair * w[r]) : 0.f;
                 }
               }
               if (DERIV) {
@@ -612,7 +633,7 @@ __global__ __launch_bounds__(DP * 4, 2) void la_pass_bf16(PassArgs a) {
                 }
               }
             }
-            o = mfma32(s ? vf[1] : vf[0], pack8(p[0], p[1]), o);
+            o = mfma32(vf[s], pack8(p[0], p[1]), o);
           }
           *reinterpret_cast<bf16x4*>(o_s + i * LD + (e0 + 4 * g) * 2) = __builtin_convertvector(o, bf16x4);
         }
@@ -626,17 +647,17 @@ __global__ __launch_bounds__(DP * 4, 2) void la_pass_bf16(PassArgs a) {
       }
 #pragma unroll
       for (int s = 0; s < 2; ++s) {
+        asm volatile("" ::: "memory");
         f32x4 w[2], wd[2];
         const uint4 raw = __builtin_bit_cast(uint4, vf[s]);
 #pragma unroll
         for (int i = 0; i < 2; ++i) {
-          const f32x4 val = widen(__builtin_bit_cast(bf16x4, i ? uint2{raw.z, raw.w} : uint2{raw.x, raw.y}));
-          const f32x4 n_j = *reinterpret_cast<const f32x4*>(n_s + 32 * s + 16 * i + 4 * g);
-#pragma unroll
-          for (int r = 0; r < 4; ++r) {
-            const float left = REV ? n_j[r] : all - n_j[r];
-            w[i][r] = val[r] * (a.c_update * lam[(int)left]);
-            if (DERIV) wd[i][r] = w[i][r] * left;
+          const int j0 = 32 * s + 16 * i + 4 * g;
+          w[i] = widen(__builtin_bit_cast(bf16x4, i ? uint2{raw.z, raw.w} : uint2{raw.x, raw.y})) *
+                 *reinterpret_cast<const f32x4*>(update_s + j0);
+          if (DERIV) {
+            const f32x4 n_j = *reinterpret_cast<const f32x4*>(n_s + j0);
+            wd[i] = w[i] * (REV ? n_j : all - n_j);
           }
         }
         bf16x8 w_hi, w_lo, wd_hi, wd_lo;
@@ -644,7 +665,7 @@ __global__ __launch_bounds__(DP * 4, 2) void la_pass_bf16(PassArgs a) {
         if (DERIV) split8(wd[0], wd[1], wd_hi, wd_lo);
 #pragma unroll
         for (int t = 0; t < NT; ++t) {
-          const bf16x8 kf = Ch::columns(k_s, 16 * t, s, lo, g);
+          const bf16x8 kf = Ch::columns(k_s, state_row(t, 0, 0), 8, s, lo, g);
           S[t] = mfma32(kf, w_lo, S[t]);
           S[t] = mfma32(kf, w_hi, S[t]);
           if (DERIV) {
@@ -673,7 +694,7 @@ __global__ __launch_bounds__(DP * 4, 2) void la_pass_bf16(PassArgs a) {
   for (int t = 0; t < NT; ++t) {
 #pragma unroll
     for (int r = 0; r < 4; ++r) {
-      const int c = 16 * t + 4 * g + r;
+      const int c = state_row(t, g, r);
       if (c < a.Dc && e < a.De) {
         const int64_t at = c * a.st_c + e * a.st_e;
         if (dst) dst[at] = S[t][r];
