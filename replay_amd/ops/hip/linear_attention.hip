@@ -438,6 +438,11 @@ __global__ __launch_bounds__(DP * 4, DP == 128 || DERIV ? 2 : 3) void la_pass_bf
   // a decay of zero (log -inf) keeps l^0 = 1
   for (int i = threadIdx.x; i <= C; i += Ch::NT) lam[i] = i ? expf(ld * i) : 1.f;
 
+  // false while the state is known to be zero, as a history's first chunk has it
+  bool started = FULL && (a.G > 1 || a.state_in);
+  // whether the state after the last chunk is asked for
+  const bool at_end = REV ? seg == 0 : seg == a.G - 1;
+  const bool want_end = STATE_ONLY || (at_end && (a.state_out || (DERIV && a.state_end_grad)));
   f32x4 S[NT], Sd[DERIV ? NT : 1];
   {
     const float* src = nullptr;
@@ -550,12 +555,14 @@ __global__ __launch_bounds__(DP * 4, DP == 128 || DERIV ? 2 : 3) void la_pass_bf
       const float all = (float)N;
 
       if (FULL) {
-        const bool whole = now == ~0ull;
+        // valid positions in one run: n_i - n_j = i - j wherever a pair counts
+        const uint64_t run = now >> __builtin_ctzll(now);
+        const bool whole = (run & (run + 1)) == 0;
         // the start state's part, a block of the contraction at a time: so the
         // split state needs registers for one block only
         f32x4 os[4] = {}, ods[DERIV ? 4 : 1] = {};
 #pragma unroll
-        for (int s = 0; s < NS; ++s) {
+        for (int s = 0; s < NS && started; ++s) {
           asm volatile("" ::: "memory");
           bf16x8 s_hi, s_lo, d_hi, d_lo;
           split8(S[2 * s], S[2 * s + 1], s_hi, s_lo);
@@ -639,14 +646,18 @@ __global__ __launch_bounds__(DP * 4, DP == 128 || DERIV ? 2 : 3) void la_pass_bf
         }
       }
 
-      const float lN = lam[N];
+      const bool update = want_end || step + 1 < last;
+      if (started && update) {
+        const float lN = lam[N];
 #pragma unroll
-      for (int t = 0; t < NT; ++t) {
-        if (DERIV) Sd[t] = lN * (Sd[t] + all * S[t]);
-        S[t] = lN * S[t];
+        for (int t = 0; t < NT; ++t) {
+          if (DERIV) Sd[t] = lN * (Sd[t] + all * S[t]);
+          S[t] = lN * S[t];
+        }
       }
+      started = true;
 #pragma unroll
-      for (int s = 0; s < 2; ++s) {
+      for (int s = 0; s < 2 && update; ++s) {
         asm volatile("" ::: "memory");
         f32x4 w[2], wd[2];
         const uint4 raw = __builtin_bit_cast(uint4, vf[s]);
@@ -681,7 +692,6 @@ __global__ __launch_bounds__(DP * 4, DP == 128 || DERIV ? 2 : 3) void la_pass_bf
 
   float* dst = nullptr;
   float* dst_d = nullptr;
-  const bool at_end = REV ? seg == 0 : seg == a.G - 1;
   if (STATE_ONLY) {
     dst = a.seg + (bh * a.G + seg) * state_size;
     if (DERIV) dst_d = a.seg_d + (bh * a.G + seg) * state_size;
