@@ -59,70 +59,89 @@ struct PassArgs {
   float* decay_part;                 // [B, H, G] partial sums of the decay's gradient
   int64_t st_c, st_e;                // strides of a state's (contraction, value) axes
   int B, H, L, Dc, De, G, seg_chunks;
-  bool vec_c, vec_e, vec_x;          // 16-byte loads are aligned (contraction / value side, x)
   float c_pair, c_inter, c_update;   // where the scale goes
 };
-
-// One 16-byte piece of a row, widened to float; beyond D it reads as zero.
-template <typename T>
-__device__ __forceinline__ void load_piece(const T* row, int d0, int D, bool vec, float* o) {
-  constexpr int V = 16 / sizeof(T);
-  if (vec) {
-    if (d0 < D) {
-      alignas(16) T t[V];
-      *reinterpret_cast<float4*>(t) = *reinterpret_cast<const float4*>(row + d0);
-#pragma unroll
-      for (int i = 0; i < V; ++i) o[i] = to_f32<T>(t[i]);
-    } else {
-#pragma unroll
-      for (int i = 0; i < V; ++i) o[i] = 0.f;
-    }
-  } else {
-#pragma unroll
-    for (int i = 0; i < V; ++i) o[i] = (d0 + i < D) ? to_f32<T>(row[d0 + i]) : 0.f;
-  }
-}
-
-// Positions [l0, l0+C) of one head into LDS as float [C][DP+4]; rows that the
-// mask or the length leaves out are zero whatever they hold.
-template <typename T, int DP, int C>
-__device__ __forceinline__ void stage(float* dst, const Rows& r, int b, int h, int l0, int D,
-                                      bool vec, unsigned bits) {
-  constexpr int V = 16 / sizeof(T), PR = DP / V, LD = DP + 4;
-  const T* base = reinterpret_cast<const T*>(r.p) + b * r.b + h * r.h;
-  for (int i = threadIdx.x; i < C * PR; i += DP * 4) {
-    const int row = i / PR, d0 = (i % PR) * V;
-    float o[V];
-    if ((bits >> row) & 1u) {
-      load_piece<T>(base + (int64_t)(l0 + row) * r.l, d0, D, vec, o);
-    } else {
-#pragma unroll
-      for (int j = 0; j < V; ++j) o[j] = 0.f;
-    }
-#pragma unroll
-    for (int j = 0; j < V; j += 4)
-      *reinterpret_cast<f32x4*>(dst + row * LD + d0 + j) = f32x4{o[j], o[j + 1], o[j + 2], o[j + 3]};
-  }
-}
 
 __device__ __forceinline__ f32x4 mfma4(float a, float b, f32x4 c) {
   return __builtin_amdgcn_mfma_f32_16x16x4f32(a, b, c, 0, 0, 0);
 }
 
-// One segment of one (batch, head).  DP/16 waves; each owns 16 value columns
-// and the whole contraction axis of the state, in the accumulator layout
-// (column = lane & 15, row = 4 (lane >> 4) + r), which is also the layout of
-// an operand whose contraction index is visited in that order: neither the
-// state nor the pair weights leave the registers between products.
+// V neighbours of a row, of which n exist; no alignment is asked for
+template <typename T, int V>
+__device__ __forceinline__ uint4 load_piece(const T* p, int n) {
+  alignas(16) T t[V];
+  if (n >= V) {
+    __builtin_memcpy(t, p, 16);
+  } else {
+#pragma unroll
+    for (int i = 0; i < V; ++i) t[i] = i < n ? p[i] : from_f32<T>(0.f);
+  }
+  return *reinterpret_cast<const uint4*>(t);
+}
+
+// One operand's 32 positions on their way from memory to LDS, where they are
+// float: 16-byte pieces, DP / V threads a row.
+template <typename T, int DP>
+struct Rows32 {
+  static constexpr int V = 16 / sizeof(T), ACROSS = DP / V, DOWN = DP * 4 / ACROSS, PIECES = 32 / DOWN;
+  static constexpr int LD = DP + 4;  // rows then start 4 banks apart
+
+  const T* at;
+  int64_t l;
+  int left;
+  uint4 r[PIECES];
+
+  __device__ __forceinline__ Rows32(const Rows& src, int b, int h, int D) {
+    const int d = (threadIdx.x % ACROSS) * V;
+    l = src.l;
+    left = D - d;
+    at = reinterpret_cast<const T*>(src.p) + b * src.b + h * src.h + (threadIdx.x / ACROSS) * l + d;
+  }
+  __device__ __forceinline__ void fetch(int l0, unsigned bits) {
+#pragma unroll
+    for (int i = 0; i < PIECES; ++i) {
+      r[i] = uint4{0, 0, 0, 0};
+      if (((bits >> (threadIdx.x / ACROSS + i * DOWN)) & 1) && left > 0)
+        r[i] = load_piece<T, V>(at + (l0 + i * DOWN) * l, left);
+    }
+  }
+  __device__ __forceinline__ void put(float* dst) const {
+    dst += (threadIdx.x / ACROSS) * LD + (threadIdx.x % ACROSS) * V;
+#pragma unroll
+    for (int i = 0; i < PIECES; ++i) {
+      alignas(16) T t[V];
+      *reinterpret_cast<uint4*>(t) = r[i];
+#pragma unroll
+      for (int j = 0; j < V; j += 4)
+        *reinterpret_cast<f32x4*>(dst + i * DOWN * LD + j) =
+            f32x4{to_f32<T>(t[j]), to_f32<T>(t[j + 1]), to_f32<T>(t[j + 2]), to_f32<T>(t[j + 3])};
+    }
+  }
+};
+
+// One segment of one (batch, head) on the float32 matrix instructions: 16
+// positions a chunk (the pair products grow with it, and these instructions
+// have a sixteenth of the 16-bit ones' rate), 32 a load.  DP/16 waves; each
+// owns 16 value columns and the whole contraction axis of the state, in the
+// accumulator layout (column = lane & 15, row = 4 (lane >> 4) + r), which is
+// also the layout of an operand whose contraction index is visited in that
+// order: neither the state nor the pair weights leave the registers between
+// products.
 template <typename T, int DP, bool REV, bool STATE_ONLY, bool DERIV>
-__global__ __launch_bounds__(DP * 4) void la_pass_f32(PassArgs a) {
-  constexpr int C = 16, LD = DP + 4, NT = DP / 16;
-  __shared__ __attribute__((aligned(16))) float q_s[STATE_ONLY ? 4 : C * LD];
-  __shared__ __attribute__((aligned(16))) float k_s[C * LD];
-  __shared__ __attribute__((aligned(16))) float v_s[C * LD];
-  __shared__ __attribute__((aligned(16))) float x_s[(DERIV && !STATE_ONLY) ? C * LD : 4];
+__global__ __launch_bounds__(DP * 4, DP == 128 ? 1 : 2) void la_pass_f32(PassArgs a) {
+  using Ch = Rows32<T, DP>;
+  constexpr int C = 16, ROWS = 32, LD = Ch::LD, NT = DP / 16, WAVES = DP / 16;
+  constexpr bool FULL = !STATE_ONLY, X = DERIV && FULL;
+  __shared__ __attribute__((aligned(16))) float q_s[FULL ? ROWS * LD : 4];
+  __shared__ __attribute__((aligned(16))) float k_s[ROWS * LD];
+  __shared__ __attribute__((aligned(16))) float v_s[ROWS * LD];
+  __shared__ __attribute__((aligned(16))) float o_s[FULL ? ROWS * LD : 4];
+  __shared__ __attribute__((aligned(16))) float x_s[X ? ROWS * LD : 4];
+  // of each position, within its chunk: the valid ones up to it, and its
+  // weights in the product with the start state and in the state's update
+  __shared__ __attribute__((aligned(16))) float n_s[ROWS], inter_s[ROWS], update_s[ROWS];
   __shared__ float lam[C + 1];
-  __shared__ float red[DP / 16];
+  __shared__ float red[WAVES];
 
   const int seg = blockIdx.x % a.G;
   const int64_t bh = blockIdx.x / a.G;
@@ -130,16 +149,22 @@ __global__ __launch_bounds__(DP * 4) void la_pass_f32(PassArgs a) {
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
   const int lo = lane & 15, g = lane >> 4;
   const int e0 = wave * 16, e = e0 + lo;
+  const bool busy = e0 < a.De;
   const int64_t state_size = (int64_t)a.Dc * a.De;
   const float ld = a.log_decay[h];
   // a decay of zero (log -inf) keeps l^0 = 1
   if (threadIdx.x <= C) lam[threadIdx.x] = threadIdx.x ? expf(ld * threadIdx.x) : 1.f;
 
+  // whether the state after the last chunk is asked for
+  const bool at_end = REV ? seg == 0 : seg == a.G - 1;
+  const bool want_end = STATE_ONLY || (at_end && (a.state_out || (DERIV && a.state_end_grad)));
+  // false while the state is known to be zero, as a history's first chunk has it
+  bool started = FULL && (a.G > 1 || a.state_in);
   f32x4 S[NT], Sd[DERIV ? NT : 1];
   {
     const float* src = nullptr;
     const float* src_d = nullptr;
-    if (!STATE_ONLY) {
+    if (FULL) {
       if (a.G > 1) {
         src = a.seg + (bh * a.G + seg) * state_size;
         if (DERIV) src_d = a.seg_d + (bh * a.G + seg) * state_size;
@@ -158,97 +183,188 @@ __global__ __launch_bounds__(DP * 4) void la_pass_f32(PassArgs a) {
       }
     }
   }
+  __syncthreads();  // lam
+  // the pair weights of a chunk without gaps
+  f32x4 full = {};
+  if (FULL) {
+#pragma unroll
+    for (int r = 0; r < 4; ++r) {
+      const int gap = REV ? 4 * g + r - lo : lo - 4 * g - r;
+      full[r] = gap >= 0 ? a.c_pair * lam[max(gap, 0)] : 0.f;
+    }
+  }
 
-  const int n_chunks = (a.L + C - 1) / C;
-  const int first = seg * a.seg_chunks, last = min(n_chunks, first + a.seg_chunks);
+  // seg_chunks counts loads of 32 positions here
+  const int n_loads = (a.L + ROWS - 1) / ROWS;
+  const int first = seg * a.seg_chunks, last = min(n_loads, first + a.seg_chunks);
+  auto start_of = [&](int step) { return (REV ? first + last - 1 - step : step) * ROWS; };
   int total = 0;
   float d_decay = 0.f;
-  for (int step = first; step < last; ++step) {
-    const int l0 = (REV ? first + last - 1 - step : step) * C;
-    const int pos = l0 + lo;
-    const bool ok = lane < C && pos < a.L &&
-                    (!a.mask || a.mask[b * a.mask_b + pos * a.mask_l]);
-    const unsigned bits = (unsigned)__ballot(ok);
-    const int N = __popc(bits);
-    total += N;
-    __syncthreads();  // the previous chunk's reads, and lam
-    if (!STATE_ONLY) stage<T, DP, C>(q_s, a.q, b, h, l0, a.Dc, a.vec_c, bits);
-    stage<T, DP, C>(k_s, a.k, b, h, l0, a.Dc, a.vec_c, bits);
-    stage<T, DP, C>(v_s, a.v, b, h, l0, a.De, a.vec_e, bits);
-    if (DERIV && !STATE_ONLY) stage<T, DP, C>(x_s, a.x, b, h, l0, a.De, a.vec_x, bits);
-    __syncthreads();
-    if (e0 >= a.De) continue;
-
-    const int n_i = __popc(bits & ((2u << lo) - 1u));
-    int n_j[4];
-    float vr[4];
+  Ch q_r(a.q, b, h, a.Dc), k_r(a.k, b, h, a.Dc), v_r(a.v, b, h, a.De), x_r(a.x, b, h, a.De);
+  // The mask is read a load ahead of the rows that it says to read.
+  const bool* mask = a.mask ? a.mask + b * a.mask_b : nullptr;
+  auto look = [&](int step) {
+    const int pos = start_of(step) + lane;
+    return lane < ROWS && step < last && pos < a.L && (!mask || mask[pos * a.mask_l]);
+  };
+  auto fetch = [&](int step, unsigned bits) {
+    const int l0 = start_of(step);
+    if (FULL) q_r.fetch(l0, bits);
+    k_r.fetch(l0, bits);
+    v_r.fetch(l0, bits);
+    if (X) x_r.fetch(l0, bits);
+  };
+  T* out = nullptr;
+  if (FULL)
+    out = reinterpret_cast<T*>(a.out) + b * a.out_b + h * a.out_h +
+          (threadIdx.x / Ch::ACROSS) * a.out_l + (threadIdx.x % Ch::ACROSS) * Ch::V;
+  // outputs of the rows at l0 in whole rows, from LDS or zeros
+  auto store = [&](int l0, bool zero) {
+    const int row = threadIdx.x / Ch::ACROSS, left = v_r.left;
+    const float* from = o_s + row * LD + (threadIdx.x % Ch::ACROSS) * Ch::V;
 #pragma unroll
-    for (int r = 0; r < 4; ++r) {
-      n_j[r] = __popc(bits & ((2u << (4 * g + r)) - 1u));
-      vr[r] = v_s[(4 * g + r) * LD + e];
+    for (int i = 0; i < Ch::PIECES; ++i) {
+      if (l0 + row + Ch::DOWN * i >= a.L || left <= 0) continue;
+      alignas(16) T t[Ch::V];
+#pragma unroll
+      for (int j = 0; j < Ch::V; j += 4) {
+        f32x4 v = {0.f, 0.f, 0.f, 0.f};
+        if (!zero) v = *reinterpret_cast<const f32x4*>(from + i * Ch::DOWN * LD + j);
+#pragma unroll
+        for (int r = 0; r < 4; ++r) t[j + r] = from_f32<T>(v[r]);
+      }
+      T* p = out + (l0 + Ch::DOWN * i) * a.out_l;
+      if (left >= Ch::V) {
+        __builtin_memcpy(p, t, 16);
+      } else {
+#pragma unroll
+        for (int j = 0; j < Ch::V; ++j)
+          if (j < left) p[j] = t[j];
+      }
     }
-    if (!STATE_ONLY) {
-      // pair products, transposed: rows j (keys), columns i (queries)
-      f32x4 pt = {0.f, 0.f, 0.f, 0.f};
+  };
+
+  unsigned bits = (unsigned)__ballot(look(first));
+  fetch(first, bits);
+  bool ahead = look(first + 1);
+#pragma unroll 1
+  for (int step = first; step < last; ++step) {
+    const int l0 = start_of(step);
+    const unsigned now = bits;
+    total += __popc(now);
+    if (now == 0) {  // nothing is seen, added or forgotten
+      if (FULL) store(l0, true);
+      bits = (unsigned)__ballot(ahead);
+      fetch(step + 1, bits);
+      ahead = look(step + 2);
+      continue;
+    }
+    if (FULL) q_r.put(q_s);
+    k_r.put(k_s);
+    v_r.put(v_s);
+    if (X) x_r.put(x_s);
+    if (threadIdx.x < ROWS) {
+      const unsigned own = (now >> (lane & 16)) & 0xffffu;
+      const int n = __popc(own & ((2u << (lane & 15)) - 1)), N = __popc(own);
+      n_s[lane] = (float)n;
+      inter_s[lane] = a.c_inter * lam[REV ? N - n : n];
+      update_s[lane] = a.c_update * lam[REV ? n : N - n];
+    }
+    __syncthreads();
+    bits = (unsigned)__ballot(ahead);
+    fetch(step + 1, bits);
+    ahead = look(step + 2);
+
+    if (busy) {
+#pragma unroll 1
+      for (int half = 0; half < 2; ++half) {
+        const int r0 = (REV ? 1 - half : half) * C;
+        const unsigned own = (now >> r0) & 0xffffu;
+        const int N = __popc(own);
+        if (N == 0) {
+          if (FULL) *reinterpret_cast<f32x4*>(o_s + (r0 + lo) * LD + e0 + 4 * g) = f32x4{0.f, 0.f, 0.f, 0.f};
+          continue;
+        }
+        const float* k_c = k_s + r0 * LD;
+        float vr[4];
 #pragma unroll
-      for (int s = 0; s < DP / 4; ++s)
-        pt = mfma4(k_s[lo * LD + 4 * s + g], q_s[lo * LD + 4 * s + g], pt);
-      f32x4 o = {0.f, 0.f, 0.f, 0.f}, od = {0.f, 0.f, 0.f, 0.f};
+        for (int r = 0; r < 4; ++r) vr[r] = v_s[(r0 + 4 * g + r) * LD + e];
+        const f32x4 n_j = *reinterpret_cast<const f32x4*>(n_s + r0 + 4 * g);
+        if (FULL) {
+          const float* q_c = q_s + (r0 + lo) * LD;
+          const float n_i = n_s[r0 + lo], w_i = inter_s[r0 + lo];
+          f32x4 pt = {0.f, 0.f, 0.f, 0.f}, o = pt, od = pt;
 #pragma unroll
-      for (int t = 0; t < NT; ++t) {
-        const f32x4 qv = *reinterpret_cast<const f32x4*>(q_s + lo * LD + 16 * t + 4 * g);
+          for (int t = 0; t < NT; ++t) {
+            const f32x4 qv = *reinterpret_cast<const f32x4*>(q_c + 16 * t + 4 * g);
+            const f32x4 kv = *reinterpret_cast<const f32x4*>(k_c + lo * LD + 16 * t + 4 * g);
+#pragma unroll
+            for (int r = 0; r < 4; ++r) pt = mfma4(kv[r], qv[r], pt);
+            if (started) {
+#pragma unroll
+              for (int r = 0; r < 4; ++r) {
+                o = mfma4(S[t][r], qv[r], o);
+                if (DERIV) od = mfma4(Sd[t][r], qv[r], od);
+              }
+            }
+          }
+          if (DERIV) od = w_i * (od + n_i * o);
+          o = w_i * o;
+          // valid positions in one run: n_i - n_j = i - j wherever a pair counts
+          const unsigned run = own >> __builtin_ctz(own);
+          const bool whole = (run & (run + 1)) == 0;
+          const f32x4 gaps = REV ? n_j - n_i : n_i - n_j;
+          f32x4 p = pt * full;
+          if (!whole) {
+#pragma unroll
+            for (int r = 0; r < 4; ++r) {
+              const bool seen = REV ? 4 * g + r >= lo : 4 * g + r <= lo;
+              p[r] = seen ? pt[r] * (a.c_pair * lam[max((int)gaps[r], 0)]) : 0.f;
+            }
+          }
+#pragma unroll
+          for (int r = 0; r < 4; ++r) {
+            o = mfma4(vr[r], p[r], o);
+            if (DERIV) od = mfma4(vr[r], p[r] * gaps[r], od);
+          }
+          if (DERIV) {
+            const f32x4 xv = *reinterpret_cast<const f32x4*>(x_s + (r0 + lo) * LD + e0 + 4 * g);
+#pragma unroll
+            for (int r = 0; r < 4; ++r) d_decay += xv[r] * od[r];
+          }
+          *reinterpret_cast<f32x4*>(o_s + (r0 + lo) * LD + e0 + 4 * g) = o;
+        }
+        const bool update = want_end || step + 1 < last || half == 0;
+        if (started && update) {
+          const float lN = lam[N];
+#pragma unroll
+          for (int t = 0; t < NT; ++t) {
+            if (DERIV) Sd[t] = lN * (Sd[t] + (float)N * S[t]);
+            S[t] = lN * S[t];
+          }
+        }
+        started = true;
+        if (!update) continue;
+        const f32x4 w = *reinterpret_cast<const f32x4*>(update_s + r0 + 4 * g);
+        const f32x4 left = REV ? n_j : (float)N - n_j;
 #pragma unroll
         for (int r = 0; r < 4; ++r) {
-          o = mfma4(S[t][r], qv[r], o);
-          if (DERIV) od = mfma4(Sd[t][r], qv[r], od);
+          const float weighted = vr[r] * w[r];
+#pragma unroll
+          for (int t = 0; t < NT; ++t) {
+            const float kv = k_c[(4 * g + r) * LD + 16 * t + lo];
+            S[t] = mfma4(kv, weighted, S[t]);
+            if (DERIV) Sd[t] = mfma4(kv, weighted * left[r], Sd[t]);
+          }
         }
       }
-      const float w_i = a.c_inter * lam[REV ? N - n_i : n_i];
-      if (DERIV) od = w_i * (od + (float)n_i * o);
-      o = w_i * o;
-#pragma unroll
-      for (int r = 0; r < 4; ++r) {
-        const int j = 4 * g + r;
-        const bool seen = REV ? j >= lo : j <= lo;
-        const int gap = REV ? n_j[r] - n_i : n_i - n_j[r];
-        const float p = seen ? pt[r] * (a.c_pair * lam[seen ? gap : 0]) : 0.f;
-        o = mfma4(vr[r], p, o);
-        if (DERIV) od = mfma4(vr[r], p * (float)(seen ? gap : 0), od);
-      }
-      if (DERIV) {
-        const f32x4 xv = *reinterpret_cast<const f32x4*>(x_s + lo * LD + e0 + 4 * g);
-#pragma unroll
-        for (int r = 0; r < 4; ++r) d_decay += xv[r] * od[r];
-      }
-      if (pos < a.L) {
-        T* row = reinterpret_cast<T*>(a.out) + b * a.out_b + h * a.out_h + (int64_t)pos * a.out_l;
-#pragma unroll
-        for (int r = 0; r < 4; ++r)
-          if (e0 + 4 * g + r < a.De) row[e0 + 4 * g + r] = from_f32<T>(o[r]);
-      }
     }
-    const float lN = lam[N];
-#pragma unroll
-    for (int t = 0; t < NT; ++t) {
-      if (DERIV) Sd[t] = lN * (Sd[t] + (float)N * S[t]);
-      S[t] = lN * S[t];
-    }
-#pragma unroll
-    for (int r = 0; r < 4; ++r) {
-      const int left = REV ? n_j[r] : N - n_j[r];
-      const float w = vr[r] * (a.c_update * lam[left]);
-#pragma unroll
-      for (int t = 0; t < NT; ++t) {
-        const float kv = k_s[(4 * g + r) * LD + 16 * t + lo];
-        S[t] = mfma4(kv, w, S[t]);
-        if (DERIV) Sd[t] = mfma4(kv, w * (float)left, Sd[t]);
-      }
-    }
+    __syncthreads();  // the rows are read and their outputs are in LDS
+    if (FULL) store(l0, false);
   }
 
   float* dst = nullptr;
   float* dst_d = nullptr;
-  const bool at_end = REV ? seg == 0 : seg == a.G - 1;
   if (STATE_ONLY) {
     dst = a.seg + (bh * a.G + seg) * state_size;
     if (DERIV) dst_d = a.seg_d + (bh * a.G + seg) * state_size;
@@ -256,8 +372,7 @@ __global__ __launch_bounds__(DP * 4) void la_pass_f32(PassArgs a) {
   } else if (at_end && a.state_out) {
     dst = a.state_out + bh * state_size;
   }
-  const float* end_grad = (DERIV && !STATE_ONLY && at_end && a.state_end_grad)
-                              ? a.state_end_grad + bh * state_size : nullptr;
+  const float* end_grad = (X && at_end && a.state_end_grad) ? a.state_end_grad + bh * state_size : nullptr;
 #pragma unroll
   for (int t = 0; t < NT; ++t) {
 #pragma unroll
@@ -271,13 +386,13 @@ __global__ __launch_bounds__(DP * 4) void la_pass_f32(PassArgs a) {
       }
     }
   }
-  if (DERIV && !STATE_ONLY) {
+  if (X) {
     d_decay = wave_reduce_sum(d_decay);
     if (lane == 0) red[wave] = d_decay;
     __syncthreads();
     if (threadIdx.x == 0) {
       float sum = 0.f;
-      for (int w = 0; w < DP / 16; ++w) sum += red[w];
+      for (int w = 0; w < WAVES; ++w) sum += red[w];
       a.decay_part[bh * a.G + seg] = sum;
     }
   }
@@ -298,8 +413,9 @@ __global__ __launch_bounds__(DP * 4) void la_pass_f32(PassArgs a) {
 // head are 32 KB, some 2500 cycles of a CU's share, against 930 of products).
 //
 // Roundings to bfloat16: the pair weights, once (half a step of each term).
-// The state, and the values weighted into it, go in as the sum of two bfloat16
-// (2^-17): what reaches the float32 states is no coarser than their sums.
+// The state goes into the outputs as the sum of two bfloat16s (2^-17), into
+// the decay's float32 gradient as three; the values weighted into the float32
+// states go in as three, so that these are no coarser than their sums.
 
 typedef __attribute__((ext_vector_type(8))) __bf16 bf16x8;
 typedef __attribute__((ext_vector_type(4))) __bf16 bf16x4;
@@ -320,12 +436,32 @@ __device__ __forceinline__ bf16x8 pack8(f32x4 a, f32x4 b) {
 
 __device__ __forceinline__ f32x4 widen(bf16x4 a) { return __builtin_convertvector(a, f32x4); }
 
-// v = hi + lo to 2^-17
-__device__ __forceinline__ void split8(f32x4 a, f32x4 b, bf16x8& hi, bf16x8& lo) {
-  const bf16x4 x = __builtin_convertvector(a, bf16x4), y = __builtin_convertvector(b, bf16x4);
-  hi = join8(__builtin_bit_cast(uint2, x), __builtin_bit_cast(uint2, y));
-  lo = pack8(a - widen(x), b - widen(y));
-}
+// A float operand as a sum of N bfloat16s: to 2^-17 with two, exact with three
+// (but for what underflows).
+template <int N>
+struct Split8 {
+  bf16x8 part[N];
+  __device__ __forceinline__ Split8(f32x4 a, f32x4 b) {
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+      const bf16x4 x = __builtin_convertvector(a, bf16x4), y = __builtin_convertvector(b, bf16x4);
+      part[i] = join8(__builtin_bit_cast(uint2, x), __builtin_bit_cast(uint2, y));
+      a = a - widen(x);
+      b = b - widen(y);
+    }
+  }
+  // c + this . other, the small parts first; this as the left operand or the right
+  __device__ __forceinline__ f32x4 times(bf16x8 other, f32x4 c) const {
+#pragma unroll
+    for (int i = N - 1; i >= 0; --i) c = mfma32(part[i], other, c);
+    return c;
+  }
+  __device__ __forceinline__ f32x4 after(bf16x8 other, f32x4 c) const {
+#pragma unroll
+    for (int i = N - 1; i >= 0; --i) c = mfma32(other, part[i], c);
+    return c;
+  }
+};
 
 // 8 neighbours of a row, of which n exist (all of them unless EDGE); no
 // alignment is asked for
@@ -564,18 +700,13 @@ __global__ __launch_bounds__(DP * 4, DP == 128 || DERIV ? 2 : 3) void la_pass_bf
 #pragma unroll
         for (int s = 0; s < NS && started; ++s) {
           asm volatile("" ::: "memory");
-          bf16x8 s_hi, s_lo, d_hi, d_lo;
-          split8(S[2 * s], S[2 * s + 1], s_hi, s_lo);
-          if (DERIV) split8(Sd[2 * s], Sd[2 * s + 1], d_hi, d_lo);
+          const Split8<DERIV ? 3 : 2> state(S[2 * s], S[2 * s + 1]);
+          const Split8<3> state_d(Sd[DERIV ? 2 * s : 0], Sd[DERIV ? 2 * s + 1 : 0]);
 #pragma unroll
           for (int it = 0; it < 4; ++it) {
             const bf16x8 qf = Ch::rows(q_s, 16 * it, s, lo, g);
-            os[it] = mfma32(s_lo, qf, os[it]);
-            os[it] = mfma32(s_hi, qf, os[it]);
-            if (DERIV) {
-              ods[it] = mfma32(d_lo, qf, ods[it]);
-              ods[it] = mfma32(d_hi, qf, ods[it]);
-            }
+            os[it] = state.times(qf, os[it]);
+            if (DERIV) ods[it] = state_d.times(qf, ods[it]);
           }
         }
 #pragma unroll
@@ -659,7 +790,7 @@ __global__ __launch_bounds__(DP * 4, DP == 128 || DERIV ? 2 : 3) void la_pass_bf
 #pragma unroll
       for (int s = 0; s < 2 && update; ++s) {
         asm volatile("" ::: "memory");
-        f32x4 w[2], wd[2];
+        f32x4 w[2], wd[2] = {};
         const uint4 raw = __builtin_bit_cast(uint4, vf[s]);
 #pragma unroll
         for (int i = 0; i < 2; ++i) {
@@ -671,18 +802,12 @@ __global__ __launch_bounds__(DP * 4, DP == 128 || DERIV ? 2 : 3) void la_pass_bf
             wd[i] = w[i] * (REV ? n_j : all - n_j);
           }
         }
-        bf16x8 w_hi, w_lo, wd_hi, wd_lo;
-        split8(w[0], w[1], w_hi, w_lo);
-        if (DERIV) split8(wd[0], wd[1], wd_hi, wd_lo);
+        const Split8<3> weighted(w[0], w[1]), weighted_d(wd[0], wd[1]);
 #pragma unroll
         for (int t = 0; t < NT; ++t) {
           const bf16x8 kf = Ch::columns(k_s, state_row(t, 0, 0), 8, s, lo, g);
-          S[t] = mfma32(kf, w_lo, S[t]);
-          S[t] = mfma32(kf, w_hi, S[t]);
-          if (DERIV) {
-            Sd[t] = mfma32(kf, wd_lo, Sd[t]);
-            Sd[t] = mfma32(kf, wd_hi, Sd[t]);
-          }
+          S[t] = weighted.after(kf, S[t]);
+          if (DERIV) Sd[t] = weighted_d.after(kf, Sd[t]);
         }
       }
     }
@@ -765,32 +890,91 @@ __global__ void la_decay_sum(const float* part, float* out, int B, int H, int G)
   if (threadIdx.x == 0) out[h] = (float)(red[0] + red[1] + red[2] + red[3]);
 }
 
-// One position for each row: the state is read, updated and written once.
-template <typename T>
-__global__ void la_step_kernel(Rows q, Rows k, Rows v, const float* log_decay, float* state,
-                               int64_t st_b, int64_t st_h, const bool* active, int64_t act_b,
-                               T* out, int H, int Dk, int Dv, float scale) {
-  const int64_t bh = blockIdx.x;
+// One position for each row: the state is read, updated and written once, and
+// that is the bound.  A wave takes 4 LE columns of one (batch, head): LE lanes
+// with four neighbours each across, 64 / LE groups of rows down, BATCH rows of
+// a group in flight; the groups' outputs meet in two or three shuffles.  No
+// LDS and no barrier: 4096 x 4 states of 64 x 64 in 80 us (6.7 TB/s, the
+// last-level cache keeping a part of the 268 MB; a loop of one column a
+// thread: 253).  EDGE: any head sizes, else whole batches.
+template <typename T, int LE, int BATCH, bool EDGE>
+__global__ __launch_bounds__(256) void la_step_kernel(Rows q, Rows k, Rows v, const float* log_decay,
+                                                      float* state, int64_t st_b, int64_t st_h,
+                                                      const bool* active, int64_t act_b, T* out,
+                                                      int64_t waves, int H, int Dk, int Dv, float scale) {
+  constexpr int RG = 64 / LE;
+  const int lane = threadIdx.x & 63, rg = lane / LE;
+  const int64_t wave = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
+  if (wave >= waves) return;
+  const int across = (Dv + 4 * LE - 1) / (4 * LE);
+  const int64_t bh = wave / across;
   const int b = bh / H, h = bh % H;
-  T* o = out + bh * Dv;
-  if (active && !active[b * act_b]) {
-    for (int e = threadIdx.x; e < Dv; e += blockDim.x) o[e] = from_f32<T>(0.f);
-    return;
-  }
-  const float l = expf(log_decay[h]);
-  const T* qr = reinterpret_cast<const T*>(q.p) + b * q.b + h * q.h;
-  const T* kr = reinterpret_cast<const T*>(k.p) + b * k.b + h * k.h;
-  const T* vr = reinterpret_cast<const T*>(v.p) + b * v.b + h * v.h;
-  float* S = state + b * st_b + h * st_h;
-  for (int e = threadIdx.x; e < Dv; e += blockDim.x) {
-    const float ve = to_f32<T>(vr[e]);
-    float sum = 0.f;
-    for (int c = 0; c < Dk; ++c) {
-      const float s = l * S[(int64_t)c * Dv + e] + to_f32<T>(kr[c]) * ve;
-      S[(int64_t)c * Dv + e] = s;
-      sum += to_f32<T>(qr[c]) * s;
+  const int e = (int)(wave % across) * 4 * LE + (lane % LE) * 4, n = EDGE ? Dv - e : 4;
+  T* o = out + bh * Dv + e;
+  float sum[4] = {};
+  if (!active || active[b * act_b]) {
+    const float l = expf(log_decay[h]);
+    const T* qr = reinterpret_cast<const T*>(q.p) + b * q.b + h * q.h;
+    const T* kr = reinterpret_cast<const T*>(k.p) + b * k.b + h * k.h;
+    const T* vr = reinterpret_cast<const T*>(v.p) + b * v.b + h * v.h;
+    float* S = state + b * st_b + h * st_h + e;
+    float ve[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) ve[i] = i < n ? to_f32<T>(vr[e + i]) : 0.f;
+    const int rows = (Dk + RG - 1) / RG, row0 = rg * rows, row_end = min(Dk, row0 + rows);
+    if (n > 0) {
+      for (int c0 = row0; c0 < row_end; c0 += BATCH) {
+        f32x4 st[BATCH];
+        T kc[BATCH], qc[BATCH];
+#pragma unroll
+        for (int i = 0; i < BATCH; ++i) {
+          const float* at = S + (int64_t)(c0 + i) * Dv;
+          if (!EDGE || (c0 + i < row_end && n >= 4)) {
+            __builtin_memcpy(&st[i], at, 16);
+          } else {
+#pragma unroll
+            for (int j = 0; j < 4; ++j) st[i][j] = (c0 + i < row_end && j < n) ? at[j] : 0.f;
+          }
+        }
+        if (!EDGE) {
+          __builtin_memcpy(kc, kr + c0, BATCH * sizeof(T));
+          __builtin_memcpy(qc, qr + c0, BATCH * sizeof(T));
+        } else {
+#pragma unroll
+          for (int i = 0; i < BATCH; ++i) {
+            kc[i] = c0 + i < row_end ? kr[c0 + i] : from_f32<T>(0.f);
+            qc[i] = c0 + i < row_end ? qr[c0 + i] : from_f32<T>(0.f);
+          }
+        }
+#pragma unroll
+        for (int i = 0; i < BATCH; ++i) {
+          if (EDGE && c0 + i >= row_end) continue;
+          const float ki = to_f32<T>(kc[i]), qi = to_f32<T>(qc[i]);
+#pragma unroll
+          for (int j = 0; j < 4; ++j) {
+            st[i][j] = l * st[i][j] + ki * ve[j];
+            sum[j] += qi * st[i][j];
+          }
+          float* at = S + (int64_t)(c0 + i) * Dv;
+          if (!EDGE || n >= 4) {
+            __builtin_memcpy(at, &st[i], 16);
+          } else {
+#pragma unroll
+            for (int j = 0; j < 4; ++j)
+              if (j < n) at[j] = st[i][j];
+          }
+        }
+      }
     }
-    o[e] = from_f32<T>(scale * sum);
+#pragma unroll
+    for (int off = LE; off < 64; off *= 2)
+#pragma unroll
+      for (int j = 0; j < 4; ++j) sum[j] += __shfl_xor(sum[j], off, WAVE);
+  }
+  if (rg == 0) {
+#pragma unroll
+    for (int j = 0; j < 4; ++j)
+      if (!EDGE || j < n) o[j] = from_f32<T>(scale * sum[j]);
   }
 }
 
@@ -800,31 +984,25 @@ Rows rows_of(const torch::Tensor& t) {
   return {t.data_ptr(), t.stride(0), t.stride(1), t.dim() == 4 ? t.stride(2) : 0};
 }
 
-bool vec16(const torch::Tensor& t) {
-  const int64_t v = 16 / t.element_size();
-  if (reinterpret_cast<uintptr_t>(t.data_ptr()) % 16 || t.size(3) % v) return false;
-  for (int i = 0; i < 3; ++i)
-    if (t.size(i) > 1 && t.stride(i) % v) return false;
-  return true;
-}
-
 int padded(int64_t d) { return d <= 32 ? 32 : d <= 64 ? 64 : 128; }
 
 struct Split {
   int G, seg_chunks;
 };
 
-// Positions of a chunk: bfloat16's pass takes 64; float16 shares float32's (its
+// Positions of one load: bfloat16's pass takes 64; float16 shares float32's (its
 // range does not hold a state that long histories add up to).
-int chunk_of(torch::ScalarType dt) { return dt == torch::kBFloat16 ? 64 : 16; }
+int chunk_of(torch::ScalarType dt) { return dt == torch::kBFloat16 ? 64 : 32; }
 
 // One workgroup for each (batch, head) where these alone give every CU two;
 // else the history is cut until there are about that many, in segments of at
-// least 256 positions so that the state-only pass and the scan stay small
-// beside the work they split.
+// least 256 positions (64 of the slower float32 pass: 33 x 3 heads of 333, 50 us
+// in two segments of 192, 35 in six of 64), so that the state-only pass and the
+// scan stay small beside the work they split.
 Split split_of(int64_t BH, int64_t L, int C) {
   const int64_t chunks = (L + C - 1) / C;
-  int64_t G = BH ? std::min<int64_t>((512 + BH - 1) / BH, chunks * C / 256) : 1;
+  int64_t G = BH ? std::min<int64_t>((512 + BH - 1) / BH, chunks / (C == 64 ? 4 : 2)) : 1;
+  if (const char* g = getenv("LA_G")) G = std::min<int64_t>(atoi(g), chunks);
   G = std::max<int64_t>(G, 1);
   const int64_t per = std::max<int64_t>((chunks + G - 1) / G, 1);
   return {(int)std::max<int64_t>((chunks + per - 1) / per, 1), (int)per};
@@ -924,8 +1102,6 @@ PassArgs args_of(const torch::Tensor& q, const torch::Tensor& k, const torch::Te
   a.L = q.size(2);
   a.Dc = q.size(3);
   a.De = v.size(3);
-  a.vec_c = vec16(q) && vec16(k);
-  a.vec_e = vec16(v);
   // a state lies in memory as [Dk, Dv]; flipped passes contract over Dv
   a.st_c = flip ? 1 : a.De;
   a.st_e = flip ? a.Dc : 1;
@@ -1025,7 +1201,6 @@ std::vector<torch::Tensor> linear_attention_bwd(
     a.c_pair = a.c_inter = (float)scale;
     a.c_update = 1.f;
     a.x = rows_of(q);
-    a.vec_x = vec16(q);
     if (split) {
       a.seg = seg.data_ptr<float>();
       a.seg_count = count.data_ptr<int>();
@@ -1097,14 +1272,32 @@ torch::Tensor linear_attention_step(torch::Tensor q, torch::Tensor k, torch::Ten
   if (B * H == 0) return out;
   const bool* act = active.has_value() ? active->data_ptr<bool>() : nullptr;
   const int64_t act_b = active.has_value() ? active->stride(0) : 0;
-#define LA_STEP(T)                                                                              \
-  hipLaunchKernelGGL((la_step_kernel<T>), dim3((unsigned)(B * H)), dim3(128), 0, stream,        \
-                     rows_of(q), rows_of(k), rows_of(v), log_decay.data_ptr<float>(),           \
-                     state.data_ptr<float>(), state.stride(0), state.stride(1), act, act_b,     \
-                     reinterpret_cast<T*>(out.data_ptr()), (int)H, (int)Dk, (int)Dv, (float)scale)
-  if (q.scalar_type() == torch::kBFloat16) LA_STEP(__hip_bfloat16);
-  else if (q.scalar_type() == torch::kHalf) LA_STEP(__half);
-  else LA_STEP(float);
+  // 16 lanes across, 8 for heads of up to 32 values; batches of 16 rows where
+  // the rows of a group fill them, else 4
+  const int LE = Dv > 32 ? 16 : 8, RG = 64 / LE;
+  const int64_t waves = B * H * ((Dv + 4 * LE - 1) / (4 * LE));
+  const bool cols = Dv % (4 * LE) == 0;
+  const bool whole16 = cols && Dk % (RG * 16) == 0, whole4 = cols && Dk % (RG * 4) == 0;
+  TORCH_CHECK(waves / 4 < (int64_t(1) << 31), "linear attention: too many (batch, head)s");
+#define LA_STEP(T, LE, BATCH, EDGE)                                                              \
+  hipLaunchKernelGGL((la_step_kernel<T, LE, BATCH, EDGE>), dim3((unsigned)((waves + 3) / 4)),    \
+                     dim3(256), 0, stream, rows_of(q), rows_of(k), rows_of(v),                   \
+                     log_decay.data_ptr<float>(), state.data_ptr<float>(), state.stride(0),      \
+                     state.stride(1), act, act_b, reinterpret_cast<T*>(out.data_ptr()), waves,   \
+                     (int)H, (int)Dk, (int)Dv, (float)scale)
+#define LA_STEP_T(T)                                                                             \
+  do {                                                                                           \
+    if (LE == 16 && whole16) LA_STEP(T, 16, 16, false);                                          \
+    else if (LE == 16 && whole4) LA_STEP(T, 16, 4, false);                                       \
+    else if (LE == 16) LA_STEP(T, 16, 8, true);                                                  \
+    else if (whole16) LA_STEP(T, 8, 16, false);                                                  \
+    else if (whole4) LA_STEP(T, 8, 4, false);                                                    \
+    else LA_STEP(T, 8, 8, true);                                                                 \
+  } while (0)
+  if (q.scalar_type() == torch::kBFloat16) LA_STEP_T(__hip_bfloat16);
+  else if (q.scalar_type() == torch::kHalf) LA_STEP_T(__half);
+  else LA_STEP_T(float);
+#undef LA_STEP_T
 #undef LA_STEP
   HIP_CHECK(hipGetLastError());
   return out;
