@@ -322,7 +322,8 @@ __global__ __launch_bounds__(WM * WN * 64) void gemm_tile(Gemm p) {
   const unsigned band = t / (8 * tn), rows = min(8u, tm - band * 8), in = t - band * 8 * tn;
   const int m0 = (int)(band * 8 + in % rows) * BM, n0 = (int)(in / rows) * BN;
 
-  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+  const int tid = threadIdx.x, lane = tid & 63;
+  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);  // the same for its lanes
   const int lo = lane & 15, g = lane >> 4;
   const int wm = (wave / WN) * (BM / WM), wn = (wave % WN) * (BN / WN);
   const T* a_src = reinterpret_cast<const T*>(p.a);

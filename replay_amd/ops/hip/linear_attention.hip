@@ -80,19 +80,20 @@ __device__ __forceinline__ uint4 load_piece(const T* p, int n) {
 }
 
 // One operand's 32 positions on their way from memory to LDS, where they are
-// float: 16-byte pieces, DP / V threads a row.
-template <typename T, int DP>
+// float: 16-byte pieces, W / V of THREADS threads a row.
+template <typename T, int W, int THREADS>
 struct Rows32 {
-  static constexpr int V = 16 / sizeof(T), ACROSS = DP / V, DOWN = DP * 4 / ACROSS, PIECES = 32 / DOWN;
-  static constexpr int LD = DP + 4;  // rows then start 4 banks apart
+  static constexpr int V = 16 / sizeof(T), ACROSS = W / V, DOWN = THREADS / ACROSS, PIECES = 32 / DOWN;
+  static constexpr int LD = W + 4;  // rows then start 4 banks apart
 
   const T* at;
   int64_t l;
   int left;
   uint4 r[PIECES];
 
-  __device__ __forceinline__ Rows32(const Rows& src, int b, int h, int D) {
-    const int d = (threadIdx.x % ACROSS) * V;
+  // columns from column d0 on, of D
+  __device__ __forceinline__ Rows32(const Rows& src, int b, int h, int d0, int D) {
+    const int d = d0 + (threadIdx.x % ACROSS) * V;
     l = src.l;
     left = D - d;
     at = reinterpret_cast<const T*>(src.p) + b * src.b + h * src.h + (threadIdx.x / ACROSS) * l + d;
@@ -121,22 +122,23 @@ struct Rows32 {
 
 // One segment of one (batch, head) on the float32 matrix instructions: 16
 // positions a chunk (the pair products grow with it, and these instructions
-// have a sixteenth of the 16-bit ones' rate), 32 a load.  DP/16 waves; each
+// have a sixteenth of the 16-bit ones' rate), 32 a load.  DE/16 waves; each
 // owns 16 value columns and the whole contraction axis of the state, in the
 // accumulator layout (column = lane & 15, row = 4 (lane >> 4) + r), which is
 // also the layout of an operand whose contraction index is visited in that
 // order: neither the state nor the pair weights leave the registers between
-// products.
-template <typename T, int DP, bool REV, bool STATE_ONLY, bool DERIV>
-__global__ __launch_bounds__(DP * 4, DP == 128 ? 1 : 2) void la_pass_f32(PassArgs a) {
-  using Ch = Rows32<T, DP>;
-  constexpr int C = 16, ROWS = 32, LD = Ch::LD, NT = DP / 16, WAVES = DP / 16;
+// products.  DE value columns a workgroup, chosen as in la_pass_bf16: no spills.
+template <typename T, int DP, int DE, bool REV, bool STATE_ONLY, bool DERIV>
+__global__ __launch_bounds__(DE * 4, DE < DP ? 1 : 2) void la_pass_f32(PassArgs a) {
+  using Ch = Rows32<T, DP, DE * 4>;  // q and k
+  using Cv = Rows32<T, DE, DE * 4>;  // v, x and the outputs
+  constexpr int C = 16, ROWS = 32, LD = Ch::LD, LDV = Cv::LD, NT = DP / 16, WAVES = DE / 16;
   constexpr bool FULL = !STATE_ONLY, X = DERIV && FULL;
   __shared__ __attribute__((aligned(16))) float q_s[FULL ? ROWS * LD : 4];
   __shared__ __attribute__((aligned(16))) float k_s[ROWS * LD];
-  __shared__ __attribute__((aligned(16))) float v_s[ROWS * LD];
-  __shared__ __attribute__((aligned(16))) float o_s[FULL ? ROWS * LD : 4];
-  __shared__ __attribute__((aligned(16))) float x_s[X ? ROWS * LD : 4];
+  __shared__ __attribute__((aligned(16))) float v_s[ROWS * LDV];
+  __shared__ __attribute__((aligned(16))) float o_s[FULL ? ROWS * LDV : 4];
+  __shared__ __attribute__((aligned(16))) float x_s[X ? ROWS * LDV : 4];
   // of each position, within its chunk: the valid ones up to it, and its
   // weights in the product with the start state and in the state's update
   __shared__ __attribute__((aligned(16))) float n_s[ROWS], inter_s[ROWS], update_s[ROWS];
@@ -145,11 +147,14 @@ __global__ __launch_bounds__(DP * 4, DP == 128 ? 1 : 2) void la_pass_f32(PassArg
 
   const int seg = blockIdx.x % a.G;
   const int64_t bh = blockIdx.x / a.G;
+  const int first_e = blockIdx.y * DE;  // this workgroup's value columns
   const int b = bh / a.H, h = bh % a.H;
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  // the wave's index is the same for its lanes, which the compiler cannot see:
+  // what depends on it alone then needs no vector registers and no masks
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int lo = lane & 15, g = lane >> 4;
-  const int e0 = wave * 16, e = e0 + lo;
-  const bool busy = e0 < a.De;
+  const int e0 = wave * 16, e = first_e + e0 + lo;
+  const bool busy = first_e + e0 < a.De;
   const int64_t state_size = (int64_t)a.Dc * a.De;
   const float ld = a.log_decay[h];
   // a decay of zero (log -inf) keeps l^0 = 1
@@ -174,9 +179,13 @@ __global__ __launch_bounds__(DP * 4, DP == 128 ? 1 : 2) void la_pass_f32(PassArg
     }
 #pragma unroll
     for (int t = 0; t < NT; ++t) {
+      // the addresses of a tile at a time: worked out together, they take two
+      // registers for each element of the state
+      int g_t = g;
+      asm volatile("" : "+v"(g_t)::"memory");
 #pragma unroll
       for (int r = 0; r < 4; ++r) {
-        const int c = 16 * t + 4 * g + r;
+        const int c = 16 * t + 4 * g_t + r;
         const bool in = c < a.Dc && e < a.De;
         S[t][r] = (src && in) ? src[c * a.st_c + e * a.st_e] : 0.f;
         if (DERIV) Sd[t][r] = (src_d && in) ? src_d[c * a.st_c + e * a.st_e] : 0.f;
@@ -200,7 +209,8 @@ __global__ __launch_bounds__(DP * 4, DP == 128 ? 1 : 2) void la_pass_f32(PassArg
   auto start_of = [&](int step) { return (REV ? first + last - 1 - step : step) * ROWS; };
   int total = 0;
   float d_decay = 0.f;
-  Ch q_r(a.q, b, h, a.Dc), k_r(a.k, b, h, a.Dc), v_r(a.v, b, h, a.De), x_r(a.x, b, h, a.De);
+  Ch q_r(a.q, b, h, 0, a.Dc), k_r(a.k, b, h, 0, a.Dc);
+  Cv v_r(a.v, b, h, first_e, a.De), x_r(a.x, b, h, first_e, a.De);
   // The mask is read a load ahead of the rows that it says to read.
   const bool* mask = a.mask ? a.mask + b * a.mask_b : nullptr;
   auto look = [&](int step) {
@@ -216,29 +226,29 @@ __global__ __launch_bounds__(DP * 4, DP == 128 ? 1 : 2) void la_pass_f32(PassArg
   };
   T* out = nullptr;
   if (FULL)
-    out = reinterpret_cast<T*>(a.out) + b * a.out_b + h * a.out_h +
-          (threadIdx.x / Ch::ACROSS) * a.out_l + (threadIdx.x % Ch::ACROSS) * Ch::V;
+    out = reinterpret_cast<T*>(a.out) + b * a.out_b + h * a.out_h + first_e +
+          (threadIdx.x / Cv::ACROSS) * a.out_l + (threadIdx.x % Cv::ACROSS) * Cv::V;
   // outputs of the rows at l0 in whole rows, from LDS or zeros
   auto store = [&](int l0, bool zero) {
-    const int row = threadIdx.x / Ch::ACROSS, left = v_r.left;
-    const float* from = o_s + row * LD + (threadIdx.x % Ch::ACROSS) * Ch::V;
+    const int row = threadIdx.x / Cv::ACROSS, left = v_r.left;
+    const float* from = o_s + row * LDV + (threadIdx.x % Cv::ACROSS) * Cv::V;
 #pragma unroll
-    for (int i = 0; i < Ch::PIECES; ++i) {
-      if (l0 + row + Ch::DOWN * i >= a.L || left <= 0) continue;
-      alignas(16) T t[Ch::V];
+    for (int i = 0; i < Cv::PIECES; ++i) {
+      if (l0 + row + Cv::DOWN * i >= a.L || left <= 0) continue;
+      alignas(16) T t[Cv::V];
 #pragma unroll
-      for (int j = 0; j < Ch::V; j += 4) {
+      for (int j = 0; j < Cv::V; j += 4) {
         f32x4 v = {0.f, 0.f, 0.f, 0.f};
-        if (!zero) v = *reinterpret_cast<const f32x4*>(from + i * Ch::DOWN * LD + j);
+        if (!zero) v = *reinterpret_cast<const f32x4*>(from + i * Cv::DOWN * LDV + j);
 #pragma unroll
         for (int r = 0; r < 4; ++r) t[j + r] = from_f32<T>(v[r]);
       }
-      T* p = out + (l0 + Ch::DOWN * i) * a.out_l;
-      if (left >= Ch::V) {
+      T* p = out + (l0 + Cv::DOWN * i) * a.out_l;
+      if (left >= Cv::V) {
         __builtin_memcpy(p, t, 16);
       } else {
 #pragma unroll
-        for (int j = 0; j < Ch::V; ++j)
+        for (int j = 0; j < Cv::V; ++j)
           if (j < left) p[j] = t[j];
       }
     }
@@ -282,13 +292,13 @@ __global__ __launch_bounds__(DP * 4, DP == 128 ? 1 : 2) void la_pass_f32(PassArg
         const unsigned own = (now >> r0) & 0xffffu;
         const int N = __popc(own);
         if (N == 0) {
-          if (FULL) *reinterpret_cast<f32x4*>(o_s + (r0 + lo) * LD + e0 + 4 * g) = f32x4{0.f, 0.f, 0.f, 0.f};
+          if (FULL) *reinterpret_cast<f32x4*>(o_s + (r0 + lo) * LDV + e0 + 4 * g) = f32x4{0.f, 0.f, 0.f, 0.f};
           continue;
         }
         const float* k_c = k_s + r0 * LD;
         float vr[4];
 #pragma unroll
-        for (int r = 0; r < 4; ++r) vr[r] = v_s[(r0 + 4 * g + r) * LD + e];
+        for (int r = 0; r < 4; ++r) vr[r] = v_s[(r0 + 4 * g + r) * LDV + e0 + lo];
         const f32x4 n_j = *reinterpret_cast<const f32x4*>(n_s + r0 + 4 * g);
         if (FULL) {
           const float* q_c = q_s + (r0 + lo) * LD;
@@ -296,6 +306,7 @@ __global__ __launch_bounds__(DP * 4, DP == 128 ? 1 : 2) void la_pass_f32(PassArg
           f32x4 pt = {0.f, 0.f, 0.f, 0.f}, o = pt, od = pt;
 #pragma unroll
           for (int t = 0; t < NT; ++t) {
+            if (DERIV) asm volatile("" ::: "memory");
             const f32x4 qv = *reinterpret_cast<const f32x4*>(q_c + 16 * t + 4 * g);
             const f32x4 kv = *reinterpret_cast<const f32x4*>(k_c + lo * LD + 16 * t + 4 * g);
 #pragma unroll
@@ -328,11 +339,11 @@ __global__ __launch_bounds__(DP * 4, DP == 128 ? 1 : 2) void la_pass_f32(PassArg
             if (DERIV) od = mfma4(vr[r], p[r] * gaps[r], od);
           }
           if (DERIV) {
-            const f32x4 xv = *reinterpret_cast<const f32x4*>(x_s + (r0 + lo) * LD + e0 + 4 * g);
+            const f32x4 xv = *reinterpret_cast<const f32x4*>(x_s + (r0 + lo) * LDV + e0 + 4 * g);
 #pragma unroll
             for (int r = 0; r < 4; ++r) d_decay += xv[r] * od[r];
           }
-          *reinterpret_cast<f32x4*>(o_s + (r0 + lo) * LD + e0 + 4 * g) = o;
+          *reinterpret_cast<f32x4*>(o_s + (r0 + lo) * LDV + e0 + 4 * g) = o;
         }
         const bool update = want_end || step + 1 < last || half == 0;
         if (started && update) {
@@ -349,6 +360,7 @@ __global__ __launch_bounds__(DP * 4, DP == 128 ? 1 : 2) void la_pass_f32(PassArg
         const f32x4 left = REV ? n_j : (float)N - n_j;
 #pragma unroll
         for (int r = 0; r < 4; ++r) {
+          if (DERIV) asm volatile("" ::: "memory");
           const float weighted = vr[r] * w[r];
 #pragma unroll
           for (int t = 0; t < NT; ++t) {
@@ -368,16 +380,18 @@ __global__ __launch_bounds__(DP * 4, DP == 128 ? 1 : 2) void la_pass_f32(PassArg
   if (STATE_ONLY) {
     dst = a.seg + (bh * a.G + seg) * state_size;
     if (DERIV) dst_d = a.seg_d + (bh * a.G + seg) * state_size;
-    if (threadIdx.x == 0) a.seg_count[bh * a.G + seg] = total;
+    if (threadIdx.x == 0 && blockIdx.y == 0) a.seg_count[bh * a.G + seg] = total;
   } else if (at_end && a.state_out) {
     dst = a.state_out + bh * state_size;
   }
   const float* end_grad = (X && at_end && a.state_end_grad) ? a.state_end_grad + bh * state_size : nullptr;
 #pragma unroll
   for (int t = 0; t < NT; ++t) {
+    int g_t = g;
+    asm volatile("" : "+v"(g_t)::"memory");
 #pragma unroll
     for (int r = 0; r < 4; ++r) {
-      const int c = 16 * t + 4 * g + r;
+      const int c = 16 * t + 4 * g_t + r;
       if (c < a.Dc && e < a.De) {
         const int64_t at = c * a.st_c + e * a.st_e;
         if (dst) dst[at] = S[t][r];
@@ -393,7 +407,7 @@ __global__ __launch_bounds__(DP * 4, DP == 128 ? 1 : 2) void la_pass_f32(PassArg
     if (threadIdx.x == 0) {
       float sum = 0.f;
       for (int w = 0; w < WAVES; ++w) sum += red[w];
-      a.decay_part[bh * a.G + seg] = sum;
+      a.decay_part[(bh * a.G + seg) * gridDim.y + blockIdx.y] = sum;
     }
   }
 }
@@ -407,10 +421,11 @@ __global__ __launch_bounds__(DP * 4, DP == 128 ? 1 : 2) void la_pass_f32(PassArg
 // 8g .. 8g+7, to which the rows of the state's tiles are permuted.  Everything
 // comes from row-major LDS tiles, the transposed operands by transposing reads.
 //
-// Each wave computes all pair products for itself: 20 of its 58 matrix
-// instructions a chunk at head size 64, which costs less than sharing them
-// through LDS would, since the card's memory is the bound (64 positions of one
-// head are 32 KB, some 2500 cycles of a CU's share, against 930 of products).
+// The pair weights of a chunk are 6 units of a tile row by 32 keys (those on
+// one side of the diagonal), shared out among the waves and handed round through
+// LDS in operand layout.  (Each wave computing all of them took 90 more vector
+// and 14 more matrix instructions a chunk at head size 64, and at 128, where 8
+// waves did so, twice the time.)
 //
 // Roundings to bfloat16: the pair weights, once (half a step of each term).
 // The state goes into the outputs as the sum of two bfloat16s (2^-17), into
@@ -490,37 +505,40 @@ __device__ __forceinline__ void store8(__hip_bfloat16* p, int n, uint4 v) {
   }
 }
 
-// One operand's 64 positions on their way from memory to LDS, two 16-byte
-// pieces a thread: rows row and row + 32 of the chunk, columns d .. d + 7.
-template <int DP, bool EDGE>
+// One operand's 64 positions on their way from memory to LDS: 16-byte pieces,
+// W / 8 of THREADS threads a row.
+template <int W, int THREADS, bool EDGE>
 struct Chunk {
-  static constexpr int C = 64, NT = DP * 4;
+  static constexpr int C = 64, ACROSS = W / 8, DOWN = THREADS / ACROSS, PIECES = C / DOWN;
   // rows 16 bytes apart from a power of two: the fragment reads of 16 rows
   // then start in banks 4 words apart
-  static constexpr int LD = DP * 2 + 16, BYTES = C * LD;
+  static constexpr int LD = W * 2 + 16, BYTES = C * LD;
 
   const __hip_bfloat16* at;  // this thread's first piece of position 0
   int64_t l;
   int left;                  // columns from d on that exist
-  uint4 r[2];
+  uint4 r[PIECES];
 
-  __device__ __forceinline__ Chunk(const Rows& src, int b, int h, int D) {
-    const int d = (threadIdx.x % (DP / 8)) * 8;
+  // columns from column d0 on, of D
+  __device__ __forceinline__ Chunk(const Rows& src, int b, int h, int d0, int D) {
+    const int d = d0 + (threadIdx.x % ACROSS) * 8;
     l = src.l;
     left = D - d;
     at = reinterpret_cast<const __hip_bfloat16*>(src.p) + b * src.b + h * src.h +
-         (threadIdx.x / (DP / 8)) * l + d;
+         (threadIdx.x / ACROSS) * l + d;
   }
   __device__ __forceinline__ void fetch(int l0, uint64_t bits) {
-    const uint64_t mine = bits >> (threadIdx.x / (DP / 8));
-    r[0] = r[1] = uint4{0, 0, 0, 0};
-    if ((mine & 1) && left > 0) r[0] = load8<EDGE>(at + l0 * l, left);
-    if (((mine >> 32) & 1) && left > 0) r[1] = load8<EDGE>(at + (l0 + 32) * l, left);
+    const uint64_t mine = bits >> (threadIdx.x / ACROSS);
+#pragma unroll
+    for (int i = 0; i < PIECES; ++i) {
+      r[i] = uint4{0, 0, 0, 0};
+      if (((mine >> (i * DOWN)) & 1) && left > 0) r[i] = load8<EDGE>(at + (l0 + i * DOWN) * l, left);
+    }
   }
   __device__ __forceinline__ void put(char* dst) const {
-    dst += (threadIdx.x / (DP / 8)) * LD + (threadIdx.x % (DP / 8)) * 16;
-    *reinterpret_cast<uint4*>(dst) = r[0];
-    *reinterpret_cast<uint4*>(dst + 32 * LD) = r[1];
+    dst += (threadIdx.x / ACROSS) * LD + (threadIdx.x % ACROSS) * 16;
+#pragma unroll
+    for (int i = 0; i < PIECES; ++i) *reinterpret_cast<uint4*>(dst + i * DOWN * LD) = r[i];
   }
   // operand rows row0 + (lane & 15), contraction block s of the head size
   static __device__ __forceinline__ bf16x8 rows(const char* t, int row0, int s, int lo, int g) {
@@ -545,17 +563,23 @@ __device__ __forceinline__ int state_row(int t, int g, int r) {
   return 32 * (t >> 1) + 8 * g + 4 * (t & 1) + r;
 }
 
-template <int DP, bool REV, bool STATE_ONLY, bool DERIV, bool EDGE>
-__global__ __launch_bounds__(DP * 4, DP == 128 || DERIV ? 2 : 3) void la_pass_bf16(PassArgs a) {
-  using Ch = Chunk<DP, EDGE>;
-  constexpr int C = 64, NS = DP / 32, NT = DP / 16, LD = Ch::LD;
-  constexpr int WAVES = DP / 16;
+// DE value columns a workgroup, DE / 16 waves of 16.  The launch bounds are the
+// tightest that need no spills: with spills, first chunks came out wrong now and
+// then.  The decay's gradient at head size 128 does not fit 256 registers a
+// lane; there a workgroup takes half the value columns, in 4 waves of up to 512.
+template <int DP, int DE, bool REV, bool STATE_ONLY, bool DERIV, bool EDGE>
+__global__ __launch_bounds__(DE * 4, DE < DP ? 1 : DERIV || DP > 32 ? 2 : 3) void la_pass_bf16(PassArgs a) {
+  using Ch = Chunk<DP, DE * 4, EDGE>;  // q and k
+  using Cv = Chunk<DE, DE * 4, EDGE>;  // v, x and the outputs
+  constexpr int C = 64, NS = DP / 32, NT = DP / 16, LDV = Cv::LD;
+  constexpr int WAVES = DE / 16;
   constexpr bool FULL = !STATE_ONLY, X = DERIV && FULL;
   __shared__ __attribute__((aligned(16))) char q_s[FULL ? Ch::BYTES : 16];
   __shared__ __attribute__((aligned(16))) char k_s[Ch::BYTES];
-  __shared__ __attribute__((aligned(16))) char v_s[Ch::BYTES];
-  __shared__ __attribute__((aligned(16))) char o_s[FULL ? Ch::BYTES : 16];
-  __shared__ __attribute__((aligned(16))) char x_s[X ? Ch::BYTES : 16];
+  __shared__ __attribute__((aligned(16))) char v_s[Cv::BYTES];
+  __shared__ uint4 p_s[FULL ? 6 : 1][64];    // pair weights, as operands
+  __shared__ f32x4 full_s[FULL ? 4 : 1][64]; // those of a chunk without gaps, by tile distance
+  __shared__ __attribute__((aligned(16))) char x_s[X ? Cv::BYTES : 16];
   // of each position: the valid ones up to it, and its weights in the product
   // with the start state and in the state's update
   __shared__ __attribute__((aligned(16))) float n_s[C], inter_s[C], update_s[C];
@@ -564,15 +588,18 @@ __global__ __launch_bounds__(DP * 4, DP == 128 || DERIV ? 2 : 3) void la_pass_bf
 
   const int seg = blockIdx.x % a.G;
   const int64_t bh = blockIdx.x / a.G;
+  const int first_e = blockIdx.y * DE;  // this workgroup's value columns
   const int b = bh / a.H, h = bh % a.H;
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  // the wave's index is the same for its lanes, which the compiler cannot see:
+  // what depends on it alone then needs no vector registers and no masks
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int lo = lane & 15, g = lane >> 4;
-  const int e0 = wave * 16, e = e0 + lo;
-  const bool busy = e0 < a.De;
+  const int e0 = wave * 16, e = first_e + e0 + lo;
+  const bool busy = first_e + e0 < a.De;
   const int64_t state_size = (int64_t)a.Dc * a.De;
   const float ld = a.log_decay[h];
   // a decay of zero (log -inf) keeps l^0 = 1
-  for (int i = threadIdx.x; i <= C; i += Ch::NT) lam[i] = i ? expf(ld * i) : 1.f;
+  for (int i = threadIdx.x; i <= C; i += DE * 4) lam[i] = i ? expf(ld * i) : 1.f;
 
   // false while the state is known to be zero, as a history's first chunk has it
   bool started = FULL && (a.G > 1 || a.state_in);
@@ -593,9 +620,13 @@ __global__ __launch_bounds__(DP * 4, DP == 128 || DERIV ? 2 : 3) void la_pass_bf
     }
 #pragma unroll
     for (int t = 0; t < NT; ++t) {
+      // the addresses of a tile at a time: worked out together, they take two
+      // registers for each element of the state
+      int g_t = g;
+      asm volatile("" : "+v"(g_t)::"memory");
 #pragma unroll
       for (int r = 0; r < 4; ++r) {
-        const int c = state_row(t, g, r);
+        const int c = state_row(t, g_t, r);
         const bool in = c < a.Dc && e < a.De;
         S[t][r] = (src && in) ? src[c * a.st_c + e * a.st_e] : 0.f;
         if (DERIV) Sd[t][r] = (src_d && in) ? src_d[c * a.st_c + e * a.st_e] : 0.f;
@@ -604,25 +635,27 @@ __global__ __launch_bounds__(DP * 4, DP == 128 || DERIV ? 2 : 3) void la_pass_bf
   }
   __syncthreads();  // lam
 
-  // The pair weights of a chunk without gaps, by the distance of the tiles.
-  f32x4 full[FULL ? 4 : 1];
   if (FULL) {
-#pragma unroll
-    for (int d = 0; d < 4; ++d) {
+    for (int d = wave; d < 4; d += WAVES) {
 #pragma unroll
       for (int r = 0; r < 4; ++r) {
         const int gap = 16 * d + (REV ? 4 * g + r - lo : lo - 4 * g - r);
-        full[d][r] = gap >= 0 ? a.c_pair * lam[max(gap, 0)] : 0.f;
+        full_s[d][lane][r] = gap >= 0 ? a.c_pair * lam[max(gap, 0)] : 0.f;
       }
     }
   }
+  // Unit u: tile row it by key block s; the first four have two tiles each, the
+  // last two one.  Mirrored in the reversed pass.
+  auto unit_it = [](int u) { const int it = (0x203321 >> (4 * u)) & 15; return REV ? 3 - it : it; };
+  auto unit_s = [](int u) { const int s = (0x101000 >> (4 * u)) & 15; return REV ? 1 - s : s; };
 
   const int n_chunks = (a.L + C - 1) / C;
   const int first = seg * a.seg_chunks, last = min(n_chunks, first + a.seg_chunks);
   auto start_of = [&](int step) { return (REV ? first + last - 1 - step : step) * C; };
   int total = 0;
   float d_decay = 0.f;
-  Ch q_r(a.q, b, h, a.Dc), k_r(a.k, b, h, a.Dc), v_r(a.v, b, h, a.De), x_r(a.x, b, h, a.De);
+  Ch q_r(a.q, b, h, 0, a.Dc), k_r(a.k, b, h, 0, a.Dc);
+  Cv v_r(a.v, b, h, first_e, a.De), x_r(a.x, b, h, first_e, a.De);
   // The mask is read a chunk ahead of the rows that it says to read.
   const bool* mask = a.mask ? a.mask + b * a.mask_b : nullptr;
   auto look = [&](int step) {
@@ -638,18 +671,19 @@ __global__ __launch_bounds__(DP * 4, DP == 128 || DERIV ? 2 : 3) void la_pass_bf
   };
   __hip_bfloat16* out = nullptr;
   if (FULL)
-    out = reinterpret_cast<__hip_bfloat16*>(a.out) + b * a.out_b + h * a.out_h +
-          (threadIdx.x / (DP / 8)) * a.out_l + (threadIdx.x % (DP / 8)) * 8;
-  // outputs of the chunk at l0 in whole rows, from LDS or zeros
+    out = reinterpret_cast<__hip_bfloat16*>(a.out) + b * a.out_b + h * a.out_h + first_e +
+          (threadIdx.x / Cv::ACROSS) * a.out_l + (threadIdx.x % Cv::ACROSS) * 8;
+  // outputs of the chunk at l0 in whole rows, from LDS (where they take v's
+  // place: a thread reads what it alone will overwrite) or zeros
   auto store = [&](int l0, bool zero) {
-    const int row = threadIdx.x / (DP / 8), left = v_r.left;
-    const char* from = o_s + row * LD + (threadIdx.x % (DP / 8)) * 16;
+    const int row = threadIdx.x / Cv::ACROSS, left = v_r.left;
+    const char* from = v_s + row * LDV + (threadIdx.x % Cv::ACROSS) * 16;
 #pragma unroll
-    for (int i = 0; i < 2; ++i) {
-      if (l0 + row + 32 * i >= a.L || left <= 0) continue;
+    for (int i = 0; i < Cv::PIECES; ++i) {
+      if (l0 + row + Cv::DOWN * i >= a.L || left <= 0) continue;
       uint4 v = {0, 0, 0, 0};
-      if (!zero) v = *reinterpret_cast<const uint4*>(from + 32 * i * LD);
-      store8<EDGE>(out + (l0 + 32 * i) * a.out_l, left, v);
+      if (!zero) v = *reinterpret_cast<const uint4*>(from + i * Cv::DOWN * LDV);
+      store8<EDGE>(out + (l0 + Cv::DOWN * i) * a.out_l, left, v);
     }
   };
 
@@ -684,99 +718,123 @@ __global__ __launch_bounds__(DP * 4, DP == 128 || DERIV ? 2 : 3) void la_pass_bf
     fetch(step + 1, bits);
     ahead = look(step + 2);
 
-    if (busy) {
-      bf16x8 vf[2];
+    const float all = (float)N;
+    if (FULL) {
+      // valid positions in one run: n_i - n_j = i - j wherever a pair counts
+      const uint64_t run = now >> __builtin_ctzll(now);
+      const bool whole = (run & (run + 1)) == 0;
+#pragma unroll 1
+      for (int unit = wave; unit < 6; unit += WAVES) {
+        const int it = unit_it(unit), s = unit_s(unit), i = 16 * it + lo;
+        const float n_i = n_s[i];
+        bf16x8 qf[NS];
 #pragma unroll
-      for (int s = 0; s < 2; ++s) vf[s] = Ch::columns(v_s, e0, 4, s, lo, g);
-      const float all = (float)N;
+        for (int c = 0; c < NS; ++c) qf[c] = Ch::rows(q_s, 16 * it, c, lo, g);
+        f32x4 p[2];
+#pragma unroll
+        for (int u = 0; u < 2; ++u) {
+          const int jt = 2 * s + u, apart = REV ? jt - it : it - jt;
+          p[u] = f32x4{0.f, 0.f, 0.f, 0.f};
+          if (apart < 0) continue;
+          f32x4 acc = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+          for (int c = 0; c < NS; ++c) acc = mfma32(Ch::rows(k_s, 16 * jt, c, lo, g), qf[c], acc);
+          f32x4 gaps;
+          if (DERIV || !whole) {
+            const f32x4 n_j = *reinterpret_cast<const f32x4*>(n_s + 16 * jt + 4 * g);
+            gaps = REV ? n_j - n_i : n_i - n_j;
+          }
+          if (whole) {
+            p[u] = acc * full_s[apart][lane];
+          } else {
+            f32x4 w;
+#pragma unroll
+            for (int r = 0; r < 4; ++r) w[r] = lam[max((int)gaps[r], 0)];
+#pragma unroll
+            for (int r = 0; r < 4; ++r) {
+              const bool seen = apart > 0 || (REV ? 4 * g + r >= lo : 4 * g + r <= lo);
+              p[u][r] = seen ? acc[r] * (a.c_pair * w[r]) : 0.f;
+            }
+          }
+          if (DERIV) {  // sum of gap weight (q_i.k_j) (x_i.v_j)
+            asm volatile("" ::: "memory");
+            f32x4 other = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+            for (int c = 0; c < DE / 32; ++c)
+              other = mfma32(Cv::rows(v_s, 16 * jt, c, lo, g), Cv::rows(x_s, 16 * it, c, lo, g), other);
+#pragma unroll
+            for (int r = 0; r < 4; ++r) d_decay += p[u][r] * gaps[r] * other[r];
+          }
+        }
+        p_s[unit][lane] = __builtin_bit_cast(uint4, pack8(p[0], p[1]));
+      }
+    }
+
+    bf16x8 vf[2];
+    f32x4 o[FULL ? 4 : 1];
+    if (busy) {
+#pragma unroll
+      for (int s = 0; s < 2; ++s) vf[s] = Cv::columns(v_s, e0, 4, s, lo, g);
 
       if (FULL) {
-        // valid positions in one run: n_i - n_j = i - j wherever a pair counts
-        const uint64_t run = now >> __builtin_ctzll(now);
-        const bool whole = (run & (run + 1)) == 0;
         // the start state's part, a block of the contraction at a time: so the
         // split state needs registers for one block only
-        f32x4 os[4] = {}, ods[DERIV ? 4 : 1] = {};
 #pragma unroll
-        for (int s = 0; s < NS && started; ++s) {
-          asm volatile("" ::: "memory");
-          const Split8<DERIV ? 3 : 2> state(S[2 * s], S[2 * s + 1]);
-          const Split8<3> state_d(Sd[DERIV ? 2 * s : 0], Sd[DERIV ? 2 * s + 1 : 0]);
+        for (int it = 0; it < 4; ++it) o[it] = f32x4{0.f, 0.f, 0.f, 0.f};
+        if (started) {
+          // what of the decay's gradient goes by x . (S' q) w, a block at a time too
+          auto weighted_x = [&](int it) {
+            return inter_s[16 * it + lo] *
+                   widen(*reinterpret_cast<const bf16x4*>(x_s + (16 * it + lo) * LDV + (e0 + 4 * g) * 2));
+          };
 #pragma unroll
-          for (int it = 0; it < 4; ++it) {
-            const bf16x8 qf = Ch::rows(q_s, 16 * it, s, lo, g);
-            os[it] = state.times(qf, os[it]);
-            if (DERIV) ods[it] = state_d.times(qf, ods[it]);
-          }
-        }
+          for (int s = 0; s < NS; ++s) {
+            asm volatile("" ::: "memory");
+            const Split8<DERIV ? 3 : 2> state(S[2 * s], S[2 * s + 1]);
 #pragma unroll
-        for (int it = 0; it < 4; ++it) {
-          // one tile row at a time: overlapped, they need more registers than
-          // leaves three workgroups a CU
-          asm volatile("" ::: "memory");
-          bf16x8 qf[NS];
+            for (int it = 0; it < 4; ++it) {
+              if (DERIV) asm volatile("" ::: "memory");
+              o[it] = state.times(Ch::rows(q_s, 16 * it, s, lo, g), o[it]);
+            }
+            if (DERIV) {
+              asm volatile("" ::: "memory");
+              const Split8<3> state_d(Sd[DERIV ? 2 * s : 0], Sd[DERIV ? 2 * s + 1 : 0]);
 #pragma unroll
-          for (int s = 0; s < NS; ++s) qf[s] = Ch::rows(q_s, 16 * it, s, lo, g);
-          f32x4 o = os[it], od;
-          if (DERIV) od = ods[it];
-          const int i = 16 * it + lo;
-          const float n_i = n_s[i], w_i = inter_s[i];
-          if (DERIV) {
-            od = w_i * (od + n_i * o);
-            const f32x4 xv = widen(*reinterpret_cast<const bf16x4*>(x_s + i * LD + (e0 + 4 * g) * 2));
-#pragma unroll
-            for (int r = 0; r < 4; ++r) d_decay += xv[r] * od[r];
-          }
-          o = w_i * o;
-          // pairs with the keys of tiles 2 s and 2 s + 1
-#pragma unroll
-          for (int s = 0; s < 2; ++s) {
-            if (REV ? 2 * s + 1 < it : 2 * s > it) continue;
-            f32x4 p[2];
-#pragma unroll
-            for (int u = 0; u < 2; ++u) {
-              const int jt = 2 * s + u, apart = REV ? jt - it : it - jt;
-              p[u] = f32x4{0.f, 0.f, 0.f, 0.f};
-              if (apart < 0) continue;
-              f32x4 acc = {0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-              for (int c = 0; c < NS; ++c) acc = mfma32(Ch::rows(k_s, 16 * jt, c, lo, g), qf[c], acc);
-              f32x4 gaps;
-              if (DERIV || !whole) {
-                const f32x4 n_j = *reinterpret_cast<const f32x4*>(n_s + 16 * jt + 4 * g);
-                gaps = REV ? n_j - n_i : n_i - n_j;
-              }
-              if (whole) {
-                p[u] = acc * full[apart < 0 ? 0 : apart];
-              } else {
-                f32x4 w;
-#pragma unroll
-                for (int r = 0; r < 4; ++r) w[r] = lam[max((int)gaps[r], 0)];
-#pragma unroll
-                for (int r = 0; r < 4; ++r) {
-                  const int j = 4 * g + r;
-                  const bool seen = apart > 0 || (REV ? j >= lo : j <= lo);
-                  p[u][r] = seen ? acc[r] * (a.c_pair * w[r]) : 0.f;
-                }
-              }
-              if (DERIV) {
-                // sum of gap weight (q_i.k_j) (x_i.v_j): each tile by one wave
-                if ((4 * it + jt) % ((a.De + 15) / 16) == wave) {
-                  f32x4 other = {0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-                  for (int c = 0; c < NS; ++c)
-                    other = mfma32(Ch::rows(v_s, 16 * jt, c, lo, g), Ch::rows(x_s, 16 * it, c, lo, g), other);
-#pragma unroll
-                  for (int r = 0; r < 4; ++r) d_decay += p[u][r] * gaps[r] * other[r];
-                }
+              for (int it = 0; it < 4; ++it) {
+                asm volatile("" ::: "memory");
+                const f32x4 od = state_d.times(Ch::rows(q_s, 16 * it, s, lo, g), f32x4{0.f, 0.f, 0.f, 0.f});
+                const f32x4 part = weighted_x(it) * od;
+                d_decay += (part[0] + part[1]) + (part[2] + part[3]);
               }
             }
-            o = mfma32(vf[s], pack8(p[0], p[1]), o);
           }
-          *reinterpret_cast<bf16x4*>(o_s + i * LD + (e0 + 4 * g) * 2) = __builtin_convertvector(o, bf16x4);
+#pragma unroll
+          for (int it = 0; it < 4; ++it) {
+            if (DERIV) {
+              const f32x4 part = weighted_x(it) * o[it];
+              d_decay += n_s[16 * it + lo] * ((part[0] + part[1]) + (part[2] + part[3]));
+            }
+            o[it] = inter_s[16 * it + lo] * o[it];
+          }
         }
       }
+    }
 
+    if (FULL) {
+      __syncthreads();  // the pair weights are there, and v is read
+      if (busy) {
+#pragma unroll
+        for (int u = 0; u < 6; ++u) {
+          const int it = unit_it(u), s = unit_s(u);
+          o[it] = mfma32(vf[s], __builtin_bit_cast(bf16x8, p_s[u][lane]), o[it]);
+        }
+#pragma unroll
+        for (int it = 0; it < 4; ++it)
+          *reinterpret_cast<bf16x4*>(v_s + (16 * it + lo) * LDV + (e0 + 4 * g) * 2) =
+              __builtin_convertvector(o[it], bf16x4);
+      }
+    }
+    if (busy) {
       const bool update = want_end || step + 1 < last;
       if (started && update) {
         const float lN = lam[N];
@@ -790,24 +848,29 @@ __global__ __launch_bounds__(DP * 4, DP == 128 || DERIV ? 2 : 3) void la_pass_bf
 #pragma unroll
       for (int s = 0; s < 2 && update; ++s) {
         asm volatile("" ::: "memory");
-        f32x4 w[2], wd[2] = {};
+        f32x4 w[2];
         const uint4 raw = __builtin_bit_cast(uint4, vf[s]);
 #pragma unroll
-        for (int i = 0; i < 2; ++i) {
-          const int j0 = 32 * s + 16 * i + 4 * g;
+        for (int i = 0; i < 2; ++i)
           w[i] = widen(__builtin_bit_cast(bf16x4, i ? uint2{raw.z, raw.w} : uint2{raw.x, raw.y})) *
-                 *reinterpret_cast<const f32x4*>(update_s + j0);
-          if (DERIV) {
-            const f32x4 n_j = *reinterpret_cast<const f32x4*>(n_s + j0);
-            wd[i] = w[i] * (REV ? n_j : all - n_j);
-          }
-        }
-        const Split8<3> weighted(w[0], w[1]), weighted_d(wd[0], wd[1]);
+                 *reinterpret_cast<const f32x4*>(update_s + 32 * s + 16 * i + 4 * g);
+        auto add = [&](f32x4* state) {
+          const Split8<3> weighted(w[0], w[1]);
 #pragma unroll
-        for (int t = 0; t < NT; ++t) {
-          const bf16x8 kf = Ch::columns(k_s, state_row(t, 0, 0), 8, s, lo, g);
-          S[t] = weighted.after(kf, S[t]);
-          if (DERIV) Sd[t] = weighted_d.after(kf, Sd[t]);
+          for (int t = 0; t < NT; ++t) {
+            if (DERIV && t % 2 == 0) asm volatile("" ::: "memory");
+            state[t] = weighted.after(Ch::columns(k_s, state_row(t, 0, 0), 8, s, lo, g), state[t]);
+          }
+        };
+        add(S);
+        if (DERIV) {
+          asm volatile("" ::: "memory");
+#pragma unroll
+          for (int i = 0; i < 2; ++i) {
+            const f32x4 n_j = *reinterpret_cast<const f32x4*>(n_s + 32 * s + 16 * i + 4 * g);
+            w[i] = w[i] * (REV ? n_j : all - n_j);
+          }
+          add(Sd);
         }
       }
     }
@@ -820,16 +883,18 @@ __global__ __launch_bounds__(DP * 4, DP == 128 || DERIV ? 2 : 3) void la_pass_bf
   if (STATE_ONLY) {
     dst = a.seg + (bh * a.G + seg) * state_size;
     if (DERIV) dst_d = a.seg_d + (bh * a.G + seg) * state_size;
-    if (threadIdx.x == 0) a.seg_count[bh * a.G + seg] = total;
+    if (threadIdx.x == 0 && blockIdx.y == 0) a.seg_count[bh * a.G + seg] = total;
   } else if (at_end && a.state_out) {
     dst = a.state_out + bh * state_size;
   }
   const float* end_grad = (X && at_end && a.state_end_grad) ? a.state_end_grad + bh * state_size : nullptr;
 #pragma unroll
   for (int t = 0; t < NT; ++t) {
+    int g_t = g;
+    asm volatile("" : "+v"(g_t)::"memory");
 #pragma unroll
     for (int r = 0; r < 4; ++r) {
-      const int c = state_row(t, g, r);
+      const int c = state_row(t, g_t, r);
       if (c < a.Dc && e < a.De) {
         const int64_t at = c * a.st_c + e * a.st_e;
         if (dst) dst[at] = S[t][r];
@@ -845,7 +910,7 @@ __global__ __launch_bounds__(DP * 4, DP == 128 || DERIV ? 2 : 3) void la_pass_bf
     if (threadIdx.x == 0) {
       float sum = 0.f;
       for (int w = 0; w < WAVES; ++w) sum += red[w];
-      a.decay_part[bh * a.G + seg] = sum;
+      a.decay_part[(bh * a.G + seg) * gridDim.y + blockIdx.y] = sum;
     }
   }
 }
@@ -994,15 +1059,16 @@ struct Split {
 // range does not hold a state that long histories add up to).
 int chunk_of(torch::ScalarType dt) { return dt == torch::kBFloat16 ? 64 : 32; }
 
-// One workgroup for each (batch, head) where these alone give every CU two;
-// else the history is cut until there are about that many, in segments of at
-// least 256 positions (64 of the slower float32 pass: 33 x 3 heads of 333, 50 us
-// in two segments of 192, 35 in six of 64), so that the state-only pass and the
-// scan stay small beside the work they split.
-Split split_of(int64_t BH, int64_t L, int C) {
-  const int64_t chunks = (L + C - 1) / C;
-  int64_t G = BH ? std::min<int64_t>((512 + BH - 1) / BH, chunks / (C == 64 ? 4 : 2)) : 1;
-  if (const char* g = getenv("LA_G")) G = std::min<int64_t>(atoi(g), chunks);
+// One workgroup for each (batch, head) where these alone fill the card (two a
+// CU; one, of 8 waves, at head sizes past 64); else the history is cut until
+// there are about that many, in segments of at least 256 positions (64 of the
+// slower float32 pass: 33 x 3 heads of 333, 50 us in two segments of 192, 35 in
+// six of 64), so that the state-only pass and the scan stay small beside the
+// work they split.  2 x 8 heads of 16384 at head size 128, by segments: 16, 146
+// us; 32, 165; 64, 189; 4, 473.
+Split split_of(int64_t BH, int64_t L, int64_t D, int C) {
+  const int64_t chunks = (L + C - 1) / C, want = D > 64 ? 256 : 512;
+  int64_t G = BH ? std::min<int64_t>((want + BH - 1) / BH, chunks / (C == 64 ? 4 : 2)) : 1;
   G = std::max<int64_t>(G, 1);
   const int64_t per = std::max<int64_t>((chunks + G - 1) / G, 1);
   return {(int)std::max<int64_t>((chunks + per - 1) / per, 1), (int)per};
@@ -1014,18 +1080,21 @@ void launch_pass(torch::ScalarType dt, const PassArgs& a, hipStream_t stream) {
   TORCH_CHECK(blocks < (int64_t(1) << 31), "linear attention: too many (batch, head, segment)s");
   const int dp = padded(std::max(a.Dc, a.De));
   const bool edge = a.Dc % 8 || a.De % 8;
-#define LA_LAUNCH(DP, ...)                                                                   \
-  hipLaunchKernelGGL((__VA_ARGS__), dim3((unsigned)blocks), dim3(DP * 4), 0, stream, a)
-#define LA_PASS(DP)                                                                          \
-  do {                                                                                       \
-    if (dt == torch::kBFloat16 && edge) LA_LAUNCH(DP, la_pass_bf16<DP, REV, STATE_ONLY, DERIV, true>); \
-    else if (dt == torch::kBFloat16) LA_LAUNCH(DP, la_pass_bf16<DP, REV, STATE_ONLY, DERIV, false>); \
-    else if (dt == torch::kHalf) LA_LAUNCH(DP, la_pass_f32<__half, DP, REV, STATE_ONLY, DERIV>); \
-    else LA_LAUNCH(DP, la_pass_f32<float, DP, REV, STATE_ONLY, DERIV>);                      \
+#define LA_LAUNCH(DE, ...)                                                                         \
+  hipLaunchKernelGGL((__VA_ARGS__), dim3((unsigned)blocks, (unsigned)((a.De + DE - 1) / DE)),      \
+                     dim3(DE * 4), 0, stream, a)
+#define LA_PASS(DP, DE)                                                                            \
+  do {                                                                                             \
+    if (dt == torch::kBFloat16 && edge)                                                            \
+      LA_LAUNCH(DE, la_pass_bf16<DP, DE, REV, STATE_ONLY, DERIV, true>);                           \
+    else if (dt == torch::kBFloat16) LA_LAUNCH(DE, la_pass_bf16<DP, DE, REV, STATE_ONLY, DERIV, false>); \
+    else if (dt == torch::kHalf) LA_LAUNCH(DE, la_pass_f32<__half, DP, DE, REV, STATE_ONLY, DERIV>); \
+    else LA_LAUNCH(DE, la_pass_f32<float, DP, DE, REV, STATE_ONLY, DERIV>);                        \
   } while (0)
-  if (dp == 32) LA_PASS(32);
-  else if (dp == 64) LA_PASS(64);
-  else LA_PASS(128);
+  if (dp == 32) LA_PASS(32, 32);
+  else if (dp == 64) LA_PASS(64, 64);
+  else if constexpr (DERIV && !STATE_ONLY) LA_PASS(128, 64);
+  else LA_PASS(128, 128);
 #undef LA_PASS
 #undef LA_LAUNCH
   HIP_CHECK(hipGetLastError());
@@ -1137,7 +1206,7 @@ std::vector<torch::Tensor> linear_attention_fwd(torch::Tensor q, torch::Tensor k
 
   PassArgs a = args_of(q, k, v, log_decay, mask, false);
   set_out(a, out);
-  const Split s = split_of(B * H, L, chunk_of(q.scalar_type()));
+  const Split s = split_of(B * H, L, std::max(Dk, Dv), chunk_of(q.scalar_type()));
   a.G = s.G;
   a.seg_chunks = s.seg_chunks;
   a.state_in = state.has_value() ? state->data_ptr<float>() : nullptr;
@@ -1182,7 +1251,7 @@ std::vector<torch::Tensor> linear_attention_bwd(
     if (need_decay) ddecay.zero_();
     return {dq, dk, dv, ddecay, ds0};
   }
-  const Split s = split_of(B * H, L, chunk_of(q.scalar_type()));
+  const Split s = split_of(B * H, L, std::max(Dk, Dv), chunk_of(q.scalar_type()));
   const bool split = s.G > 1;
   TORCH_CHECK(!split || (seg.dim() == 5 && seg.size(2) == s.G && seg.is_contiguous()),
               "linear attention: the forward pass's segment states are missing");
@@ -1206,7 +1275,9 @@ std::vector<torch::Tensor> linear_attention_bwd(
       a.seg_count = count.data_ptr<int>();
     }
     if (need_decay) {
-      part = torch::empty({B, H, s.G}, f32);
+      // one for each workgroup: at head size 128 there are two across the columns
+      const int64_t across = std::max(Dk, Dv) > 64 ? (Dk + 63) / 64 : 1;
+      part = torch::empty({B, H, s.G * across}, f32);
       a.decay_part = part.data_ptr<float>();
       if (split) {
         // S' is linear in what the segments add, so it needs these again;
@@ -1222,7 +1293,7 @@ std::vector<torch::Tensor> linear_attention_bwd(
         launch_pass<false, false, true>(dt, a, stream);
       }
       hipLaunchKernelGGL(la_decay_sum, dim3((unsigned)H), dim3(256), 0, stream,
-                         part.data_ptr<float>(), ddecay.data_ptr<float>(), (int)B, (int)H, s.G);
+                         part.data_ptr<float>(), ddecay.data_ptr<float>(), (int)B, (int)H, (int)(s.G * across));
       HIP_CHECK(hipGetLastError());
     } else {
       launch_pass<false, false, false>(dt, a, stream);
