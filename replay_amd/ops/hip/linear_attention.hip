@@ -23,6 +23,9 @@
 //   S' <- l^N (S' + N S) + sum_j (N-n_j) l^{N-n_j} k_j v_j^T
 // and rides on the dq pass as sum_i q_i . dq'_i.  (The shorter formula
 // sum_t t (q_t.dq_t - k_t.dk_t) cancels nearly everything on long histories.)
+// In a cut history each segment takes its start state as constant; what that
+// state's own derivative adds is <S'_start, V>, V = the segment's contribution
+// to dL/dS, which a scan sums up over the segments.
 //
 // Where batch x heads alone cannot fill the card, the history is cut into
 // segments: a state-only pass gives each segment's own contribution, a scan
@@ -54,9 +57,10 @@ struct PassArgs {
   float* state_out;                  // same or nullptr: the state after the last chunk
   const float* state_end_grad;       // same or nullptr: for <S'_end, dS_end>
   float* seg;                        // [B, H, G, Dk, Dv]: contributions, then start states
-  float* seg_d;                      // the same for S'
+  float* seg_d;                      // of each segment: S' at its end, for a constant start
   int* seg_count;                    // [B, H, G] valid positions
-  float* decay_part;                 // [B, H, G] partial sums of the decay's gradient
+  float* decay_part;                 // [B, H, parts] partial sums of the decay's gradient
+  int parts;
   int64_t st_c, st_e;                // strides of a state's (contraction, value) axes
   int B, H, L, Dc, De, G, seg_chunks;
   float c_pair, c_inter, c_update;   // where the scale goes
@@ -162,20 +166,15 @@ __global__ __launch_bounds__(DE * 4, DE < DP ? 1 : 2) void la_pass_f32(PassArgs 
 
   // whether the state after the last chunk is asked for
   const bool at_end = REV ? seg == 0 : seg == a.G - 1;
-  const bool want_end = STATE_ONLY || (at_end && (a.state_out || (DERIV && a.state_end_grad)));
+  const bool want_end = STATE_ONLY || (at_end && a.state_out) || (DERIV && (a.G > 1 || a.state_end_grad));
   // false while the state is known to be zero, as a history's first chunk has it
   bool started = FULL && (a.G > 1 || a.state_in);
   f32x4 S[NT], Sd[DERIV ? NT : 1];
   {
     const float* src = nullptr;
-    const float* src_d = nullptr;
     if (FULL) {
-      if (a.G > 1) {
-        src = a.seg + (bh * a.G + seg) * state_size;
-        if (DERIV) src_d = a.seg_d + (bh * a.G + seg) * state_size;
-      } else if (a.state_in) {
-        src = a.state_in + bh * state_size;
-      }
+      if (a.G > 1) src = a.seg + (bh * a.G + seg) * state_size;
+      else if (a.state_in) src = a.state_in + bh * state_size;
     }
 #pragma unroll
     for (int t = 0; t < NT; ++t) {
@@ -188,7 +187,7 @@ __global__ __launch_bounds__(DE * 4, DE < DP ? 1 : 2) void la_pass_f32(PassArgs 
         const int c = 16 * t + 4 * g_t + r;
         const bool in = c < a.Dc && e < a.De;
         S[t][r] = (src && in) ? src[c * a.st_c + e * a.st_e] : 0.f;
-        if (DERIV) Sd[t][r] = (src_d && in) ? src_d[c * a.st_c + e * a.st_e] : 0.f;
+        if (DERIV) Sd[t][r] = 0.f;
       }
     }
   }
@@ -379,12 +378,13 @@ __global__ __launch_bounds__(DE * 4, DE < DP ? 1 : 2) void la_pass_f32(PassArgs 
   float* dst_d = nullptr;
   if (STATE_ONLY) {
     dst = a.seg + (bh * a.G + seg) * state_size;
-    if (DERIV) dst_d = a.seg_d + (bh * a.G + seg) * state_size;
     if (threadIdx.x == 0 && blockIdx.y == 0) a.seg_count[bh * a.G + seg] = total;
   } else if (at_end && a.state_out) {
     dst = a.state_out + bh * state_size;
   }
-  const float* end_grad = (X && at_end && a.state_end_grad) ? a.state_end_grad + bh * state_size : nullptr;
+  // the derivative of the end state: for the scan, or here if it ends the history
+  if (X && a.G > 1) dst_d = a.seg_d + (bh * a.G + seg) * state_size;
+  const float* end_grad = (X && a.G == 1 && a.state_end_grad) ? a.state_end_grad + bh * state_size : nullptr;
 #pragma unroll
   for (int t = 0; t < NT; ++t) {
     int g_t = g;
@@ -407,7 +407,7 @@ __global__ __launch_bounds__(DE * 4, DE < DP ? 1 : 2) void la_pass_f32(PassArgs 
     if (threadIdx.x == 0) {
       float sum = 0.f;
       for (int w = 0; w < WAVES; ++w) sum += red[w];
-      a.decay_part[(bh * a.G + seg) * gridDim.y + blockIdx.y] = sum;
+      a.decay_part[bh * a.parts + seg * gridDim.y + blockIdx.y] = sum;
     }
   }
 }
@@ -605,18 +605,13 @@ __global__ __launch_bounds__(DE * 4, DE < DP ? 1 : DERIV || DP > 32 ? 2 : 3) voi
   bool started = FULL && (a.G > 1 || a.state_in);
   // whether the state after the last chunk is asked for
   const bool at_end = REV ? seg == 0 : seg == a.G - 1;
-  const bool want_end = STATE_ONLY || (at_end && (a.state_out || (DERIV && a.state_end_grad)));
+  const bool want_end = STATE_ONLY || (at_end && a.state_out) || (DERIV && (a.G > 1 || a.state_end_grad));
   f32x4 S[NT], Sd[DERIV ? NT : 1];
   {
     const float* src = nullptr;
-    const float* src_d = nullptr;
     if (FULL) {
-      if (a.G > 1) {
-        src = a.seg + (bh * a.G + seg) * state_size;
-        if (DERIV) src_d = a.seg_d + (bh * a.G + seg) * state_size;
-      } else if (a.state_in) {
-        src = a.state_in + bh * state_size;
-      }
+      if (a.G > 1) src = a.seg + (bh * a.G + seg) * state_size;
+      else if (a.state_in) src = a.state_in + bh * state_size;
     }
 #pragma unroll
     for (int t = 0; t < NT; ++t) {
@@ -629,7 +624,7 @@ __global__ __launch_bounds__(DE * 4, DE < DP ? 1 : DERIV || DP > 32 ? 2 : 3) voi
         const int c = state_row(t, g_t, r);
         const bool in = c < a.Dc && e < a.De;
         S[t][r] = (src && in) ? src[c * a.st_c + e * a.st_e] : 0.f;
-        if (DERIV) Sd[t][r] = (src_d && in) ? src_d[c * a.st_c + e * a.st_e] : 0.f;
+        if (DERIV) Sd[t][r] = 0.f;
       }
     }
   }
@@ -882,12 +877,13 @@ __global__ __launch_bounds__(DE * 4, DE < DP ? 1 : DERIV || DP > 32 ? 2 : 3) voi
   float* dst_d = nullptr;
   if (STATE_ONLY) {
     dst = a.seg + (bh * a.G + seg) * state_size;
-    if (DERIV) dst_d = a.seg_d + (bh * a.G + seg) * state_size;
     if (threadIdx.x == 0 && blockIdx.y == 0) a.seg_count[bh * a.G + seg] = total;
   } else if (at_end && a.state_out) {
     dst = a.state_out + bh * state_size;
   }
-  const float* end_grad = (X && at_end && a.state_end_grad) ? a.state_end_grad + bh * state_size : nullptr;
+  // the derivative of the end state: for the scan, or here if it ends the history
+  if (X && a.G > 1) dst_d = a.seg_d + (bh * a.G + seg) * state_size;
+  const float* end_grad = (X && a.G == 1 && a.state_end_grad) ? a.state_end_grad + bh * state_size : nullptr;
 #pragma unroll
   for (int t = 0; t < NT; ++t) {
     int g_t = g;
@@ -910,44 +906,64 @@ __global__ __launch_bounds__(DE * 4, DE < DP ? 1 : DERIV || DP > 32 ? 2 : 3) voi
     if (threadIdx.x == 0) {
       float sum = 0.f;
       for (int w = 0; w < WAVES; ++w) sum += red[w];
-      a.decay_part[(bh * a.G + seg) * gridDim.y + blockIdx.y] = sum;
+      a.decay_part[bh * a.parts + seg * gridDim.y + blockIdx.y] = sum;
     }
   }
 }
 
 // Contributions of the segments -> start states, in place, one thread for
 // each element of a state.
-template <bool REV, bool DERIV>
-__global__ void la_scan(float* seg, float* seg_d, const int* count, const float* state_in,
-                        const float* log_decay, int H, int G, int64_t state_size) {
+template <bool REV>
+__global__ void la_scan(float* seg, const int* count, const float* state_in, const float* log_decay,
+                        int H, int G, int64_t state_size) {
   const int64_t bh = blockIdx.x;
   const float ld = log_decay[bh % H];
   for (int64_t at = threadIdx.x + (int64_t)blockIdx.y * blockDim.x; at < state_size;
        at += (int64_t)gridDim.y * blockDim.x) {
-    float run = state_in ? state_in[bh * state_size + at] : 0.f, run_d = 0.f;
+    float run = state_in ? state_in[bh * state_size + at] : 0.f;
     for (int s = 0; s < G; ++s) {
       const int64_t i = bh * G + (REV ? G - 1 - s : s);
       const int N = count[i];
-      const float lN = N ? expf(ld * N) : 1.f;
       const float own = seg[i * state_size + at];
       seg[i * state_size + at] = run;
-      if (DERIV) {
-        const float own_d = seg_d[i * state_size + at];
-        seg_d[i * state_size + at] = run_d;
-        run_d = lN * (run_d + (float)N * run) + own_d;
-      }
-      run = lN * run + own;
+      run = (N ? expf(ld * N) : 1.f) * run + own;
     }
   }
 }
 
-// decay_part [B, H, G] -> [H]; a fixed order, in 64 bits (the parts may cancel).
-__global__ void la_decay_sum(const float* part, float* out, int B, int H, int G) {
+// What the start states' own derivatives add to the decay's gradient: the sum
+// over the segments of <S'_start, V>, and <S'_end, dL/dS_end>; a partial sum for
+// each workgroup of 256 elements.  seg_v: the contributions V.
+__global__ __launch_bounds__(256) void la_scan_decay(const float* seg_d, const float* seg_v,
+                                                     const int* count, const float* end_grad,
+                                                     const float* log_decay, float* part, int parts,
+                                                     int first_part, int H, int G, int64_t state_size) {
+  __shared__ float red[4];
+  const int64_t bh = blockIdx.x, at = threadIdx.x + (int64_t)blockIdx.y * 256;
+  const float ld = log_decay[bh % H];
+  float run = 0.f, sum = 0.f;
+  if (at < state_size) {
+    for (int s = 0; s < G; ++s) {
+      const int64_t i = bh * G + s;
+      const int N = count[i];
+      sum += run * seg_v[i * state_size + at];
+      run = (N ? expf(ld * N) : 1.f) * run + seg_d[i * state_size + at];
+    }
+    if (end_grad) sum += run * end_grad[bh * state_size + at];
+  }
+  sum = wave_reduce_sum(sum);
+  if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = sum;
+  __syncthreads();
+  if (threadIdx.x == 0) part[bh * parts + first_part + blockIdx.y] = (red[0] + red[1]) + (red[2] + red[3]);
+}
+
+// part [B, H, parts] -> [H]; a fixed order, in 64 bits (the parts may cancel).
+__global__ void la_decay_sum(const float* part, float* out, int B, int H, int parts) {
   __shared__ double red[4];
   const int h = blockIdx.x;
   double sum = 0.0;
-  for (int64_t i = threadIdx.x; i < (int64_t)B * G; i += blockDim.x)
-    sum += part[((i / G) * H + h) * G + i % G];
+  for (int64_t i = threadIdx.x; i < (int64_t)B * parts; i += blockDim.x)
+    sum += part[((i / parts) * H + h) * parts + i % parts];
 #pragma unroll
   for (int off = 32; off > 0; off >>= 1) sum += __shfl_xor(sum, off, WAVE);
   if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = sum;
@@ -1100,12 +1116,11 @@ void launch_pass(torch::ScalarType dt, const PassArgs& a, hipStream_t stream) {
   HIP_CHECK(hipGetLastError());
 }
 
-template <bool REV, bool DERIV>
+template <bool REV>
 void launch_scan(const PassArgs& a, const float* state_in, hipStream_t stream) {
   const int64_t size = (int64_t)a.Dc * a.De;
-  const unsigned y = (unsigned)((size + 255) / 256);
-  hipLaunchKernelGGL((la_scan<REV, DERIV>), dim3((unsigned)(a.B * a.H), y), dim3(256), 0, stream,
-                     a.seg, a.seg_d, a.seg_count, state_in, a.log_decay, a.H, a.G, size);
+  hipLaunchKernelGGL((la_scan<REV>), dim3((unsigned)(a.B * a.H), (unsigned)((size + 255) / 256)),
+                     dim3(256), 0, stream, a.seg, a.seg_count, state_in, a.log_decay, a.H, a.G, size);
   HIP_CHECK(hipGetLastError());
 }
 
@@ -1220,7 +1235,7 @@ std::vector<torch::Tensor> linear_attention_fwd(torch::Tensor q, torch::Tensor k
     a.seg = seg.data_ptr<float>();
     a.seg_count = count.data_ptr<int>();
     launch_pass<false, true, false>(q.scalar_type(), a, stream);
-    launch_scan<false, false>(a, a.state_in, stream);
+    launch_scan<false>(a, a.state_in, stream);
   }
   launch_pass<false, false, false>(q.scalar_type(), a, stream);
   return {out, end, seg};
@@ -1260,6 +1275,22 @@ std::vector<torch::Tensor> linear_attention_bwd(
   torch::Tensor count, part, seg_d, seg_r;
   if (split) count = torch::empty({B, H, s.G}, q.options().dtype(torch::kInt32));
 
+  // the reversed passes: dv with the state's gradient, and dk
+  PassArgs v_args = args_of(k, q, dout, log_decay, mask, false);
+  set_out(v_args, dv);
+  v_args.G = s.G;
+  v_args.seg_chunks = s.seg_chunks;
+  v_args.state_in = dstate_in;
+  v_args.state_out = need_state ? ds0.data_ptr<float>() : nullptr;
+  v_args.c_pair = v_args.c_update = (float)scale;
+  v_args.c_inter = 1.f;
+  if (split) {
+    seg_r = torch::empty_like(seg);
+    v_args.seg = seg_r.data_ptr<float>();
+    v_args.seg_count = count.data_ptr<int>();
+    launch_pass<true, true, false>(dt, v_args, stream);
+  }
+
   {  // dq, and the decay's gradient
     PassArgs a = args_of(dout, v, k, log_decay, mask, true);
     set_out(a, dq);
@@ -1270,62 +1301,45 @@ std::vector<torch::Tensor> linear_attention_bwd(
     a.c_pair = a.c_inter = (float)scale;
     a.c_update = 1.f;
     a.x = rows_of(q);
-    if (split) {
-      a.seg = seg.data_ptr<float>();
-      a.seg_count = count.data_ptr<int>();
-    }
+    if (split) a.seg = seg.data_ptr<float>();
     if (need_decay) {
-      // one for each workgroup: at head size 128 there are two across the columns
+      // partial sums: one for each workgroup of the pass (at head size 128 there
+      // are two across the columns), and of the scan over the segments
       const int64_t across = std::max(Dk, Dv) > 64 ? (Dk + 63) / 64 : 1;
-      part = torch::empty({B, H, s.G * across}, f32);
+      const int64_t blocks = split ? (Dk * Dv + 255) / 256 : 0;
+      a.parts = (int)(s.G * across + blocks);
+      part = torch::empty({B, H, a.parts}, f32);
       a.decay_part = part.data_ptr<float>();
       if (split) {
-        // S' is linear in what the segments add, so it needs these again;
-        // the start states come out as the forward pass left them
-        auto seg2 = torch::empty_like(seg);
         seg_d = torch::empty_like(seg);
-        a.seg = seg2.data_ptr<float>();
         a.seg_d = seg_d.data_ptr<float>();
-        launch_pass<false, true, true>(dt, a, stream);
-        launch_scan<false, true>(a, state_in, stream);
-        launch_pass<false, false, true>(dt, a, stream);
-      } else {
-        launch_pass<false, false, true>(dt, a, stream);
+      }
+      launch_pass<false, false, true>(dt, a, stream);
+      if (split) {
+        hipLaunchKernelGGL(la_scan_decay, dim3((unsigned)(B * H), (unsigned)blocks), dim3(256), 0, stream,
+                           a.seg_d, v_args.seg, v_args.seg_count, dstate_in, a.log_decay, a.decay_part,
+                           a.parts, (int)(s.G * across), (int)H, s.G, Dk * Dv);
+        HIP_CHECK(hipGetLastError());
       }
       hipLaunchKernelGGL(la_decay_sum, dim3((unsigned)H), dim3(256), 0, stream,
-                         part.data_ptr<float>(), ddecay.data_ptr<float>(), (int)B, (int)H, (int)(s.G * across));
+                         part.data_ptr<float>(), ddecay.data_ptr<float>(), (int)B, (int)H, a.parts);
       HIP_CHECK(hipGetLastError());
     } else {
       launch_pass<false, false, false>(dt, a, stream);
     }
   }
-  {  // dv, with the state's gradient, then dk
-    PassArgs a = args_of(k, q, dout, log_decay, mask, false);
-    set_out(a, dv);
-    a.G = s.G;
-    a.seg_chunks = s.seg_chunks;
-    a.state_in = dstate_in;
-    a.state_out = need_state ? ds0.data_ptr<float>() : nullptr;
-    a.c_pair = a.c_update = (float)scale;
-    a.c_inter = 1.f;
-    if (split) {
-      seg_r = torch::empty_like(seg);
-      a.seg = seg_r.data_ptr<float>();
-      a.seg_count = count.data_ptr<int>();
-      launch_pass<true, true, false>(dt, a, stream);
-      launch_scan<true, false>(a, dstate_in, stream);
-    }
-    launch_pass<true, false, false>(dt, a, stream);
-    PassArgs c = args_of(v, dout, q, log_decay, mask, true);
-    set_out(c, dk);
-    c.G = s.G;
-    c.seg_chunks = s.seg_chunks;
-    c.state_in = dstate_in;
-    c.seg = a.seg;
-    c.c_pair = c.c_update = (float)scale;
-    c.c_inter = 1.f;
-    launch_pass<true, false, false>(dt, c, stream);
-  }
+
+  if (split) launch_scan<true>(v_args, dstate_in, stream);
+  launch_pass<true, false, false>(dt, v_args, stream);
+  PassArgs c = args_of(v, dout, q, log_decay, mask, true);
+  set_out(c, dk);
+  c.G = s.G;
+  c.seg_chunks = s.seg_chunks;
+  c.state_in = dstate_in;
+  c.seg = v_args.seg;
+  c.c_pair = c.c_update = (float)scale;
+  c.c_inter = 1.f;
+  launch_pass<true, false, false>(dt, c, stream);
   return {dq, dk, dv, ddecay, ds0};
 }
 
