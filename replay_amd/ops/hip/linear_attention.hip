@@ -84,20 +84,19 @@ __device__ __forceinline__ uint4 load_piece(const T* p, int n) {
 }
 
 // One operand's 32 positions on their way from memory to LDS, where they are
-// float: 16-byte pieces, W / V of THREADS threads a row.
-template <typename T, int W, int THREADS>
+// float: 16-byte pieces, DP / V of 4 DP threads a row.
+template <typename T, int DP>
 struct Rows32 {
-  static constexpr int V = 16 / sizeof(T), ACROSS = W / V, DOWN = THREADS / ACROSS, PIECES = 32 / DOWN;
-  static constexpr int LD = W + 4;  // rows then start 4 banks apart
+  static constexpr int V = 16 / sizeof(T), ACROSS = DP / V, DOWN = DP * 4 / ACROSS, PIECES = 32 / DOWN;
+  static constexpr int LD = DP + 4;  // rows then start 4 banks apart
 
   const T* at;
   int64_t l;
   int left;
   uint4 r[PIECES];
 
-  // columns from column d0 on, of D
-  __device__ __forceinline__ Rows32(const Rows& src, int b, int h, int d0, int D) {
-    const int d = d0 + (threadIdx.x % ACROSS) * V;
+  __device__ __forceinline__ Rows32(const Rows& src, int b, int h, int D) {
+    const int d = (threadIdx.x % ACROSS) * V;
     l = src.l;
     left = D - d;
     at = reinterpret_cast<const T*>(src.p) + b * src.b + h * src.h + (threadIdx.x / ACROSS) * l + d;
@@ -131,18 +130,17 @@ struct Rows32 {
 // accumulator layout (column = lane & 15, row = 4 (lane >> 4) + r), which is
 // also the layout of an operand whose contraction index is visited in that
 // order: neither the state nor the pair weights leave the registers between
-// products.  DE value columns a workgroup, chosen as in la_pass_bf16: no spills.
-template <typename T, int DP, int DE, bool REV, bool STATE_ONLY, bool DERIV>
-__global__ __launch_bounds__(DE * 4, DE < DP ? 1 : 2) void la_pass_f32(PassArgs a) {
-  using Ch = Rows32<T, DP, DE * 4>;  // q and k
-  using Cv = Rows32<T, DE, DE * 4>;  // v, x and the outputs
-  constexpr int C = 16, ROWS = 32, LD = Ch::LD, LDV = Cv::LD, NT = DP / 16, WAVES = DE / 16;
+// products.  (Launch bounds as in la_pass_bf16: none that need spills.)
+template <typename T, int DP, bool REV, bool STATE_ONLY, bool DERIV>
+__global__ __launch_bounds__(DP * 4, 2) void la_pass_f32(PassArgs a) {
+  using Ch = Rows32<T, DP>;
+  constexpr int C = 16, ROWS = 32, LD = Ch::LD, NT = DP / 16, WAVES = DP / 16;
   constexpr bool FULL = !STATE_ONLY, X = DERIV && FULL;
   __shared__ __attribute__((aligned(16))) float q_s[FULL ? ROWS * LD : 4];
   __shared__ __attribute__((aligned(16))) float k_s[ROWS * LD];
-  __shared__ __attribute__((aligned(16))) float v_s[ROWS * LDV];
-  __shared__ __attribute__((aligned(16))) float o_s[FULL ? ROWS * LDV : 4];
-  __shared__ __attribute__((aligned(16))) float x_s[X ? ROWS * LDV : 4];
+  __shared__ __attribute__((aligned(16))) float v_s[ROWS * LD];
+  __shared__ __attribute__((aligned(16))) float o_s[FULL ? ROWS * LD : 4];
+  __shared__ __attribute__((aligned(16))) float x_s[X ? ROWS * LD : 4];
   // of each position, within its chunk: the valid ones up to it, and its
   // weights in the product with the start state and in the state's update
   __shared__ __attribute__((aligned(16))) float n_s[ROWS], inter_s[ROWS], update_s[ROWS];
@@ -151,14 +149,13 @@ __global__ __launch_bounds__(DE * 4, DE < DP ? 1 : 2) void la_pass_f32(PassArgs 
 
   const int seg = blockIdx.x % a.G;
   const int64_t bh = blockIdx.x / a.G;
-  const int first_e = blockIdx.y * DE;  // this workgroup's value columns
   const int b = bh / a.H, h = bh % a.H;
   // the wave's index is the same for its lanes, which the compiler cannot see:
   // what depends on it alone then needs no vector registers and no masks
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int lo = lane & 15, g = lane >> 4;
-  const int e0 = wave * 16, e = first_e + e0 + lo;
-  const bool busy = first_e + e0 < a.De;
+  const int e0 = wave * 16, e = e0 + lo;
+  const bool busy = e0 < a.De;
   const int64_t state_size = (int64_t)a.Dc * a.De;
   const float ld = a.log_decay[h];
   // a decay of zero (log -inf) keeps l^0 = 1
@@ -208,8 +205,7 @@ __global__ __launch_bounds__(DE * 4, DE < DP ? 1 : 2) void la_pass_f32(PassArgs 
   auto start_of = [&](int step) { return (REV ? first + last - 1 - step : step) * ROWS; };
   int total = 0;
   float d_decay = 0.f;
-  Ch q_r(a.q, b, h, 0, a.Dc), k_r(a.k, b, h, 0, a.Dc);
-  Cv v_r(a.v, b, h, first_e, a.De), x_r(a.x, b, h, first_e, a.De);
+  Ch q_r(a.q, b, h, a.Dc), k_r(a.k, b, h, a.Dc), v_r(a.v, b, h, a.De), x_r(a.x, b, h, a.De);
   // The mask is read a load ahead of the rows that it says to read.
   const bool* mask = a.mask ? a.mask + b * a.mask_b : nullptr;
   auto look = [&](int step) {
@@ -225,29 +221,29 @@ __global__ __launch_bounds__(DE * 4, DE < DP ? 1 : 2) void la_pass_f32(PassArgs 
   };
   T* out = nullptr;
   if (FULL)
-    out = reinterpret_cast<T*>(a.out) + b * a.out_b + h * a.out_h + first_e +
-          (threadIdx.x / Cv::ACROSS) * a.out_l + (threadIdx.x % Cv::ACROSS) * Cv::V;
+    out = reinterpret_cast<T*>(a.out) + b * a.out_b + h * a.out_h +
+          (threadIdx.x / Ch::ACROSS) * a.out_l + (threadIdx.x % Ch::ACROSS) * Ch::V;
   // outputs of the rows at l0 in whole rows, from LDS or zeros
   auto store = [&](int l0, bool zero) {
-    const int row = threadIdx.x / Cv::ACROSS, left = v_r.left;
-    const float* from = o_s + row * LDV + (threadIdx.x % Cv::ACROSS) * Cv::V;
+    const int row = threadIdx.x / Ch::ACROSS, left = v_r.left;
+    const float* from = o_s + row * LD + (threadIdx.x % Ch::ACROSS) * Ch::V;
 #pragma unroll
-    for (int i = 0; i < Cv::PIECES; ++i) {
-      if (l0 + row + Cv::DOWN * i >= a.L || left <= 0) continue;
-      alignas(16) T t[Cv::V];
+    for (int i = 0; i < Ch::PIECES; ++i) {
+      if (l0 + row + Ch::DOWN * i >= a.L || left <= 0) continue;
+      alignas(16) T t[Ch::V];
 #pragma unroll
-      for (int j = 0; j < Cv::V; j += 4) {
+      for (int j = 0; j < Ch::V; j += 4) {
         f32x4 v = {0.f, 0.f, 0.f, 0.f};
-        if (!zero) v = *reinterpret_cast<const f32x4*>(from + i * Cv::DOWN * LDV + j);
+        if (!zero) v = *reinterpret_cast<const f32x4*>(from + i * Ch::DOWN * LD + j);
 #pragma unroll
         for (int r = 0; r < 4; ++r) t[j + r] = from_f32<T>(v[r]);
       }
-      T* p = out + (l0 + Cv::DOWN * i) * a.out_l;
-      if (left >= Cv::V) {
+      T* p = out + (l0 + Ch::DOWN * i) * a.out_l;
+      if (left >= Ch::V) {
         __builtin_memcpy(p, t, 16);
       } else {
 #pragma unroll
-        for (int j = 0; j < Cv::V; ++j)
+        for (int j = 0; j < Ch::V; ++j)
           if (j < left) p[j] = t[j];
       }
     }
@@ -261,13 +257,10 @@ __global__ __launch_bounds__(DE * 4, DE < DP ? 1 : 2) void la_pass_f32(PassArgs 
     const int l0 = start_of(step);
     const unsigned now = bits;
     total += __popc(now);
-    if (now == 0) {  // nothing is seen, added or forgotten
-      if (FULL) store(l0, true);
-      bits = (unsigned)__ballot(ahead);
-      fetch(step + 1, bits);
-      ahead = look(step + 2);
-      continue;
-    }
+    // without valid positions nothing is seen, added or forgotten.  (One way
+    // round the loop for both cases: a second one, with a continue, kept copies
+    // of the state.)
+    if (now) {
     if (FULL) q_r.put(q_s);
     k_r.put(k_s);
     v_r.put(v_s);
@@ -280,24 +273,22 @@ __global__ __launch_bounds__(DE * 4, DE < DP ? 1 : 2) void la_pass_f32(PassArgs 
       update_s[lane] = a.c_update * lam[REV ? n : N - n];
     }
     __syncthreads();
+    }
     bits = (unsigned)__ballot(ahead);
     fetch(step + 1, bits);
     ahead = look(step + 2);
 
-    if (busy) {
+    if (busy && now) {
 #pragma unroll 1
       for (int half = 0; half < 2; ++half) {
         const int r0 = (REV ? 1 - half : half) * C;
         const unsigned own = (now >> r0) & 0xffffu;
         const int N = __popc(own);
-        if (N == 0) {
-          if (FULL) *reinterpret_cast<f32x4*>(o_s + (r0 + lo) * LDV + e0 + 4 * g) = f32x4{0.f, 0.f, 0.f, 0.f};
-          continue;
-        }
+        // (an empty half: its products are of zeros, and decay by l^0)
         const float* k_c = k_s + r0 * LD;
         float vr[4];
 #pragma unroll
-        for (int r = 0; r < 4; ++r) vr[r] = v_s[(r0 + 4 * g + r) * LDV + e0 + lo];
+        for (int r = 0; r < 4; ++r) vr[r] = v_s[(r0 + 4 * g + r) * LD + e0 + lo];
         const f32x4 n_j = *reinterpret_cast<const f32x4*>(n_s + r0 + 4 * g);
         if (FULL) {
           const float* q_c = q_s + (r0 + lo) * LD;
@@ -321,7 +312,7 @@ __global__ __launch_bounds__(DE * 4, DE < DP ? 1 : 2) void la_pass_f32(PassArgs 
           if (DERIV) od = w_i * (od + n_i * o);
           o = w_i * o;
           // valid positions in one run: n_i - n_j = i - j wherever a pair counts
-          const unsigned run = own >> __builtin_ctz(own);
+          const unsigned run = own >> __builtin_ctz(own | 0x10000u);
           const bool whole = (run & (run + 1)) == 0;
           const f32x4 gaps = REV ? n_j - n_i : n_i - n_j;
           f32x4 p = pt * full;
@@ -338,23 +329,21 @@ __global__ __launch_bounds__(DE * 4, DE < DP ? 1 : 2) void la_pass_f32(PassArgs 
             if (DERIV) od = mfma4(vr[r], p[r] * gaps[r], od);
           }
           if (DERIV) {
-            const f32x4 xv = *reinterpret_cast<const f32x4*>(x_s + (r0 + lo) * LDV + e0 + 4 * g);
+            const f32x4 xv = *reinterpret_cast<const f32x4*>(x_s + (r0 + lo) * LD + e0 + 4 * g);
 #pragma unroll
             for (int r = 0; r < 4; ++r) d_decay += xv[r] * od[r];
           }
-          *reinterpret_cast<f32x4*>(o_s + (r0 + lo) * LDV + e0 + 4 * g) = o;
+          *reinterpret_cast<f32x4*>(o_s + (r0 + lo) * LD + e0 + 4 * g) = o;
         }
         const bool update = want_end || step + 1 < last || half == 0;
-        if (started && update) {
-          const float lN = lam[N];
-#pragma unroll
-          for (int t = 0; t < NT; ++t) {
-            if (DERIV) Sd[t] = lN * (Sd[t] + (float)N * S[t]);
-            S[t] = lN * S[t];
-          }
-        }
         started = true;
-        if (!update) continue;
+        if (update) {
+        const float lN = lam[N];
+#pragma unroll
+        for (int t = 0; t < NT; ++t) {
+          if (DERIV) Sd[t] = lN * (Sd[t] + (float)N * S[t]);
+          S[t] = lN * S[t];
+        }
         const f32x4 w = *reinterpret_cast<const f32x4*>(update_s + r0 + 4 * g);
         const f32x4 left = REV ? n_j : (float)N - n_j;
 #pragma unroll
@@ -368,17 +357,18 @@ __global__ __launch_bounds__(DE * 4, DE < DP ? 1 : 2) void la_pass_f32(PassArgs 
             if (DERIV) Sd[t] = mfma4(kv, weighted * left[r], Sd[t]);
           }
         }
+        }
       }
     }
-    __syncthreads();  // the rows are read and their outputs are in LDS
-    if (FULL) store(l0, false);
+    if (now) __syncthreads();  // the rows are read and their outputs are in LDS
+    if (FULL) store(l0, now == 0);
   }
 
   float* dst = nullptr;
   float* dst_d = nullptr;
   if (STATE_ONLY) {
     dst = a.seg + (bh * a.G + seg) * state_size;
-    if (threadIdx.x == 0 && blockIdx.y == 0) a.seg_count[bh * a.G + seg] = total;
+    if (threadIdx.x == 0) a.seg_count[bh * a.G + seg] = total;
   } else if (at_end && a.state_out) {
     dst = a.state_out + bh * state_size;
   }
@@ -407,7 +397,7 @@ __global__ __launch_bounds__(DE * 4, DE < DP ? 1 : 2) void la_pass_f32(PassArgs 
     if (threadIdx.x == 0) {
       float sum = 0.f;
       for (int w = 0; w < WAVES; ++w) sum += red[w];
-      a.decay_part[bh * a.parts + seg * gridDim.y + blockIdx.y] = sum;
+      a.decay_part[bh * a.parts + seg] = sum;
     }
   }
 }
@@ -506,22 +496,21 @@ __device__ __forceinline__ void store8(__hip_bfloat16* p, int n, uint4 v) {
 }
 
 // One operand's 64 positions on their way from memory to LDS: 16-byte pieces,
-// W / 8 of THREADS threads a row.
-template <int W, int THREADS, bool EDGE>
+// DP / 8 of 4 DP threads a row.
+template <int DP, bool EDGE>
 struct Chunk {
-  static constexpr int C = 64, ACROSS = W / 8, DOWN = THREADS / ACROSS, PIECES = C / DOWN;
+  static constexpr int C = 64, ACROSS = DP / 8, DOWN = DP * 4 / ACROSS, PIECES = C / DOWN;
   // rows 16 bytes apart from a power of two: the fragment reads of 16 rows
   // then start in banks 4 words apart
-  static constexpr int LD = W * 2 + 16, BYTES = C * LD;
+  static constexpr int LD = DP * 2 + 16, BYTES = C * LD;
 
   const __hip_bfloat16* at;  // this thread's first piece of position 0
   int64_t l;
   int left;                  // columns from d on that exist
   uint4 r[PIECES];
 
-  // columns from column d0 on, of D
-  __device__ __forceinline__ Chunk(const Rows& src, int b, int h, int d0, int D) {
-    const int d = d0 + (threadIdx.x % ACROSS) * 8;
+  __device__ __forceinline__ Chunk(const Rows& src, int b, int h, int D) {
+    const int d = (threadIdx.x % ACROSS) * 8;
     l = src.l;
     left = D - d;
     at = reinterpret_cast<const __hip_bfloat16*>(src.p) + b * src.b + h * src.h +
@@ -563,23 +552,20 @@ __device__ __forceinline__ int state_row(int t, int g, int r) {
   return 32 * (t >> 1) + 8 * g + 4 * (t & 1) + r;
 }
 
-// DE value columns a workgroup, DE / 16 waves of 16.  The launch bounds are the
-// tightest that need no spills: with spills, first chunks came out wrong now and
-// then.  The decay's gradient at head size 128 does not fit 256 registers a
-// lane; there a workgroup takes half the value columns, in 4 waves of up to 512.
-template <int DP, int DE, bool REV, bool STATE_ONLY, bool DERIV, bool EDGE>
-__global__ __launch_bounds__(DE * 4, DE < DP ? 1 : DERIV || DP > 32 ? 2 : 3) void la_pass_bf16(PassArgs a) {
-  using Ch = Chunk<DP, DE * 4, EDGE>;  // q and k
-  using Cv = Chunk<DE, DE * 4, EDGE>;  // v, x and the outputs
-  constexpr int C = 64, NS = DP / 32, NT = DP / 16, LDV = Cv::LD;
-  constexpr int WAVES = DE / 16;
+// DP / 16 waves, each with 16 value columns and the whole contraction axis.  The
+// launch bounds are the tightest that need no spills: with spills, first chunks
+// came out wrong now and then.
+template <int DP, bool REV, bool STATE_ONLY, bool DERIV, bool EDGE>
+__global__ __launch_bounds__(DP * 4, DERIV ? 2 : 3) void la_pass_bf16(PassArgs a) {
+  using Ch = Chunk<DP, EDGE>;
+  constexpr int C = 64, NS = DP / 32, NT = DP / 16, LD = Ch::LD, WAVES = DP / 16;
   constexpr bool FULL = !STATE_ONLY, X = DERIV && FULL;
   __shared__ __attribute__((aligned(16))) char q_s[FULL ? Ch::BYTES : 16];
   __shared__ __attribute__((aligned(16))) char k_s[Ch::BYTES];
-  __shared__ __attribute__((aligned(16))) char v_s[Cv::BYTES];
+  __shared__ __attribute__((aligned(16))) char v_s[Ch::BYTES];
   __shared__ uint4 p_s[FULL ? 6 : 1][64];    // pair weights, as operands
   __shared__ f32x4 full_s[FULL ? 4 : 1][64]; // those of a chunk without gaps, by tile distance
-  __shared__ __attribute__((aligned(16))) char x_s[X ? Cv::BYTES : 16];
+  __shared__ __attribute__((aligned(16))) char x_s[X ? Ch::BYTES : 16];
   // of each position: the valid ones up to it, and its weights in the product
   // with the start state and in the state's update
   __shared__ __attribute__((aligned(16))) float n_s[C], inter_s[C], update_s[C];
@@ -588,18 +574,17 @@ __global__ __launch_bounds__(DE * 4, DE < DP ? 1 : DERIV || DP > 32 ? 2 : 3) voi
 
   const int seg = blockIdx.x % a.G;
   const int64_t bh = blockIdx.x / a.G;
-  const int first_e = blockIdx.y * DE;  // this workgroup's value columns
   const int b = bh / a.H, h = bh % a.H;
   // the wave's index is the same for its lanes, which the compiler cannot see:
   // what depends on it alone then needs no vector registers and no masks
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int lo = lane & 15, g = lane >> 4;
-  const int e0 = wave * 16, e = first_e + e0 + lo;
-  const bool busy = first_e + e0 < a.De;
+  const int e0 = wave * 16, e = e0 + lo;
+  const bool busy = e0 < a.De;
   const int64_t state_size = (int64_t)a.Dc * a.De;
   const float ld = a.log_decay[h];
   // a decay of zero (log -inf) keeps l^0 = 1
-  for (int i = threadIdx.x; i <= C; i += DE * 4) lam[i] = i ? expf(ld * i) : 1.f;
+  for (int i = threadIdx.x; i <= C; i += DP * 4) lam[i] = i ? expf(ld * i) : 1.f;
 
   // false while the state is known to be zero, as a history's first chunk has it
   bool started = FULL && (a.G > 1 || a.state_in);
@@ -649,8 +634,7 @@ __global__ __launch_bounds__(DE * 4, DE < DP ? 1 : DERIV || DP > 32 ? 2 : 3) voi
   auto start_of = [&](int step) { return (REV ? first + last - 1 - step : step) * C; };
   int total = 0;
   float d_decay = 0.f;
-  Ch q_r(a.q, b, h, 0, a.Dc), k_r(a.k, b, h, 0, a.Dc);
-  Cv v_r(a.v, b, h, first_e, a.De), x_r(a.x, b, h, first_e, a.De);
+  Ch q_r(a.q, b, h, a.Dc), k_r(a.k, b, h, a.Dc), v_r(a.v, b, h, a.De), x_r(a.x, b, h, a.De);
   // The mask is read a chunk ahead of the rows that it says to read.
   const bool* mask = a.mask ? a.mask + b * a.mask_b : nullptr;
   auto look = [&](int step) {
@@ -666,19 +650,19 @@ __global__ __launch_bounds__(DE * 4, DE < DP ? 1 : DERIV || DP > 32 ? 2 : 3) voi
   };
   __hip_bfloat16* out = nullptr;
   if (FULL)
-    out = reinterpret_cast<__hip_bfloat16*>(a.out) + b * a.out_b + h * a.out_h + first_e +
-          (threadIdx.x / Cv::ACROSS) * a.out_l + (threadIdx.x % Cv::ACROSS) * 8;
+    out = reinterpret_cast<__hip_bfloat16*>(a.out) + b * a.out_b + h * a.out_h +
+          (threadIdx.x / Ch::ACROSS) * a.out_l + (threadIdx.x % Ch::ACROSS) * 8;
   // outputs of the chunk at l0 in whole rows, from LDS (where they take v's
   // place: a thread reads what it alone will overwrite) or zeros
   auto store = [&](int l0, bool zero) {
-    const int row = threadIdx.x / Cv::ACROSS, left = v_r.left;
-    const char* from = v_s + row * LDV + (threadIdx.x % Cv::ACROSS) * 16;
+    const int row = threadIdx.x / Ch::ACROSS, left = v_r.left;
+    const char* from = v_s + row * LD + (threadIdx.x % Ch::ACROSS) * 16;
 #pragma unroll
-    for (int i = 0; i < Cv::PIECES; ++i) {
-      if (l0 + row + Cv::DOWN * i >= a.L || left <= 0) continue;
+    for (int i = 0; i < Ch::PIECES; ++i) {
+      if (l0 + row + Ch::DOWN * i >= a.L || left <= 0) continue;
       uint4 v = {0, 0, 0, 0};
-      if (!zero) v = *reinterpret_cast<const uint4*>(from + i * Cv::DOWN * LDV);
-      store8<EDGE>(out + (l0 + Cv::DOWN * i) * a.out_l, left, v);
+      if (!zero) v = *reinterpret_cast<const uint4*>(from + i * Ch::DOWN * LD);
+      store8<EDGE>(out + (l0 + Ch::DOWN * i) * a.out_l, left, v);
     }
   };
 
@@ -691,13 +675,10 @@ __global__ __launch_bounds__(DE * 4, DE < DP ? 1 : DERIV || DP > 32 ? 2 : 3) voi
     const uint64_t now = bits;
     const int N = __popcll(now);
     total += N;
-    if (N == 0) {  // nothing is seen, added or forgotten
-      if (FULL) store(l0, true);
-      bits = __ballot(ahead);
-      fetch(step + 1, bits);
-      ahead = look(step + 2);
-      continue;
-    }
+    // without valid positions nothing is seen, added or forgotten.  (One way
+    // round the loop for both cases: a second one, with a continue, kept copies
+    // of the state, 50 registers of it at head size 64.)
+    if (N) {
     if (FULL) q_r.put(q_s);
     k_r.put(k_s);
     v_r.put(v_s);
@@ -709,10 +690,12 @@ __global__ __launch_bounds__(DE * 4, DE < DP ? 1 : DERIV || DP > 32 ? 2 : 3) voi
       update_s[lane] = a.c_update * lam[REV ? n : N - n];
     }
     __syncthreads();
+    }
     bits = __ballot(ahead);
     fetch(step + 1, bits);
     ahead = look(step + 2);
 
+    if (N) {
     const float all = (float)N;
     if (FULL) {
       // valid positions in one run: n_i - n_j = i - j wherever a pair counts
@@ -755,8 +738,8 @@ __global__ __launch_bounds__(DE * 4, DE < DP ? 1 : DERIV || DP > 32 ? 2 : 3) voi
             asm volatile("" ::: "memory");
             f32x4 other = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-            for (int c = 0; c < DE / 32; ++c)
-              other = mfma32(Cv::rows(v_s, 16 * jt, c, lo, g), Cv::rows(x_s, 16 * it, c, lo, g), other);
+            for (int c = 0; c < NS; ++c)
+              other = mfma32(Ch::rows(v_s, 16 * jt, c, lo, g), Ch::rows(x_s, 16 * it, c, lo, g), other);
 #pragma unroll
             for (int r = 0; r < 4; ++r) d_decay += p[u][r] * gaps[r] * other[r];
           }
@@ -769,7 +752,7 @@ __global__ __launch_bounds__(DE * 4, DE < DP ? 1 : DERIV || DP > 32 ? 2 : 3) voi
     f32x4 o[FULL ? 4 : 1];
     if (busy) {
 #pragma unroll
-      for (int s = 0; s < 2; ++s) vf[s] = Cv::columns(v_s, e0, 4, s, lo, g);
+      for (int s = 0; s < 2; ++s) vf[s] = Ch::columns(v_s, e0, 4, s, lo, g);
 
       if (FULL) {
         // the start state's part, a block of the contraction at a time: so the
@@ -780,7 +763,7 @@ __global__ __launch_bounds__(DE * 4, DE < DP ? 1 : DERIV || DP > 32 ? 2 : 3) voi
           // what of the decay's gradient goes by x . (S' q) w, a block at a time too
           auto weighted_x = [&](int it) {
             return inter_s[16 * it + lo] *
-                   widen(*reinterpret_cast<const bf16x4*>(x_s + (16 * it + lo) * LDV + (e0 + 4 * g) * 2));
+                   widen(*reinterpret_cast<const bf16x4*>(x_s + (16 * it + lo) * LD + (e0 + 4 * g) * 2));
           };
 #pragma unroll
           for (int s = 0; s < NS; ++s) {
@@ -825,23 +808,22 @@ __global__ __launch_bounds__(DE * 4, DE < DP ? 1 : DERIV || DP > 32 ? 2 : 3) voi
         }
 #pragma unroll
         for (int it = 0; it < 4; ++it)
-          *reinterpret_cast<bf16x4*>(v_s + (16 * it + lo) * LDV + (e0 + 4 * g) * 2) =
+          *reinterpret_cast<bf16x4*>(v_s + (16 * it + lo) * LD + (e0 + 4 * g) * 2) =
               __builtin_convertvector(o[it], bf16x4);
       }
     }
     if (busy) {
       const bool update = want_end || step + 1 < last;
-      if (started && update) {
-        const float lN = lam[N];
-#pragma unroll
-        for (int t = 0; t < NT; ++t) {
-          if (DERIV) Sd[t] = lN * (Sd[t] + all * S[t]);
-          S[t] = lN * S[t];
-        }
-      }
       started = true;
+      if (update) {
+      const float lN = lam[N];
 #pragma unroll
-      for (int s = 0; s < 2 && update; ++s) {
+      for (int t = 0; t < NT; ++t) {
+        if (DERIV) Sd[t] = lN * (Sd[t] + all * S[t]);
+        S[t] = lN * S[t];
+      }
+#pragma unroll
+      for (int s = 0; s < 2; ++s) {
         asm volatile("" ::: "memory");
         f32x4 w[2];
         const uint4 raw = __builtin_bit_cast(uint4, vf[s]);
@@ -868,16 +850,18 @@ __global__ __launch_bounds__(DE * 4, DE < DP ? 1 : DERIV || DP > 32 ? 2 : 3) voi
           add(Sd);
         }
       }
+      }
     }
     __syncthreads();  // the chunk is read and its outputs are in LDS
-    if (FULL) store(l0, false);
+    }
+    if (FULL) store(l0, N == 0);
   }
 
   float* dst = nullptr;
   float* dst_d = nullptr;
   if (STATE_ONLY) {
     dst = a.seg + (bh * a.G + seg) * state_size;
-    if (threadIdx.x == 0 && blockIdx.y == 0) a.seg_count[bh * a.G + seg] = total;
+    if (threadIdx.x == 0) a.seg_count[bh * a.G + seg] = total;
   } else if (at_end && a.state_out) {
     dst = a.state_out + bh * state_size;
   }
@@ -906,7 +890,7 @@ __global__ __launch_bounds__(DE * 4, DE < DP ? 1 : DERIV || DP > 32 ? 2 : 3) voi
     if (threadIdx.x == 0) {
       float sum = 0.f;
       for (int w = 0; w < WAVES; ++w) sum += red[w];
-      a.decay_part[bh * a.parts + seg * gridDim.y + blockIdx.y] = sum;
+      a.decay_part[bh * a.parts + seg] = sum;
     }
   }
 }
@@ -1096,21 +1080,18 @@ void launch_pass(torch::ScalarType dt, const PassArgs& a, hipStream_t stream) {
   TORCH_CHECK(blocks < (int64_t(1) << 31), "linear attention: too many (batch, head, segment)s");
   const int dp = padded(std::max(a.Dc, a.De));
   const bool edge = a.Dc % 8 || a.De % 8;
-#define LA_LAUNCH(DE, ...)                                                                         \
-  hipLaunchKernelGGL((__VA_ARGS__), dim3((unsigned)blocks, (unsigned)((a.De + DE - 1) / DE)),      \
-                     dim3(DE * 4), 0, stream, a)
-#define LA_PASS(DP, DE)                                                                            \
-  do {                                                                                             \
-    if (dt == torch::kBFloat16 && edge)                                                            \
-      LA_LAUNCH(DE, la_pass_bf16<DP, DE, REV, STATE_ONLY, DERIV, true>);                           \
-    else if (dt == torch::kBFloat16) LA_LAUNCH(DE, la_pass_bf16<DP, DE, REV, STATE_ONLY, DERIV, false>); \
-    else if (dt == torch::kHalf) LA_LAUNCH(DE, la_pass_f32<__half, DP, DE, REV, STATE_ONLY, DERIV>); \
-    else LA_LAUNCH(DE, la_pass_f32<float, DP, DE, REV, STATE_ONLY, DERIV>);                        \
+#define LA_LAUNCH(DP, ...)                                                                     \
+  hipLaunchKernelGGL((__VA_ARGS__), dim3((unsigned)blocks), dim3(DP * 4), 0, stream, a)
+#define LA_PASS(DP)                                                                            \
+  do {                                                                                         \
+    if (dt == torch::kBFloat16 && edge) LA_LAUNCH(DP, la_pass_bf16<DP, REV, STATE_ONLY, DERIV, true>); \
+    else if (dt == torch::kBFloat16) LA_LAUNCH(DP, la_pass_bf16<DP, REV, STATE_ONLY, DERIV, false>);   \
+    else if (dt == torch::kHalf) LA_LAUNCH(DP, la_pass_f32<__half, DP, REV, STATE_ONLY, DERIV>);       \
+    else LA_LAUNCH(DP, la_pass_f32<float, DP, REV, STATE_ONLY, DERIV>);                        \
   } while (0)
-  if (dp == 32) LA_PASS(32, 32);
-  else if (dp == 64) LA_PASS(64, 64);
-  else if constexpr (DERIV && !STATE_ONLY) LA_PASS(128, 64);
-  else LA_PASS(128, 128);
+  if (dp == 32) LA_PASS(32);
+  else if (dp == 64) LA_PASS(64);
+  else LA_PASS(128);
 #undef LA_PASS
 #undef LA_LAUNCH
   HIP_CHECK(hipGetLastError());
@@ -1303,11 +1284,9 @@ std::vector<torch::Tensor> linear_attention_bwd(
     a.x = rows_of(q);
     if (split) a.seg = seg.data_ptr<float>();
     if (need_decay) {
-      // partial sums: one for each workgroup of the pass (at head size 128 there
-      // are two across the columns), and of the scan over the segments
-      const int64_t across = std::max(Dk, Dv) > 64 ? (Dk + 63) / 64 : 1;
+      // partial sums: one for each workgroup of the pass and of the scan
       const int64_t blocks = split ? (Dk * Dv + 255) / 256 : 0;
-      a.parts = (int)(s.G * across + blocks);
+      a.parts = (int)(s.G + blocks);
       part = torch::empty({B, H, a.parts}, f32);
       a.decay_part = part.data_ptr<float>();
       if (split) {
@@ -1318,7 +1297,7 @@ std::vector<torch::Tensor> linear_attention_bwd(
       if (split) {
         hipLaunchKernelGGL(la_scan_decay, dim3((unsigned)(B * H), (unsigned)blocks), dim3(256), 0, stream,
                            a.seg_d, v_args.seg, v_args.seg_count, dstate_in, a.log_decay, a.decay_part,
-                           a.parts, (int)(s.G * across), (int)H, s.G, Dk * Dv);
+                           a.parts, s.G, (int)H, s.G, Dk * Dv);
         HIP_CHECK(hipGetLastError());
       }
       hipLaunchKernelGGL(la_decay_sum, dim3((unsigned)H), dim3(256), 0, stream,
