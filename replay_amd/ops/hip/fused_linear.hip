@@ -349,6 +349,9 @@ __global__ __launch_bounds__(WM * WN * 64) void gemm_tile(Gemm p) {
     if constexpr (DIRECT) {
       const char* ab = a_base + it * a_step;
       const char* bb = b_base + it * b_step;
+      // the bases stay scalar, so that a load's address is these and one offset
+      // register; the compiler would step a pointer of two for each load
+      asm volatile("" : "+s"(ab), "+s"(bb));
       const bool whole = k0 + BK <= k_end;  // the same for all
       auto load = [&](const char* src, char* dst) {
         __builtin_amdgcn_global_load_lds((const void*)src, (__attribute__((address_space(3))) void*)dst, 16, 0, 0);
@@ -409,19 +412,17 @@ __global__ __launch_bounds__(WM * WN * 64) void gemm_tile(Gemm p) {
     const char* b_s = a_s + A::BYTES;
 #pragma unroll
     for (int kb = 0; kb < 2; ++kb) {
-      uint4 fa[MI], fb[NI];
-#pragma unroll
-      for (int i = 0; i < MI; ++i) fa[i] = a_frag.get(a_s, i, kb);
+      uint4 fb[NI];
 #pragma unroll
       for (int j = 0; j < NI; ++j) fb[j] = b_frag.get(b_s, j, kb);
 #pragma unroll
-      for (int i = 0; i < MI; ++i)
+      for (int i = 0; i < MI; ++i) {
+        const uint4 fa = a_frag.get(a_s, i, kb);
 #pragma unroll
-        for (int j = 0; j < NI; ++j) acc[i][j] = mfma_block<T>(fb[j], fa[i], acc[i][j]);
-      if constexpr (SUMS) {
-        if (want_sums)
-#pragma unroll
-          for (int i = 0; i < MI; ++i) sums[i] = mfma_block<T>(ones_chunk<T>(), fa[i], sums[i]);
+        for (int j = 0; j < NI; ++j) acc[i][j] = mfma_block<T>(fb[j], fa, acc[i][j]);
+        if constexpr (SUMS) {
+          if (want_sums) sums[i] = mfma_block<T>(ones_chunk<T>(), fa, sums[i]);
+        }
       }
     }
   };
@@ -467,9 +468,13 @@ __global__ __launch_bounds__(WM * WN * 64) void gemm_tile(Gemm p) {
   __syncthreads();  // the stages now hold the output blocks
 
   constexpr int WNC = BN / WN, V = 16 / sizeof(T);
+  // worked out anew: kept through the loop, what follows takes registers there
+  int lane_out = threadIdx.x & 63;
+  asm volatile("" : "+v"(lane_out));
+  const int lo_out = lane_out & 15, g_out = lane_out >> 4;
   float* block = reinterpret_cast<float*>(stage0) + wave * 16 * (WNC + 4);
   float bias[V];
-  const int n_lane = n0 + wn + (lane % (WNC / V)) * V;
+  const int n_lane = n0 + wn + (lane_out % (WNC / V)) * V;
   if (p.bias) {
     load_row<T, V>(reinterpret_cast<const T*>(p.bias) + n_lane, p.N - n_lane, bias);
   } else {
@@ -482,10 +487,10 @@ __global__ __launch_bounds__(WM * WN * 64) void gemm_tile(Gemm p) {
       const int m = m0 + wm + 16 * i;
 #pragma unroll
       for (int j = 0; j < NI; ++j)
-        *reinterpret_cast<f32x4*>(block + lo * (WNC + 4) + 16 * j + 4 * g) = acc[i][j];
-      finish_block<T, WNC, decltype(act)::value>(p, block, lane, m, n0 + wn, bias);
+        *reinterpret_cast<f32x4*>(block + lo_out * (WNC + 4) + 16 * j + 4 * g_out) = acc[i][j];
+      finish_block<T, WNC, decltype(act)::value>(p, block, lane_out, m, n0 + wn, bias);
       if constexpr (SUMS) {
-        if (want_sums && g == 0 && m + lo < p.M) p.row_part[(int64_t)blockIdx.y * p.M + m + lo] = sums[i][0];
+        if (want_sums && g_out == 0 && m + lo_out < p.M) p.row_part[(int64_t)blockIdx.y * p.M + m + lo_out] = sums[i][0];
       }
     }
   };
@@ -652,7 +657,11 @@ void launch_gemm(const Gemm& p, Tile tile, int parts, hipStream_t stream) {
     }
     FL_TILE(64, 64, 2, 2, true, 2);
   }
-  if (tile == T256 || tile == T128) FL_TILE(128, 128, 2, 2, false, 2);
+  // through registers the larger tile only pays where the products bound
+  // (20001 x 501 by K 1001: 131 us with T128, 101 with T64)
+  if constexpr (A_KM) {
+    if (tile == T256) FL_TILE(128, 128, 2, 2, false, 2);
+  }
   FL_TILE(64, 64, 2, 2, false, 2);
 #undef FL_TILE
 }
@@ -756,13 +765,18 @@ void backward_t(const torch::Tensor& dy, const torch::Tensor& x, const torch::Te
     p.M = N;
     p.N = K;
     p.K = M;
-    // the rows are cut into parts of 256 at least, for two workgroups a CU (of
-    // the smallest tile, which holds less in flight, four)
-    const int64_t most = std::max<int64_t>(1, M / 256);
-    // (T256's registers are full already: 849 us against 647 for 4096 x 4096 by 16384)
-    const Tile dw_tile = N <= 64 || K <= 64 ? T64 : T128;
+    // The rows are cut into parts, of 256 rows at least, until there is a
+    // workgroup a CU: more parts are more float partials to write and read back.
+    // us by workgroups 128, 256, 512, 1024: 1024 x 256 by 25601 rows 46, 37, 42,
+    // 56; 64 x 64 by 409600 (T64) 30, 21, 24, 27.  Where the tiles alone fill
+    // half the card, two a CU (2048 x 2048 by 8192: 131, 118).  (T256's registers
+    // are full already: 849 us against 647 for 4096 x 4096 by 16384.)  Through
+    // registers, small tiles and many: 500 x 1000 by 20000, 154 with T128, 89.
+    const bool direct = chunks_aligned<T>(p.a, p.lda, N) && chunks_aligned<T>(p.b, p.ldb, K);
+    const Tile dw_tile = !direct || N <= 64 || K <= 64 ? T64 : T128;
     const int64_t tiles = std::max<int64_t>(tile_count(dw_tile, N, K), 1);
-    int64_t parts = std::max<int64_t>(1, std::min<int64_t>((dw_tile == T64 ? 1024 : 512) / tiles, most));
+    const int64_t most = std::max<int64_t>(1, M / 256), want = !direct ? 1024 : tiles >= 128 ? 512 : 256;
+    int64_t parts = std::max<int64_t>(1, std::min<int64_t>(want / tiles, most));
     p.k_part = std::max<int64_t>(64, ((M + parts - 1) / parts + 63) / 64 * 64);
     parts = std::max<int64_t>(1, (M + p.k_part - 1) / p.k_part);
     auto part = torch::empty({parts, N, K}, f32);
