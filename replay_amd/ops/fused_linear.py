@@ -37,30 +37,18 @@ def eager_fused_linear(x, weight, bias, activation: str, residual) -> torch.Tens
     return z if residual is None else z + residual
 
 
-def _unit_stride(t: torch.Tensor) -> torch.Tensor:
-    return t if t.stride(-1) == 1 or t.shape[-1] == 1 else t.contiguous()
-
-
 class FusedLinearFunction(torch.autograd.Function):
     """Saves x, the weight, and what the activation's slope is taken at: the
     product before the activation, or for relu without a residual the output."""
 
     @staticmethod
-    def forward(ctx, x2d, weight, bias, residual2d, activation):
-        ext = hip_ext()
-        x2d, weight = _unit_stride(x2d), _unit_stride(weight)
+    def forward(ctx, x, weight, bias, residual, act):
         grads = any(ctx.needs_input_grad[:3])
-        from_y = activation == "relu" and residual2d is None
-        want_z = grads and activation != "none" and not from_y
-        y, z = ext.fused_linear_fwd(
-            x2d, weight,
-            None if bias is None else bias.contiguous(),
-            None if residual2d is None else _unit_stride(residual2d),
-            ACTIVATIONS[activation], want_z,
-        )
+        from_y = act == ACTIVATIONS["relu"] and residual is None
+        y, z = hip_ext().fused_linear_fwd(x, weight, bias, residual, act, grads and act != 0 and not from_y)
         if grads:
-            ctx.save_for_backward(x2d, weight, y if from_y else z)
-        ctx.activation = activation
+            ctx.save_for_backward(x, weight, y if from_y else z)
+        ctx.act = act
         return y
 
     @staticmethod
@@ -69,10 +57,8 @@ class FusedLinearFunction(torch.autograd.Function):
         need_x, need_w, need_b, need_r = ctx.needs_input_grad[:4]
         dx = dw = db = None
         if need_x or need_w or need_b:
-            x2d, weight, z = ctx.saved_tensors
-            dx, dw, db = hip_ext().fused_linear_bwd(
-                _unit_stride(dy), x2d, weight, z, ACTIVATIONS[ctx.activation], need_x, need_w, need_b
-            )
+            x, weight, z = ctx.saved_tensors
+            dx, dw, db = hip_ext().fused_linear_bwd(dy, x, weight, z, ctx.act, need_x, need_w, need_b)
         return (
             dx if need_x else None,
             dw if need_w else None,
@@ -80,6 +66,24 @@ class FusedLinearFunction(torch.autograd.Function):
             dy if need_r else None,
             None,
         )
+
+
+def _check(x, weight, bias, residual) -> None:
+    given = [t for t in (x, weight, bias, residual) if t is not None]
+    if any(t.device != x.device for t in given):
+        raise ValueError("x, weight, bias and residual must be on one device")
+    if any(t.dtype != x.dtype for t in given):
+        raise ValueError("x, weight, bias and residual must share one dtype")
+    if x.dtype not in (_DTYPES if x.is_cuda else (*_DTYPES, torch.float64)):
+        raise ValueError(f"unsupported dtype {x.dtype}")
+    if x.dim() < 1 or weight.dim() != 2 or x.shape[-1] != weight.shape[1]:
+        raise ValueError(f"x [..., K] and weight [N, K] do not fit: {tuple(x.shape)}, {tuple(weight.shape)}")
+    N = weight.shape[0]
+    if bias is not None and bias.shape != (N,):
+        raise ValueError(f"bias must be ({N},), got {tuple(bias.shape)}")
+    shape = (*x.shape[:-1], N)
+    if residual is not None and residual.shape != shape:
+        raise ValueError(f"residual must be {shape}, got {tuple(residual.shape)}")
 
 
 def fused_linear(
@@ -100,36 +104,26 @@ def fused_linear(
     All tensors share dtype and device; under CUDA autocast they are cast to
     its dtype first, as ``torch.nn.Linear``'s are.  Differentiable once.
     """
-    if activation not in ACTIVATIONS:
+    act = ACTIVATIONS.get(activation)
+    if act is None:
         raise ValueError(f"activation must be one of {sorted(ACTIVATIONS)}, got {activation!r}")
-    given = [t for t in (x, weight, bias, residual) if t is not None]
-    if any(t.device != x.device for t in given):
-        raise ValueError("x, weight, bias and residual must be on one device")
-    if x.is_cuda and torch.is_autocast_enabled("cuda"):
+    if not require_hip_on_gpu(x):
+        _check(x, weight, bias, residual)
+        return eager_fused_linear(x, weight, bias, activation, residual)
+    if torch.is_autocast_enabled("cuda"):
         dt = torch.get_autocast_dtype("cuda")
         x, weight = x.to(dt), weight.to(dt)
         bias = bias.to(dt) if bias is not None else None
         residual = residual.to(dt) if residual is not None else None
-        given = [t for t in (x, weight, bias, residual) if t is not None]
-    if any(t.dtype != x.dtype for t in given):
-        raise ValueError("x, weight, bias and residual must share one dtype")
-    if x.dtype not in (_DTYPES if x.is_cuda else (*_DTYPES, torch.float64)):
-        raise ValueError(f"unsupported dtype {x.dtype}")
-    if x.dim() < 1 or weight.dim() != 2 or x.shape[-1] != weight.shape[1]:
-        raise ValueError(f"x [..., K] and weight [N, K] do not fit: {tuple(x.shape)}, {tuple(weight.shape)}")
-    N = weight.shape[0]
-    if bias is not None and bias.shape != (N,):
-        raise ValueError(f"bias must be ({N},), got {tuple(bias.shape)}")
-    shape = (*x.shape[:-1], N)
-    if residual is not None and residual.shape != shape:
-        raise ValueError(f"residual must be {shape}, got {tuple(residual.shape)}")
-    if not require_hip_on_gpu(x):
-        return eager_fused_linear(x, weight, bias, activation, residual)
-    rows = 1
-    for n in shape[:-1]:
-        rows *= n
-    y = FusedLinearFunction.apply(
-        x.reshape(rows, x.shape[-1]), weight, bias,
-        None if residual is None else residual.reshape(rows, N), activation,
-    )
-    return y.view(shape)
+    try:
+        if torch.is_grad_enabled() and (
+            x.requires_grad or weight.requires_grad
+            or (bias is not None and bias.requires_grad)
+            or (residual is not None and residual.requires_grad)
+        ):
+            return FusedLinearFunction.apply(x, weight, bias, residual, act)
+        return hip_ext().fused_linear_fwd(x, weight, bias, residual, act, False)[0]
+    except RuntimeError:
+        # the extension refuses what _check does, without the cost of asking twice
+        _check(x, weight, bias, residual)
+        raise

@@ -503,13 +503,22 @@ __global__ __launch_bounds__(WM * WN * 64) void gemm_tile(Gemm p) {
 }
 
 // out[i] = sum of the parts' element i, in a fixed order: X lanes by 4 elements
-// across, 256 / X groups down the parts, whose sums meet in LDS.
+// across, 256 / X groups down the parts, whose sums meet in LDS.  The elements
+// from size on lie apart, as another array of the same number of parts.
 template <typename T, int X>
-__global__ __launch_bounds__(256) void join_parts(const float* part, T* out, int64_t size, int parts) {
+__global__ __launch_bounds__(256) void join_parts(const float* part, T* out, int64_t size, const float* part2,
+                                                  T* out2, int64_t size2, int64_t blocks, int parts) {
   constexpr int Y = 256 / X;
   __shared__ __attribute__((aligned(16))) f32x4 group[Y][X];
   const int x = threadIdx.x % X, y = threadIdx.x / X;
-  const int64_t i = ((int64_t)blockIdx.x * X + x) * 4;
+  int64_t block = blockIdx.x;
+  if (block >= blocks) {
+    block -= blocks;
+    part = part2;
+    out = out2;
+    size = size2;
+  }
+  const int64_t i = (block * X + x) * 4;
   const int left = (int)min((int64_t)4, size - i);
   float sum[4] = {};
   if (left > 0) {
@@ -666,29 +675,45 @@ void launch_gemm(const Gemm& p, Tile tile, int parts, hipStream_t stream) {
 #undef FL_TILE
 }
 
+// Parts of out, and where given of out2, joined in one launch.
 template <typename T>
-void join(const torch::Tensor& part, torch::Tensor& out, int parts, hipStream_t stream) {
-  const int64_t size = out.numel();
-  if (size == 0) return;
+void join(const torch::Tensor& part, torch::Tensor& out, const torch::Tensor& part2, torch::Tensor out2,
+          int parts, hipStream_t stream) {
+  const int64_t size = out.numel(), size2 = out2.defined() ? out2.numel() : 0;
   // many parts of few elements: more groups a workgroup, and more workgroups
   // (1024 parts of 64 x 64: 13 us with 16 lanes across, 5 with 4)
   const int X = parts >= 128 ? 4 : 16;
-  const int64_t blocks = (size + 4 * X - 1) / (4 * X);
-  TORCH_CHECK(blocks < (int64_t(1) << 31), "fused_linear: weight too large");
-#define FL_JOIN(X)                                                                       \
-  hipLaunchKernelGGL((join_parts<T, X>), dim3((unsigned)blocks), dim3(256), 0, stream,   \
-                     part.data_ptr<float>(), reinterpret_cast<T*>(out.data_ptr()), size, parts)
+  const int64_t blocks = (size + 4 * X - 1) / (4 * X), all = blocks + (size2 + 4 * X - 1) / (4 * X);
+  if (all == 0) return;
+  TORCH_CHECK(all < (int64_t(1) << 31), "fused_linear: weight too large");
+  const float* p2 = size2 ? part2.data_ptr<float>() : nullptr;
+  T* o2 = size2 ? reinterpret_cast<T*>(out2.data_ptr()) : nullptr;
+#define FL_JOIN(X)                                                                         \
+  hipLaunchKernelGGL((join_parts<T, X>), dim3((unsigned)all), dim3(256), 0, stream,        \
+                     part.data_ptr<float>(), reinterpret_cast<T*>(out.data_ptr()), size,   \
+                     p2, o2, size2, blocks, parts)
   if (X == 4) FL_JOIN(4);
   else FL_JOIN(16);
 #undef FL_JOIN
   HIP_CHECK(hipGetLastError());
 }
 
+// [..., D] as rows of D, the last dimension contiguous.
+torch::Tensor rows_of(const torch::Tensor& t) {
+  auto r = t;
+  if (t.dim() != 2) {
+    TORCH_CHECK(t.dim() >= 1, "fused_linear: needs at least one dimension");
+    int64_t rows = 1;
+    for (int i = 0; i < t.dim() - 1; ++i) rows *= t.size(i);
+    r = t.reshape({rows, t.size(-1)});
+  }
+  return r.size(1) <= 1 || r.stride(1) == 1 ? r : r.contiguous();
+}
+
 void check_rows(const torch::Tensor& t, const torch::Tensor& x, const char* name) {
   TORCH_CHECK(t.device() == x.device() && t.scalar_type() == x.scalar_type(), "fused_linear: ", name,
               " must share type and device with x");
-  TORCH_CHECK(t.dim() == 2 && (t.size(1) <= 1 || t.stride(1) == 1), "fused_linear: ", name,
-              " needs two dimensions, the last contiguous");
+  TORCH_CHECK(t.dim() == 2, "fused_linear: ", name, " needs two dimensions");
   TORCH_CHECK(t.size(0) < (int64_t(1) << 31) - 256 && t.size(1) < (int64_t(1) << 31) - 256,
               "fused_linear: ", name, " is too large");
 }
@@ -742,7 +767,7 @@ void backward_t(const torch::Tensor& dy, const torch::Tensor& x, const torch::Te
                        slope ? reinterpret_cast<T*>(dz.data_ptr()) : nullptr,
                        db.defined() ? part.data_ptr<float>() : nullptr, M, (int)N, act, LC, rows);
     HIP_CHECK(hipGetLastError());
-    if (db.defined()) join<T>(part, db, (int)down, stream);
+    if (db.defined()) join<T>(part, db, {}, {}, (int)down, stream);
   }
   if (dx.defined()) {
     Gemm p = {};
@@ -784,33 +809,39 @@ void backward_t(const torch::Tensor& dy, const torch::Tensor& x, const torch::Te
     p.part = part.data_ptr<float>();
     p.row_part = sums ? row_part.data_ptr<float>() : nullptr;
     launch_gemm<T, false, false>(p, dw_tile, (int)parts, stream);
-    join<T>(part, dw, (int)parts, stream);
-    if (sums) join<T>(row_part, db, (int)parts, stream);
+    join<T>(part, dw, row_part, sums ? db : torch::Tensor(), (int)parts, stream);
   }
 }
 
 }  // namespace
 
-// -> {y, z or empty}
-std::vector<torch::Tensor> fused_linear_fwd(torch::Tensor x, torch::Tensor weight,
+// -> {y, of x's leading dimensions, z or empty, as rows}
+std::vector<torch::Tensor> fused_linear_fwd(torch::Tensor x_in, torch::Tensor weight,
                                             c10::optional<torch::Tensor> bias,
                                             c10::optional<torch::Tensor> residual, int64_t act,
                                             bool want_z) {
+  const c10::hip::OptionalHIPGuardMasqueradingAsCUDA guard(
+      x_in.is_cuda() ? c10::optional<c10::Device>(x_in.device()) : c10::nullopt);
+  auto x = rows_of(x_in);
   check_x(x, weight);
+  weight = rows_of(weight);
   const int64_t M = x.size(0), N = weight.size(0);
   TORCH_CHECK(act >= 0 && act <= 3, "fused_linear: unknown activation");
   if (bias.has_value()) {
     TORCH_CHECK(bias->device() == x.device() && bias->scalar_type() == x.scalar_type() &&
-                    bias->dim() == 1 && bias->size(0) == N && bias->is_contiguous(),
+                    bias->dim() == 1 && bias->size(0) == N,
                 "fused_linear: bias must be [N], of x's type and device");
+    bias = bias->contiguous();
   }
+  auto shape = x_in.sizes().vec();
+  shape.back() = N;
   if (residual.has_value()) {
+    TORCH_CHECK(residual->sizes() == c10::IntArrayRef(shape), "fused_linear: residual must be [..., N]");
+    residual = rows_of(*residual);
     check_rows(*residual, x, "residual");
-    TORCH_CHECK(residual->size(0) == M && residual->size(1) == N, "fused_linear: residual must be [M, N]");
   }
-  const c10::hip::HIPGuardMasqueradingAsCUDA guard(x.device());
   auto stream = at::cuda::getCurrentHIPStream();
-  auto y = torch::empty({M, N}, x.options());
+  auto y = torch::empty(shape, x.options());
   auto z = torch::empty({want_z ? M : 0, N}, x.options());
   Gemm p = {};
   p.bias = bias.has_value() ? bias->data_ptr() : nullptr;
@@ -825,24 +856,26 @@ std::vector<torch::Tensor> fused_linear_fwd(torch::Tensor x, torch::Tensor weigh
   return {y, z};
 }
 
-// -> {dx, dw, db}, empty where not needed.  z: what the slope is taken at
-// (for relu the output serves as well); unused without an activation.
-std::vector<torch::Tensor> fused_linear_bwd(torch::Tensor dy, torch::Tensor x, torch::Tensor weight,
+// -> {dx, dw, db}, empty where not needed.  z: what the slope is taken at (for
+// relu the output serves as well); unused without an activation.
+std::vector<torch::Tensor> fused_linear_bwd(torch::Tensor dy_in, torch::Tensor x_in, torch::Tensor weight,
                                             torch::Tensor z, int64_t act, bool need_x, bool need_w,
                                             bool need_b) {
+  const c10::hip::OptionalHIPGuardMasqueradingAsCUDA guard(
+      x_in.is_cuda() ? c10::optional<c10::Device>(x_in.device()) : c10::nullopt);
+  auto x = rows_of(x_in), dy = rows_of(dy_in);
   check_x(x, weight);
+  weight = rows_of(weight);
   check_rows(dy, x, "dy");
   const int64_t M = x.size(0), K = x.size(1), N = weight.size(0);
   TORCH_CHECK(act >= 0 && act <= 3, "fused_linear: unknown activation");
-  TORCH_CHECK(dy.size(0) == M && dy.size(1) == N, "fused_linear: dy must be [M, N]");
-  TORCH_CHECK(act == ACT_NONE || (z.is_contiguous() && z.dim() == 2 && z.size(0) == M &&
-                                  z.size(1) == N && z.scalar_type() == x.scalar_type() &&
-                                  z.device() == x.device()),
-              "fused_linear: z must be [M, N], of x's type and device");
-  const c10::hip::HIPGuardMasqueradingAsCUDA guard(x.device());
+  TORCH_CHECK(dy.size(0) == M && dy.size(1) == N, "fused_linear: dy must be [..., N]");
+  TORCH_CHECK(act == ACT_NONE || (z.is_contiguous() && z.numel() == M * N &&
+                                  z.scalar_type() == x.scalar_type() && z.device() == x.device()),
+              "fused_linear: z must be [..., N], of x's type and device");
   auto stream = at::cuda::getCurrentHIPStream();
   torch::Tensor dx, dw, db;
-  if (need_x) dx = torch::empty({M, K}, x.options());
+  if (need_x) dx = torch::empty(x_in.sizes(), x.options());
   if (need_w) dw = torch::empty({N, K}, x.options());
   if (need_b) db = torch::empty({N}, x.options());
 #define FL_BACKWARD(T) backward_t<T>(dy, x, weight, z, (int)act, dx, dw, db, stream)

@@ -1105,6 +1105,11 @@ void launch_scan(const PassArgs& a, const float* state_in, hipStream_t stream) {
   HIP_CHECK(hipGetLastError());
 }
 
+// The kernels read any strides but the last dimension's.
+torch::Tensor unit_stride(const torch::Tensor& t) {
+  return t.dim() == 0 || t.size(-1) <= 1 || t.stride(-1) == 1 ? t : t.contiguous();
+}
+
 void check_inputs(const torch::Tensor& q, const torch::Tensor& k, const torch::Tensor& v,
                   const torch::Tensor& log_decay, const c10::optional<torch::Tensor>& mask,
                   const c10::optional<torch::Tensor>& state, int dim) {
@@ -1117,8 +1122,6 @@ void check_inputs(const torch::Tensor& q, const torch::Tensor& k, const torch::T
   for (const auto& t : {q, k, v}) {
     TORCH_CHECK(t.scalar_type() == dt && t.device() == q.device(),
                 "linear attention: q, k, v must share type and device");
-    TORCH_CHECK(t.size(-1) <= 1 || t.stride(-1) == 1,
-                "linear attention: the last dimension must be contiguous");
     for (int i = 0; i < dim - 1; ++i)
       TORCH_CHECK(t.size(i) == q.size(i), "linear attention: q, k, v differ in dimension ", i);
   }
@@ -1127,7 +1130,7 @@ void check_inputs(const torch::Tensor& q, const torch::Tensor& k, const torch::T
               "linear attention: head sizes from 1 to 128");
   for (int i = 0; i < dim - 1; ++i)
     TORCH_CHECK(q.size(i) < (int64_t(1) << 31) - 256, "linear attention: dimension ", i, " is too large");
-  TORCH_CHECK(log_decay.dim() == 1 && log_decay.size(0) == q.size(1) && log_decay.is_contiguous() &&
+  TORCH_CHECK(log_decay.dim() == 1 && log_decay.size(0) == q.size(1) &&
                   log_decay.scalar_type() == torch::kFloat32 && log_decay.device() == q.device(),
               "linear attention: log_decay must be float32 [H] on the same device");
   if (mask.has_value()) {
@@ -1190,9 +1193,13 @@ std::vector<torch::Tensor> linear_attention_fwd(torch::Tensor q, torch::Tensor k
                                                 c10::optional<torch::Tensor> state, double scale,
                                                 bool want_state) {
   check_inputs(q, k, v, log_decay, mask, state, 4);
-  TORCH_CHECK(!state.has_value() || state->is_contiguous(), "linear attention: state not contiguous");
   const c10::hip::HIPGuardMasqueradingAsCUDA guard(q.device());
   auto stream = at::cuda::getCurrentHIPStream();
+  q = unit_stride(q);
+  k = unit_stride(k);
+  v = unit_stride(v);
+  log_decay = log_decay.contiguous();
+  if (state.has_value()) state = state->contiguous();
   const int64_t B = q.size(0), H = q.size(1), L = q.size(2), Dk = q.size(3), Dv = v.size(3);
   auto f32 = q.options().dtype(torch::kFloat32);
   auto out = heads_last(q, Dv);
@@ -1232,11 +1239,15 @@ std::vector<torch::Tensor> linear_attention_bwd(
   check_inputs(q, k, v, log_decay, mask, state, 4);
   check_inputs(q, k, dout, log_decay, mask, dstate, 4);
   TORCH_CHECK(dout.size(3) == v.size(3), "linear attention: dout differs from v in head size");
-  TORCH_CHECK((!state.has_value() || state->is_contiguous()) &&
-                  (!dstate.has_value() || dstate->is_contiguous()),
-              "linear attention: state not contiguous");
   const c10::hip::HIPGuardMasqueradingAsCUDA guard(q.device());
   auto stream = at::cuda::getCurrentHIPStream();
+  q = unit_stride(q);
+  k = unit_stride(k);
+  v = unit_stride(v);
+  dout = unit_stride(dout);
+  log_decay = log_decay.contiguous();
+  if (state.has_value()) state = state->contiguous();
+  if (dstate.has_value()) dstate = dstate->contiguous();
   const int64_t B = q.size(0), H = q.size(1), L = q.size(2), Dk = q.size(3), Dv = v.size(3);
   const auto dt = q.scalar_type();
   auto f32 = q.options().dtype(torch::kFloat32);
@@ -1327,11 +1338,26 @@ torch::Tensor linear_attention_step(torch::Tensor q, torch::Tensor k, torch::Ten
                                     c10::optional<torch::Tensor> active, double scale) {
   check_inputs(q, k, v, log_decay, active, state, 3);
   const int64_t B = q.size(0), H = q.size(1), Dk = q.size(2), Dv = v.size(2);
-  TORCH_CHECK(state.stride(3) == 1 && state.stride(2) == Dv,
+  TORCH_CHECK((Dv <= 1 || state.stride(3) == 1) && (Dk <= 1 || state.stride(2) == Dv),
               "linear attention: each head's state must be contiguous");
+  if (!state.is_contiguous() && state.numel()) {
+    // the blocks in the order of the smaller stride, then the larger: each step
+    // has to pass what lies below it
+    const int in = B > 1 && (H <= 1 || state.stride(0) < state.stride(1)) ? 0 : 1, outer = 1 - in;
+    int64_t reach = Dk * Dv;
+    for (int i : {in, outer}) {
+      if (state.size(i) <= 1) continue;
+      TORCH_CHECK(state.stride(i) >= reach, "linear attention: blocks of the state overlap in memory");
+      reach += state.stride(i) * (state.size(i) - 1);
+    }
+  }
   TORCH_CHECK(B * H < (int64_t(1) << 31), "linear attention: too many (batch, head)s");
   const c10::hip::HIPGuardMasqueradingAsCUDA guard(q.device());
   auto stream = at::cuda::getCurrentHIPStream();
+  q = unit_stride(q);
+  k = unit_stride(k);
+  v = unit_stride(v);
+  log_decay = log_decay.contiguous();
   auto out = torch::empty({B, H, Dv}, q.options());
   if (B * H == 0) return out;
   const bool* act = active.has_value() ? active->data_ptr<bool>() : nullptr;

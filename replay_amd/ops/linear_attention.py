@@ -36,6 +36,14 @@ MAX_HEAD_DIM = 128
 _DTYPES = (torch.bfloat16, torch.float16, torch.float32)
 
 
+def _scale(q: torch.Tensor, scale: Optional[float]) -> float:
+    if scale is None:
+        return 1.0 / math.sqrt(max(q.shape[-1], 1)) if q.dim() else 1.0
+    if not math.isfinite(scale):
+        raise ValueError("scale must be finite")
+    return float(scale)
+
+
 def _check(q, k, v, log_decay, mask, state, scale, dims: int, mask_name: str, state_name: str) -> None:
     where = "[B, H, L, D]" if dims == 4 else "[B, H, D]"
     for name, t in (("q", q), ("k", k), ("v", v)):
@@ -64,13 +72,6 @@ def _check(q, k, v, log_decay, mask, state, scale, dims: int, mask_name: str, st
         shape = (q.shape[0], q.shape[1], q.shape[-1], v.shape[-1])
         if state.dtype != wide or tuple(state.shape) != shape or state.device != q.device:
             raise ValueError(f"{state_name} must be {wide} of shape {shape} on q's device")
-    if not math.isfinite(scale):
-        raise ValueError("scale must be finite")
-
-
-def _unit_stride(t: torch.Tensor) -> torch.Tensor:
-    """The kernels read any strides but the last dimension's."""
-    return t if t.stride(-1) == 1 or t.shape[-1] == 1 else t.contiguous()
 
 
 def _power(log_decay: torch.Tensor, n: torch.Tensor) -> torch.Tensor:
@@ -117,12 +118,7 @@ class LinearAttentionFunction(torch.autograd.Function):
 
     @staticmethod
     def forward(ctx, q, k, v, log_decay, padding_mask, initial_state, scale, return_state):
-        ext = hip_ext()
-        q, k, v = _unit_stride(q), _unit_stride(k), _unit_stride(v)
-        log_decay = log_decay.contiguous()
-        if initial_state is not None:
-            initial_state = initial_state.contiguous()
-        out, state, seg = ext.linear_attention_fwd(
+        out, state, seg = hip_ext().linear_attention_fwd(
             q, k, v, log_decay, padding_mask, initial_state, scale, return_state
         )
         ctx.save_for_backward(q, k, v, log_decay, padding_mask, initial_state, seg)
@@ -133,25 +129,17 @@ class LinearAttentionFunction(torch.autograd.Function):
     @staticmethod
     @once_differentiable
     def backward(ctx, dout, dstate):
-        ext = hip_ext()
         q, k, v, log_decay, padding_mask, initial_state, seg = ctx.saved_tensors
         if dout is None:
             if dstate is None:
                 return (None,) * 8
             dout = torch.zeros_like(v)
-        if dstate is not None:
-            dstate = dstate.contiguous()
-        dq, dk, dv, ddecay, ds0 = ext.linear_attention_bwd(
-            q, k, v, log_decay, padding_mask, initial_state, _unit_stride(dout), dstate, seg,
-            ctx.scale, ctx.needs_input_grad[3], initial_state is not None and ctx.needs_input_grad[5],
+        need_decay = ctx.needs_input_grad[3]
+        need_state = initial_state is not None and ctx.needs_input_grad[5]
+        dq, dk, dv, ddecay, ds0 = hip_ext().linear_attention_bwd(
+            q, k, v, log_decay, padding_mask, initial_state, dout, dstate, seg, ctx.scale, need_decay, need_state
         )
-        return (
-            dq, dk, dv,
-            ddecay if ctx.needs_input_grad[3] else None,
-            None,
-            ds0 if initial_state is not None and ctx.needs_input_grad[5] else None,
-            None, None,
-        )
+        return dq, dk, dv, ddecay if need_decay else None, None, ds0 if need_state else None, None, None
 
 
 def linear_attention(
@@ -179,14 +167,24 @@ def linear_attention(
 
     Differentiable once in q, k, v, log_decay and initial_state.
     """
-    scale = 1.0 / math.sqrt(max(q.shape[-1], 1)) if scale is None else float(scale)
-    _check(q, k, v, log_decay, padding_mask, initial_state, scale, 4, "padding_mask", "initial_state")
+    scale = _scale(q, scale)
+    args = (q, k, v, log_decay, padding_mask, initial_state, scale)
     if not require_hip_on_gpu(q):
-        out, state = eager_linear_attention(q, k, v, log_decay, padding_mask, initial_state, scale)
-    else:
-        out, state = LinearAttentionFunction.apply(
-            q, k, v, log_decay, padding_mask, initial_state, scale, return_state
-        )
+        _check(*args, 4, "padding_mask", "initial_state")
+        out, state = eager_linear_attention(*args)
+        return (out, state) if return_state else out
+    try:
+        if torch.is_grad_enabled() and (
+            q.requires_grad or k.requires_grad or v.requires_grad or log_decay.requires_grad
+            or (initial_state is not None and initial_state.requires_grad)
+        ):
+            out, state = LinearAttentionFunction.apply(*args, return_state)
+        else:
+            out, state, _ = hip_ext().linear_attention_fwd(*args, return_state)
+    except RuntimeError:
+        # the extension refuses what _check does, without the cost of asking twice
+        _check(*args, 4, "padding_mask", "initial_state")
+        raise
     return (out, state) if return_state else out
 
 
@@ -208,36 +206,48 @@ def linear_attention_step(
         zero output.
     :return: [B, H, Dv] in q's dtype.
     """
-    scale = 1.0 / math.sqrt(max(q.shape[-1], 1)) if scale is None else float(scale)
-    _check(q, k, v, log_decay, active, state, scale, 3, "active", "state")
-    if torch.is_grad_enabled() and any(t.requires_grad for t in (q, k, v, log_decay, state)):
+    scale = _scale(q, scale)
+    if torch.is_grad_enabled() and (
+        q.requires_grad or k.requires_grad or v.requires_grad or log_decay.requires_grad or state.requires_grad
+    ):
         raise RuntimeError(
             "linear_attention_step updates the state in place and is not differentiable: "
             "call it under torch.no_grad(), or use linear_attention"
         )
-    B, H, Dk, Dv = state.shape
-    if state.numel() and (
-        (Dv > 1 and state.stride(3) != 1) or (Dk > 1 and state.stride(2) != Dv)
-    ):
-        raise ValueError("each head's [Dk, Dv] block of the state must be contiguous")
-    if state.numel():
-        # rows and heads in the order of their strides, each past the one before
-        reach = Dk * Dv
-        for stride, size in sorted(((state.stride(i), state.shape[i]) for i in (0, 1)), key=lambda p: p[0]):
-            if size > 1:
-                if stride < reach:
-                    raise ValueError("blocks of the state overlap in memory")
-                reach = stride * (size - 1) + reach
     if not require_hip_on_gpu(q):
-        wide = log_decay.dtype
-        qw, kw, vw = q.to(wide), k.to(wide), v.to(wide)
-        new = torch.exp(log_decay).view(1, H, 1, 1) * state + kw[..., :, None] * vw[..., None, :]
-        out = (qw[..., :, None] * new).sum(-2) * scale
-        if active is not None:
-            new = torch.where(active.view(-1, 1, 1, 1), new, state)
-            out = torch.where(active.view(-1, 1, 1), out, torch.zeros_like(out))
-        state.copy_(new)
-        return out.to(q.dtype)
-    return hip_ext().linear_attention_step(
-        _unit_stride(q), _unit_stride(k), _unit_stride(v), log_decay.contiguous(), state, active, scale
-    )
+        _check(q, k, v, log_decay, active, state, scale, 3, "active", "state")
+        _check_blocks(state)
+        return _eager_step(q, k, v, log_decay, state, active, scale)
+    try:
+        return hip_ext().linear_attention_step(q, k, v, log_decay, state, active, scale)
+    except RuntimeError:
+        # the extension refuses what these do, without the cost of asking twice
+        _check(q, k, v, log_decay, active, state, scale, 3, "active", "state")
+        _check_blocks(state)
+        raise
+
+
+def _check_blocks(state: torch.Tensor) -> None:
+    B, H, Dk, Dv = state.shape
+    if not state.numel():
+        return
+    if (Dv > 1 and state.stride(3) != 1) or (Dk > 1 and state.stride(2) != Dv):
+        raise ValueError("each head's [Dk, Dv] block of the state must be contiguous")
+    # rows and heads in the order of their strides, each past the one before
+    reach = Dk * Dv
+    for stride, size in sorted((state.stride(i), state.shape[i]) for i in (0, 1) if state.shape[i] > 1):
+        if stride < reach:
+            raise ValueError("blocks of the state overlap in memory")
+        reach += stride * (size - 1)
+
+
+def _eager_step(q, k, v, log_decay, state, active, scale: float) -> torch.Tensor:
+    wide = log_decay.dtype
+    qw, kw, vw = q.to(wide), k.to(wide), v.to(wide)
+    new = torch.exp(log_decay).view(1, -1, 1, 1) * state + kw[..., :, None] * vw[..., None, :]
+    out = (qw[..., :, None] * new).sum(-2) * scale
+    if active is not None:
+        new = torch.where(active.view(-1, 1, 1, 1), new, state)
+        out = torch.where(active.view(-1, 1, 1), out, torch.zeros_like(out))
+    state.copy_(new)
+    return out.to(q.dtype)
