@@ -157,6 +157,28 @@ __global__ __launch_bounds__(DP * 4, 2) void la_pass_f32(PassArgs a) {
   const int e0 = wave * 16, e = e0 + lo;
   const bool busy = e0 < a.De;
   const int64_t state_size = (int64_t)a.Dc * a.De;
+  // seg_chunks counts loads of 32 positions here
+  const int n_loads = (a.L + ROWS - 1) / ROWS;
+  const int first = seg * a.seg_chunks, last = min(n_loads, first + a.seg_chunks);
+  auto start_of = [&](int step) { return (REV ? first + last - 1 - step : step) * ROWS; };
+  Ch q_r(a.q, b, h, a.Dc), k_r(a.k, b, h, a.Dc), v_r(a.v, b, h, a.De), x_r(a.x, b, h, a.De);
+  // The mask is read a load ahead of the rows that it says to read.
+  const bool* mask = a.mask ? a.mask + b * a.mask_b : nullptr;
+  auto look = [&](int step) {
+    const int pos = start_of(step) + lane;
+    return lane < ROWS && step < last && pos < a.L && (!mask || mask[pos * a.mask_l]);
+  };
+  auto fetch = [&](int step, unsigned bits) {
+    const int l0 = start_of(step);
+    if (FULL) q_r.fetch(l0, bits);
+    k_r.fetch(l0, bits);
+    v_r.fetch(l0, bits);
+    if (X) x_r.fetch(l0, bits);
+  };
+  // the first loads are on their way while the rest is prepared
+  unsigned bits = (unsigned)__ballot(look(first));
+  fetch(first, bits);
+  bool ahead = look(first + 1);
   const float ld = a.log_decay[h];
   // a decay of zero (log -inf) keeps l^0 = 1
   if (threadIdx.x <= C) lam[threadIdx.x] = threadIdx.x ? expf(ld * threadIdx.x) : 1.f;
@@ -199,26 +221,6 @@ __global__ __launch_bounds__(DP * 4, 2) void la_pass_f32(PassArgs a) {
     }
   }
 
-  // seg_chunks counts loads of 32 positions here
-  const int n_loads = (a.L + ROWS - 1) / ROWS;
-  const int first = seg * a.seg_chunks, last = min(n_loads, first + a.seg_chunks);
-  auto start_of = [&](int step) { return (REV ? first + last - 1 - step : step) * ROWS; };
-  int total = 0;
-  float d_decay = 0.f;
-  Ch q_r(a.q, b, h, a.Dc), k_r(a.k, b, h, a.Dc), v_r(a.v, b, h, a.De), x_r(a.x, b, h, a.De);
-  // The mask is read a load ahead of the rows that it says to read.
-  const bool* mask = a.mask ? a.mask + b * a.mask_b : nullptr;
-  auto look = [&](int step) {
-    const int pos = start_of(step) + lane;
-    return lane < ROWS && step < last && pos < a.L && (!mask || mask[pos * a.mask_l]);
-  };
-  auto fetch = [&](int step, unsigned bits) {
-    const int l0 = start_of(step);
-    if (FULL) q_r.fetch(l0, bits);
-    k_r.fetch(l0, bits);
-    v_r.fetch(l0, bits);
-    if (X) x_r.fetch(l0, bits);
-  };
   T* out = nullptr;
   if (FULL)
     out = reinterpret_cast<T*>(a.out) + b * a.out_b + h * a.out_h +
@@ -249,9 +251,8 @@ __global__ __launch_bounds__(DP * 4, 2) void la_pass_f32(PassArgs a) {
     }
   };
 
-  unsigned bits = (unsigned)__ballot(look(first));
-  fetch(first, bits);
-  bool ahead = look(first + 1);
+  int total = 0;
+  float d_decay = 0.f;
 #pragma unroll 1
   for (int step = first; step < last; ++step) {
     const int l0 = start_of(step);
@@ -564,7 +565,10 @@ __global__ __launch_bounds__(DP * 4, DERIV ? 2 : 3) void la_pass_bf16(PassArgs a
   __shared__ __attribute__((aligned(16))) char k_s[Ch::BYTES];
   __shared__ __attribute__((aligned(16))) char v_s[Ch::BYTES];
   __shared__ uint4 p_s[FULL ? 6 : 1][64];    // pair weights, as operands
-  __shared__ f32x4 full_s[FULL ? 4 : 1][64]; // those of a chunk without gaps, by tile distance
+  // those of a chunk without gaps, by tile distance (at head size 32 not worth
+  // their room: a workgroup less a CU)
+  constexpr bool TABLE = FULL && DP > 32;
+  __shared__ f32x4 full_s[TABLE ? 4 : 1][64];
   __shared__ __attribute__((aligned(16))) char x_s[X ? Ch::BYTES : 16];
   // of each position: the valid ones up to it, and its weights in the product
   // with the start state and in the state's update
@@ -582,6 +586,27 @@ __global__ __launch_bounds__(DP * 4, DERIV ? 2 : 3) void la_pass_bf16(PassArgs a
   const int e0 = wave * 16, e = e0 + lo;
   const bool busy = e0 < a.De;
   const int64_t state_size = (int64_t)a.Dc * a.De;
+  const int n_chunks = (a.L + C - 1) / C;
+  const int first = seg * a.seg_chunks, last = min(n_chunks, first + a.seg_chunks);
+  auto start_of = [&](int step) { return (REV ? first + last - 1 - step : step) * C; };
+  Ch q_r(a.q, b, h, a.Dc), k_r(a.k, b, h, a.Dc), v_r(a.v, b, h, a.De), x_r(a.x, b, h, a.De);
+  // The mask is read a chunk ahead of the rows that it says to read.
+  const bool* mask = a.mask ? a.mask + b * a.mask_b : nullptr;
+  auto look = [&](int step) {
+    const int pos = start_of(step) + lane;
+    return step < last && pos < a.L && (!mask || mask[pos * a.mask_l]);
+  };
+  auto fetch = [&](int step, uint64_t bits) {
+    const int l0 = start_of(step);
+    if (FULL) q_r.fetch(l0, bits);
+    k_r.fetch(l0, bits);
+    v_r.fetch(l0, bits);
+    if (X) x_r.fetch(l0, bits);
+  };
+  // the first loads are on their way while the rest is prepared
+  uint64_t bits = __ballot(look(first));
+  fetch(first, bits);
+  bool ahead = look(first + 1);
   const float ld = a.log_decay[h];
   // a decay of zero (log -inf) keeps l^0 = 1
   for (int i = threadIdx.x; i <= C; i += DP * 4) lam[i] = i ? expf(ld * i) : 1.f;
@@ -615,7 +640,7 @@ __global__ __launch_bounds__(DP * 4, DERIV ? 2 : 3) void la_pass_bf16(PassArgs a
   }
   __syncthreads();  // lam
 
-  if (FULL) {
+  if (TABLE) {
     for (int d = wave; d < 4; d += WAVES) {
 #pragma unroll
       for (int r = 0; r < 4; ++r) {
@@ -629,25 +654,6 @@ __global__ __launch_bounds__(DP * 4, DERIV ? 2 : 3) void la_pass_bf16(PassArgs a
   auto unit_it = [](int u) { const int it = (0x203321 >> (4 * u)) & 15; return REV ? 3 - it : it; };
   auto unit_s = [](int u) { const int s = (0x101000 >> (4 * u)) & 15; return REV ? 1 - s : s; };
 
-  const int n_chunks = (a.L + C - 1) / C;
-  const int first = seg * a.seg_chunks, last = min(n_chunks, first + a.seg_chunks);
-  auto start_of = [&](int step) { return (REV ? first + last - 1 - step : step) * C; };
-  int total = 0;
-  float d_decay = 0.f;
-  Ch q_r(a.q, b, h, a.Dc), k_r(a.k, b, h, a.Dc), v_r(a.v, b, h, a.De), x_r(a.x, b, h, a.De);
-  // The mask is read a chunk ahead of the rows that it says to read.
-  const bool* mask = a.mask ? a.mask + b * a.mask_b : nullptr;
-  auto look = [&](int step) {
-    const int pos = start_of(step) + lane;
-    return step < last && pos < a.L && (!mask || mask[pos * a.mask_l]);
-  };
-  auto fetch = [&](int step, uint64_t bits) {
-    const int l0 = start_of(step);
-    if (FULL) q_r.fetch(l0, bits);
-    k_r.fetch(l0, bits);
-    v_r.fetch(l0, bits);
-    if (X) x_r.fetch(l0, bits);
-  };
   __hip_bfloat16* out = nullptr;
   if (FULL)
     out = reinterpret_cast<__hip_bfloat16*>(a.out) + b * a.out_b + h * a.out_h +
@@ -666,9 +672,8 @@ __global__ __launch_bounds__(DP * 4, DERIV ? 2 : 3) void la_pass_bf16(PassArgs a
     }
   };
 
-  uint64_t bits = __ballot(look(first));
-  fetch(first, bits);
-  bool ahead = look(first + 1);
+  int total = 0;
+  float d_decay = 0.f;
 #pragma unroll 1
   for (int step = first; step < last; ++step) {
     const int l0 = start_of(step);
@@ -718,11 +723,11 @@ __global__ __launch_bounds__(DP * 4, DERIV ? 2 : 3) void la_pass_bf16(PassArgs a
 #pragma unroll
           for (int c = 0; c < NS; ++c) acc = mfma32(Ch::rows(k_s, 16 * jt, c, lo, g), qf[c], acc);
           f32x4 gaps;
-          if (DERIV || !whole) {
+          if (DERIV || !TABLE || !whole) {
             const f32x4 n_j = *reinterpret_cast<const f32x4*>(n_s + 16 * jt + 4 * g);
             gaps = REV ? n_j - n_i : n_i - n_j;
           }
-          if (whole) {
+          if (TABLE && whole) {
             p[u] = acc * full_s[apart][lane];
           } else {
             f32x4 w;
