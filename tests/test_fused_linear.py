@@ -178,6 +178,74 @@ class TestKernels:
         for M, K, N in ((0, 4, 5), (3, 0, 5), (3, 4, 0)):
             check(*make(M, K, N, dtype), "gelu", dtype)
 
+    def test_refusals(self):
+        x, w, b, r, _ = make(6, 4, 5, torch.float32)
+        fused_linear(x, w, b, "relu", r)
+        for change in (
+            dict(weight=w.cpu()), dict(weight=w.half()), dict(weight=w[:, :3]), dict(weight=w[0]),
+            dict(bias=b[:4]), dict(bias=b[None]), dict(bias=b.cpu()), dict(residual=r[:1]), dict(residual=r[:, :4]),
+            dict(residual=r.half()), dict(residual=r.cpu()), dict(x=x.double()), dict(x=x[0, 0]),
+            dict(x=x.double(), weight=w.double(), bias=b.double(), residual=r.double()), dict(activation="tanh"),
+        ):
+            for grad in (False, True):
+                args = {**dict(x=x, weight=w, bias=b, residual=r, activation="none"), **change}
+                args["x"] = args["x"].detach().requires_grad_(grad)
+                with pytest.raises(ValueError):
+                    fused_linear(**args)
+
+    def test_far_offsets(self):
+        # rows that end past 2^31 elements, and outputs past 2^32 bytes
+        gen = torch.Generator().manual_seed(0)
+        store = torch.empty(2**31 + 2**22, dtype=torch.bfloat16, device="cuda")
+        M, K, stride = 2049, 64, 2**20
+        x = store.as_strided((M, K), (stride, 1)).copy_(torch.randn(M, K, generator=gen))
+        w, b = (torch.randn(48, K, generator=gen) / 8).bfloat16().cuda(), torch.randn(48, generator=gen).bfloat16().cuda()
+        dy = torch.randn(M, 48, generator=gen).bfloat16().cuda()
+        leaves, near = [[t.detach().requires_grad_() for t in (a, w, b)] for a in (x, x.contiguous())]
+        for args in zip(
+            torch.autograd.grad(fused_linear(*leaves, "gelu"), leaves, dy),
+            torch.autograd.grad(fused_linear(*near, "gelu"), near, dy),
+        ):
+            assert torch.equal(*args)
+        tall = torch.randn(2**25 + 3, 8, device="cuda").bfloat16()
+        wide = torch.randn(72, 8, device="cuda").bfloat16()
+        y = fused_linear(tall, wide)
+        assert torch.equal(y[-300:], fused_linear(tall[-300:], wide))
+
+    def test_two_graphs_in_turn(self):
+        cases = [make(3000, 64, 128, torch.bfloat16, seed=i) for i in (1, 2)]
+        graphs, held = [], []
+
+        def step(x, w, b, r, dy):
+            return torch.autograd.grad(fused_linear(x, w, b, "gelu", r), [x, w, b], dy)
+
+        for case in cases:
+            for t in case[:3]:
+                t.requires_grad_()
+            side = torch.cuda.Stream()
+            side.wait_stream(torch.cuda.current_stream())
+            with torch.cuda.stream(side):
+                step(*case)
+            torch.cuda.current_stream().wait_stream(side)
+            graph = torch.cuda.CUDAGraph()
+            with torch.cuda.graph(graph, pool=graphs[0].pool() if graphs else None):
+                held.append(step(*case))
+            graphs.append(graph)
+        for _ in range(3):
+            for i, case in enumerate(cases):
+                graphs[i].replay()
+                got = [t.clone() for t in held[i]]
+                for a, c in zip(got, step(*case)):
+                    assert torch.equal(a, c)
+
+    def test_backward_twice(self):
+        x, w, b, r, dy = make(300, 64, 48, torch.bfloat16)
+        leaves = [t.requires_grad_() for t in (x, w, b, r)]
+        y = fused_linear(x, w, b, "silu", r)
+        first = torch.autograd.grad(y, leaves, dy, retain_graph=True)
+        for a, c in zip(first, torch.autograd.grad(y, leaves, dy)):
+            assert torch.equal(a, c)
+
     def test_large_values(self):
         # far beyond where exp overflows, both ways
         x = torch.tensor([[1000.0], [-1000.0], [88.0], [-88.0], [-104.0], [0.0]], device="cuda")

@@ -145,6 +145,13 @@ def run_all(q, k, v, ld, mask, s0, scale, do, ds):
     return got
 
 
+def run_all_views(qkv, ld, do):
+    """Outputs and gradients of inputs as they lie, however far apart."""
+    leaves = [t.detach().requires_grad_() for t in (*qkv, ld)]
+    out = linear_attention(*leaves)
+    return (out.detach(), *torch.autograd.grad(out, leaves, do))
+
+
 def check_all(q, k, v, ld, mask, s0, scale, do, ds, dtype):
     got = run_all(q, k, v, ld, mask, s0, scale, do, ds)
     L, Dk, Dv = q.shape[2], q.shape[3], v.shape[3]
@@ -474,6 +481,84 @@ class TestKernels:
             for got, name in zip(grads, ("dq", "dk", "dv", "ddecay")):
                 assert torch.equal(got, want[name]), name
 
+    def test_backward_twice(self):
+        q, k, v, ld, s0, do, ds = inputs(2, 2, 1100, 32, 32, torch.bfloat16, "cuda", carry=True)
+        leaves = [t.requires_grad_() for t in (q, k, v, ld, s0)]
+        out, state = linear_attention(q, k, v, ld, initial_state=s0, return_state=True)
+        first = torch.autograd.grad([out, state], leaves, [do, ds], retain_graph=True)
+        again = torch.autograd.grad([out, state], leaves, [do, ds])
+        for a, b in zip(first, again):
+            assert torch.equal(a, b)
+
+    def test_outputs_do_not_depend_on_what_else_is_asked(self):
+        q, k, v, ld, _, _, _ = inputs(2, 2, 300, 64, 64, torch.bfloat16, "cuda")
+        plain = linear_attention(q, k, v, ld)
+        with_state, _ = linear_attention(q, k, v, ld, return_state=True)
+        q.requires_grad_()
+        assert torch.equal(plain, with_state) and torch.equal(linear_attention(q, k, v, ld).detach(), plain)
+
+    def test_later_positions_do_not_matter(self):
+        q, k, v, ld, _, _, _ = inputs(2, 2, 200, 32, 32, torch.bfloat16, "cuda")
+        want = linear_attention(q, k, v, ld)[:, :, :77]
+        for t in (q, k, v):
+            t[:, :, 77:] *= 3
+        assert torch.equal(linear_attention(q, k, v, ld)[:, :, :77], want)
+
+    @pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32], ids=str)
+    def test_far_offsets(self, dtype):
+        # the second row lies past 2^32 bytes and 2^31 elements from the first
+        far = 2**31 + 64
+        store = torch.empty(far + 2**16, dtype=dtype, device="cuda")
+        views = []
+        for i, t in enumerate(inputs(2, 2, 70, 32, 32, dtype, "cuda")[:3]):
+            view = store.as_strided((2, 2, 70, 32), (far, 70 * 32, 32, 1), i * 8192)
+            views.append(view.copy_(t))
+        near = [t.contiguous() for t in views]
+        _, _, _, ld, _, do, _ = inputs(2, 2, 70, 32, 32, dtype, "cuda")
+        got, want = run_all_views(views, ld, do), run_all_views(near, ld, do)
+        for a, b in zip(got, want):
+            assert torch.equal(a, b)
+
+    def test_two_graphs_in_turn(self):
+        args = [inputs(2, 2, 1100, 32, 32, torch.bfloat16, "cuda", seed=i) for i in (1, 2)]
+        graphs, held = [], []
+        for q, k, v, ld, _, do, _ in args:
+            leaves = [t.requires_grad_() for t in (q, k, v, ld)]
+            side = torch.cuda.Stream()
+            side.wait_stream(torch.cuda.current_stream())
+            with torch.cuda.stream(side):
+                torch.autograd.grad(linear_attention(*leaves), leaves, do)
+            torch.cuda.current_stream().wait_stream(side)
+            graph = torch.cuda.CUDAGraph()
+            with torch.cuda.graph(graph, pool=graphs[0].pool() if graphs else None):
+                held.append(torch.autograd.grad(linear_attention(*leaves), leaves, do))
+            graphs.append(graph)
+        for _ in range(3):
+            for i, (graph, (q, k, v, ld, _, do, _)) in enumerate(zip(graphs, args)):
+                graph.replay()
+                got = [t.clone() for t in held[i]]
+                want = torch.autograd.grad(linear_attention(q, k, v, ld), [q, k, v, ld], do)
+                for a, b in zip(got, want):
+                    assert torch.equal(a, b)
+
+    def test_refusals(self):
+        q, k, v, ld, s0, _, _ = inputs(2, 3, 4, 5, 6, torch.float32, "cuda", carry=True)
+        mask = torch.ones(2, 4, dtype=torch.bool, device="cuda")
+        good = dict(q=q, k=k, v=v, log_decay=ld, padding_mask=mask, initial_state=s0)
+        linear_attention(**good)
+        for change in (
+            dict(k=k.cpu()), dict(v=v.half()), dict(k=k[:, :1]), dict(k=k[..., :4]), dict(v=v[:, :, :3]),
+            dict(q=q[0]), dict(log_decay=ld[:2]), dict(log_decay=ld.double()), dict(log_decay=ld.cpu()),
+            dict(padding_mask=mask.float()), dict(padding_mask=mask.t()), dict(padding_mask=mask.cpu()),
+            dict(initial_state=s0.half()), dict(initial_state=s0.transpose(2, 3)), dict(scale=math.inf),
+            dict(q=q.double(), k=k.double(), v=v.double()), dict(v=torch.zeros(2, 3, 4, 129, device="cuda")),
+        ):
+            for grad in (False, True):
+                with pytest.raises(ValueError):
+                    args = {**good, **change}
+                    args["q"] = args["q"].detach().requires_grad_(grad)
+                    linear_attention(**args)
+
     def test_differentiable_once(self):
         q, k, v, ld, _, _, _ = inputs(1, 1, 5, 8, 8, torch.float32, "cuda")
         q.requires_grad_()
@@ -531,6 +616,24 @@ class TestStepKernel:
         assert torch.equal(store[::2, 1], want)
         kept[::2, 1] = want
         assert torch.equal(store, kept)
+
+    def test_refusals(self):
+        q, k, v, ld, s0, _, _ = inputs(2, 3, 1, 5, 6, torch.float32, "cuda", carry=True)
+        q, k, v = (t[:, :, 0] for t in (q, k, v))
+        store = torch.zeros(200, device="cuda")
+        for state in (
+            s0.cpu(), s0.half(), s0[:1], s0.transpose(2, 3).contiguous().transpose(2, 3),
+            s0[:1].expand(2, 3, 5, 6), store.as_strided((2, 3, 5, 6), (31, 30, 6, 1)),
+            store.as_strided((2, 3, 5, 6), (30, 31, 6, 1)),
+        ):
+            kept = state.clone()
+            with pytest.raises(ValueError):
+                linear_attention_step(q, k, v, ld, state)
+            assert torch.equal(state, kept)
+        # rows inside the heads' stride are as good as heads inside the rows'
+        linear_attention_step(q, k, v, ld, store.as_strided((2, 3, 5, 6), (30, 60, 6, 1)))
+        with pytest.raises(ValueError):
+            linear_attention_step(q, k, v, ld, s0, active=torch.ones(3, dtype=torch.bool, device="cuda"))
 
     def test_steps_match_the_whole(self):
         q, k, v, ld, s0, _, _ = inputs(3, 2, 20, 32, 32, torch.float32, "cuda", carry=True)
