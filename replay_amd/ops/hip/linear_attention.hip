@@ -765,39 +765,35 @@ __global__ __launch_bounds__(DP * 4, DERIV ? 2 : 3) void la_pass_bf16(PassArgs a
 #pragma unroll
         for (int it = 0; it < 4; ++it) o[it] = f32x4{0.f, 0.f, 0.f, 0.f};
         if (started) {
-          // what of the decay's gradient goes by x . (S' q) w, a block at a time too
-          auto weighted_x = [&](int it) {
-            return inter_s[16 * it + lo] *
-                   widen(*reinterpret_cast<const bf16x4*>(x_s + (16 * it + lo) * LD + (e0 + 4 * g) * 2));
-          };
+          f32x4 od[DERIV ? 4 : 1];
+          if (DERIV) {
+#pragma unroll
+            for (int it = 0; it < 4; ++it) od[it] = f32x4{0.f, 0.f, 0.f, 0.f};
+          }
 #pragma unroll
           for (int s = 0; s < NS; ++s) {
             asm volatile("" ::: "memory");
             const Split8<DERIV ? 3 : 2> state(S[2 * s], S[2 * s + 1]);
+            const Split8<3> state_d(Sd[DERIV ? 2 * s : 0], Sd[DERIV ? 2 * s + 1 : 0]);
 #pragma unroll
             for (int it = 0; it < 4; ++it) {
               if (DERIV) asm volatile("" ::: "memory");
-              o[it] = state.times(Ch::rows(q_s, 16 * it, s, lo, g), o[it]);
-            }
-            if (DERIV) {
-              asm volatile("" ::: "memory");
-              const Split8<3> state_d(Sd[DERIV ? 2 * s : 0], Sd[DERIV ? 2 * s + 1 : 0]);
-#pragma unroll
-              for (int it = 0; it < 4; ++it) {
-                asm volatile("" ::: "memory");
-                const f32x4 od = state_d.times(Ch::rows(q_s, 16 * it, s, lo, g), f32x4{0.f, 0.f, 0.f, 0.f});
-                const f32x4 part = weighted_x(it) * od;
-                d_decay += (part[0] + part[1]) + (part[2] + part[3]);
-              }
+              const bf16x8 qf = Ch::rows(q_s, 16 * it, s, lo, g);
+              o[it] = state.times(qf, o[it]);
+              if (DERIV) od[it] = state_d.times(qf, od[it]);
             }
           }
 #pragma unroll
           for (int it = 0; it < 4; ++it) {
-            if (DERIV) {
-              const f32x4 part = weighted_x(it) * o[it];
-              d_decay += n_s[16 * it + lo] * ((part[0] + part[1]) + (part[2] + part[3]));
+            const int i = 16 * it + lo;
+            const float w_i = inter_s[i];
+            if (DERIV) {  // of the decay's gradient, x . (S' + n S) q w
+              od[it] = w_i * (od[it] + n_s[i] * o[it]);
+              const f32x4 xv = widen(*reinterpret_cast<const bf16x4*>(x_s + i * LD + (e0 + 4 * g) * 2));
+#pragma unroll
+              for (int r = 0; r < 4; ++r) d_decay += xv[r] * od[it][r];
             }
-            o[it] = inter_s[16 * it + lo] * o[it];
+            o[it] = w_i * o[it];
           }
         }
       }
@@ -947,17 +943,30 @@ __global__ __launch_bounds__(256) void la_scan_decay(const float* seg_d, const f
 }
 
 // part [B, H, parts] -> [H]; a fixed order, in 64 bits (the parts may cancel).
-__global__ void la_decay_sum(const float* part, float* out, int B, int H, int parts) {
-  __shared__ double red[4];
+__global__ __launch_bounds__(1024) void la_decay_sum(const float* part, float* out, int B, int H, int parts) {
+  __shared__ double red[16];
   const int h = blockIdx.x;
+  const int64_t n = (int64_t)B * parts;
   double sum = 0.0;
-  for (int64_t i = threadIdx.x; i < (int64_t)B * parts; i += blockDim.x)
-    sum += part[((i / parts) * H + h) * parts + i % parts];
+  for (int64_t i0 = threadIdx.x; i0 < n; i0 += 8 * 1024) {
+    float v[8];  // in flight together: this is all latency
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+      const int64_t i = i0 + j * 1024;
+      v[j] = i < n ? part[((i / parts) * H + h) * parts + i % parts] : 0.f;
+    }
+#pragma unroll
+    for (int j = 0; j < 8; ++j) sum += v[j];
+  }
 #pragma unroll
   for (int off = 32; off > 0; off >>= 1) sum += __shfl_xor(sum, off, WAVE);
   if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = sum;
   __syncthreads();
-  if (threadIdx.x == 0) out[h] = (float)(red[0] + red[1] + red[2] + red[3]);
+  if (threadIdx.x == 0) {
+    double all = 0.0;
+    for (int w = 0; w < 16; ++w) all += red[w];
+    out[h] = (float)all;
+  }
 }
 
 // One position for each row: the state is read, updated and written once, and
@@ -1316,7 +1325,7 @@ std::vector<torch::Tensor> linear_attention_bwd(
                            a.parts, s.G, (int)H, s.G, Dk * Dv);
         HIP_CHECK(hipGetLastError());
       }
-      hipLaunchKernelGGL(la_decay_sum, dim3((unsigned)H), dim3(256), 0, stream,
+      hipLaunchKernelGGL(la_decay_sum, dim3((unsigned)H), dim3(1024), 0, stream,
                          part.data_ptr<float>(), ddecay.data_ptr<float>(), (int)B, (int)H, a.parts);
       HIP_CHECK(hipGetLastError());
     } else {
