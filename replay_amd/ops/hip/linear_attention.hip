@@ -498,12 +498,13 @@ __device__ __forceinline__ void store8(__hip_bfloat16* p, int n, uint4 v) {
 
 // One operand's 64 positions on their way from memory to LDS: 16-byte pieces,
 // DP / 8 of 4 DP threads a row.
-template <int DP, bool EDGE>
+template <int DP, bool EDGE, bool ROWS>
 struct Chunk {
   static constexpr int C = 64, ACROSS = DP / 8, DOWN = DP * 4 / ACROSS, PIECES = C / DOWN;
   // rows 16 bytes apart from a power of two: the fragment reads of 16 rows
-  // then start in banks 4 words apart
-  static constexpr int LD = DP * 2 + 16, BYTES = C * LD;
+  // then start in banks 4 words apart.  Without such reads, 32 bytes: the
+  // transposing reads of 8 rows then fill the banks.
+  static constexpr int LD = DP * 2 + (ROWS ? 16 : 32), BYTES = C * LD;
 
   const __hip_bfloat16* at;  // this thread's first piece of position 0
   int64_t l;
@@ -548,17 +549,23 @@ struct Chunk {
   }
 };
 
-// The contraction index of row 4 g + r of the state's tile t.
+// The contraction index of row 4 g + r of the state's tile t; in memory's order
+// (the state-only pass, whose state is no operand) or permuted.
+template <bool PERMUTED>
 __device__ __forceinline__ int state_row(int t, int g, int r) {
-  return 32 * (t >> 1) + 8 * g + 4 * (t & 1) + r;
+  return PERMUTED ? 32 * (t >> 1) + 8 * g + 4 * (t & 1) + r : 16 * t + 4 * g + r;
 }
 
 // DP / 16 waves, each with 16 value columns and the whole contraction axis.  The
 // launch bounds are the tightest that need no spills: with spills, first chunks
-// came out wrong now and then.
-template <int DP, bool REV, bool STATE_ONLY, bool DERIV, bool EDGE>
-__global__ __launch_bounds__(DP * 4, DERIV ? 2 : 3) void la_pass_bf16(PassArgs a) {
-  using Ch = Chunk<DP, EDGE>;
+// came out wrong now and then.  AHEAD: a chunk's rows are loaded while the one
+// before is worked on.  At head size 128 two workgroups a CU (128 registers)
+// without that hide the loads better than one with it, where there are as many:
+// 64 x 8 heads of 512, 57 us against 80; 2 x 8 of 16384 in 256 workgroups, 147
+// against 122.
+template <int DP, bool REV, bool STATE_ONLY, bool DERIV, bool EDGE, bool AHEAD>
+__global__ __launch_bounds__(DP * 4, DERIV ? 2 : AHEAD ? 3 : 4) void la_pass_bf16(PassArgs a) {
+  using Ch = Chunk<DP, EDGE, !STATE_ONLY>;
   constexpr int C = 64, NS = DP / 32, NT = DP / 16, LD = Ch::LD, WAVES = DP / 16;
   constexpr bool FULL = !STATE_ONLY, X = DERIV && FULL;
   __shared__ __attribute__((aligned(16))) char q_s[FULL ? Ch::BYTES : 16];
@@ -605,7 +612,7 @@ __global__ __launch_bounds__(DP * 4, DERIV ? 2 : 3) void la_pass_bf16(PassArgs a
   };
   // the first loads are on their way while the rest is prepared
   uint64_t bits = __ballot(look(first));
-  fetch(first, bits);
+  if (AHEAD) fetch(first, bits);
   bool ahead = look(first + 1);
   const float ld = a.log_decay[h];
   // a decay of zero (log -inf) keeps l^0 = 1
@@ -631,7 +638,7 @@ __global__ __launch_bounds__(DP * 4, DERIV ? 2 : 3) void la_pass_bf16(PassArgs a
       asm volatile("" : "+v"(g_t)::"memory");
 #pragma unroll
       for (int r = 0; r < 4; ++r) {
-        const int c = state_row(t, g_t, r);
+        const int c = state_row<FULL>(t, g_t, r);
         const bool in = c < a.Dc && e < a.De;
         S[t][r] = (src && in) ? src[c * a.st_c + e * a.st_e] : 0.f;
         if (DERIV) Sd[t][r] = 0.f;
@@ -684,6 +691,7 @@ __global__ __launch_bounds__(DP * 4, DERIV ? 2 : 3) void la_pass_bf16(PassArgs a
     // round the loop for both cases: a second one, with a continue, kept copies
     // of the state, 50 registers of it at head size 64.)
     if (N) {
+    if (!AHEAD) fetch(step, now);
     if (FULL) q_r.put(q_s);
     k_r.put(k_s);
     v_r.put(v_s);
@@ -697,7 +705,7 @@ __global__ __launch_bounds__(DP * 4, DERIV ? 2 : 3) void la_pass_bf16(PassArgs a
     __syncthreads();
     }
     bits = __ballot(ahead);
-    fetch(step + 1, bits);
+    if (AHEAD) fetch(step + 1, bits);
     ahead = look(step + 2);
 
     if (N) {
@@ -836,8 +844,9 @@ __global__ __launch_bounds__(DP * 4, DERIV ? 2 : 3) void la_pass_bf16(PassArgs a
           const Split8<3> weighted(w[0], w[1]);
 #pragma unroll
           for (int t = 0; t < NT; ++t) {
+            if (!AHEAD) __builtin_amdgcn_sched_barrier(0);  // in order: fewer registers
             if (DERIV && t % 2 == 0) asm volatile("" ::: "memory");
-            state[t] = weighted.after(Ch::columns(k_s, state_row(t, 0, 0), 8, s, lo, g), state[t]);
+            state[t] = weighted.after(Ch::columns(k_s, state_row<FULL>(t, 0, 0), FULL ? 8 : 4, s, lo, g), state[t]);
           }
         };
         add(S);
@@ -875,7 +884,7 @@ __global__ __launch_bounds__(DP * 4, DERIV ? 2 : 3) void la_pass_bf16(PassArgs a
     asm volatile("" : "+v"(g_t)::"memory");
 #pragma unroll
     for (int r = 0; r < 4; ++r) {
-      const int c = state_row(t, g_t, r);
+      const int c = state_row<FULL>(t, g_t, r);
       if (c < a.Dc && e < a.De) {
         const int64_t at = c * a.st_c + e * a.st_e;
         if (dst) dst[at] = S[t][r];
@@ -1079,7 +1088,7 @@ int chunk_of(torch::ScalarType dt) { return dt == torch::kBFloat16 ? 64 : 32; }
 // slower float32 pass: 33 x 3 heads of 333, 50 us in two segments of 192, 35 in
 // six of 64), so that the state-only pass and the scan stay small beside the
 // work they split.  2 x 8 heads of 16384 at head size 128, by segments: 16, 146
-// us; 32, 165; 64, 189; 4, 473.
+// us; 32, 165; 64, 189; 4, 473 (of an earlier step).
 Split split_of(int64_t BH, int64_t L, int64_t D, int C) {
   const int64_t chunks = (L + C - 1) / C, want = D > 64 ? 256 : 512;
   int64_t G = BH ? std::min<int64_t>((want + BH - 1) / BH, chunks / (C == 64 ? 4 : 2)) : 1;
@@ -1096,17 +1105,28 @@ void launch_pass(torch::ScalarType dt, const PassArgs& a, hipStream_t stream) {
   const bool edge = a.Dc % 8 || a.De % 8;
 #define LA_LAUNCH(DP, ...)                                                                     \
   hipLaunchKernelGGL((__VA_ARGS__), dim3((unsigned)blocks), dim3(DP * 4), 0, stream, a)
-#define LA_PASS(DP)                                                                            \
+#define LA_BF16(DP, AHEAD)                                                                     \
   do {                                                                                         \
-    if (dt == torch::kBFloat16 && edge) LA_LAUNCH(DP, la_pass_bf16<DP, REV, STATE_ONLY, DERIV, true>); \
-    else if (dt == torch::kBFloat16) LA_LAUNCH(DP, la_pass_bf16<DP, REV, STATE_ONLY, DERIV, false>);   \
-    else if (dt == torch::kHalf) LA_LAUNCH(DP, la_pass_f32<__half, DP, REV, STATE_ONLY, DERIV>);       \
+    if (edge) LA_LAUNCH(DP, la_pass_bf16<DP, REV, STATE_ONLY, DERIV, true, AHEAD>);            \
+    else LA_LAUNCH(DP, la_pass_bf16<DP, REV, STATE_ONLY, DERIV, false, AHEAD>);                \
+  } while (0)
+#define LA_F32(DP)                                                                             \
+  do {                                                                                         \
+    if (dt == torch::kHalf) LA_LAUNCH(DP, la_pass_f32<__half, DP, REV, STATE_ONLY, DERIV>);    \
     else LA_LAUNCH(DP, la_pass_f32<float, DP, REV, STATE_ONLY, DERIV>);                        \
   } while (0)
-  if (dp == 32) LA_PASS(32);
-  else if (dp == 64) LA_PASS(64);
-  else LA_PASS(128);
-#undef LA_PASS
+  if (dt == torch::kBFloat16) {
+    if (dp == 32) LA_BF16(32, true);
+    else if (dp == 64) LA_BF16(64, true);
+    else if (STATE_ONLY || DERIV || edge || blocks <= 256) LA_BF16(128, true);
+    else if constexpr (!STATE_ONLY && !DERIV) LA_LAUNCH(128, la_pass_bf16<128, REV, false, false, false, false>);
+  } else {
+    if (dp == 32) LA_F32(32);
+    else if (dp == 64) LA_F32(64);
+    else LA_F32(128);
+  }
+#undef LA_BF16
+#undef LA_F32
 #undef LA_LAUNCH
   HIP_CHECK(hipGetLastError());
 }

@@ -382,6 +382,12 @@ class TestKernels:
         q, k, v, ld, s0, do, ds = inputs(2, 1, 1500, D, D, dtype, "cuda", carry=True)
         check_all(q, k, v, ld, masks(mask, 2, 1500, "cuda"), s0, None, do, ds, dtype)
 
+    @pytest.mark.parametrize("Dk,Dv", [(128, 128), (100, 120), (64, 64), (32, 32), (90, 64)])
+    def test_many_heads(self, Dk, Dv):
+        # more workgroups than CUs, whole and odd head sizes
+        q, k, v, ld, _, do, _ = inputs(65, 5, 130, Dk, Dv, torch.bfloat16, "cuda")
+        check_all(q, k, v, ld, masks("left", 65, 130, "cuda"), None, None, do, None, torch.bfloat16)
+
     @pytest.mark.parametrize("dtype", DTYPES, ids=str)
     def test_strides(self, dtype):
         # one projection's output, heads side by side; odd rows; a transposed last axis
