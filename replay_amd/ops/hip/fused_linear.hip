@@ -502,13 +502,14 @@ __global__ __launch_bounds__(WM * WN * 64) void gemm_tile(Gemm p) {
   finish(std::integral_constant<int, ACT_NONE>{});
 }
 
-// out[i] = sum of the parts' element i, in a fixed order: X lanes by 4 elements
-// across, 256 / X groups down the parts, whose sums meet in LDS.  The elements
-// from size on lie apart, as another array of the same number of parts.
-template <typename T, int X>
+// out[i] = sum of the parts' element i, in a fixed order: 16 lanes by 4 elements
+// across, 16 groups down the parts, whose sums meet in LDS (256 parts of 64 x 64,
+// 4 MB: 5 us).  The elements from size on lie apart, as another array of the same
+// number of parts.
+template <typename T>
 __global__ __launch_bounds__(256) void join_parts(const float* part, T* out, int64_t size, const float* part2,
                                                   T* out2, int64_t size2, int64_t blocks, int parts) {
-  constexpr int Y = 256 / X;
+  constexpr int X = 16, Y = 16;
   __shared__ __attribute__((aligned(16))) f32x4 group[Y][X];
   const int x = threadIdx.x % X, y = threadIdx.x / X;
   int64_t block = blockIdx.x;
@@ -680,21 +681,13 @@ template <typename T>
 void join(const torch::Tensor& part, torch::Tensor& out, const torch::Tensor& part2, torch::Tensor out2,
           int parts, hipStream_t stream) {
   const int64_t size = out.numel(), size2 = out2.defined() ? out2.numel() : 0;
-  // many parts of few elements: more groups a workgroup, and more workgroups
-  // (1024 parts of 64 x 64: 13 us with 16 lanes across, 5 with 4)
-  const int X = parts >= 128 ? 4 : 16;
-  const int64_t blocks = (size + 4 * X - 1) / (4 * X), all = blocks + (size2 + 4 * X - 1) / (4 * X);
+  const int64_t blocks = (size + 63) / 64, all = blocks + (size2 + 63) / 64;
   if (all == 0) return;
   TORCH_CHECK(all < (int64_t(1) << 31), "fused_linear: weight too large");
   const float* p2 = size2 ? part2.data_ptr<float>() : nullptr;
   T* o2 = size2 ? reinterpret_cast<T*>(out2.data_ptr()) : nullptr;
-#define FL_JOIN(X)                                                                         \
-  hipLaunchKernelGGL((join_parts<T, X>), dim3((unsigned)all), dim3(256), 0, stream,        \
-                     part.data_ptr<float>(), reinterpret_cast<T*>(out.data_ptr()), size,   \
-                     p2, o2, size2, blocks, parts)
-  if (X == 4) FL_JOIN(4);
-  else FL_JOIN(16);
-#undef FL_JOIN
+  hipLaunchKernelGGL((join_parts<T>), dim3((unsigned)all), dim3(256), 0, stream, part.data_ptr<float>(),
+                     reinterpret_cast<T*>(out.data_ptr()), size, p2, o2, size2, blocks, parts);
   HIP_CHECK(hipGetLastError());
 }
 

@@ -125,7 +125,7 @@ struct Rows32 {
 
 // One segment of one (batch, head) on the float32 matrix instructions: 16
 // positions a chunk (the pair products grow with it, and these instructions
-// have a sixteenth of the 16-bit ones' rate), 32 a load.  DE/16 waves; each
+// have a sixteenth of the 16-bit ones' rate), 32 a load.  DP/16 waves; each
 // owns 16 value columns and the whole contraction axis of the state, in the
 // accumulator layout (column = lane & 15, row = 4 (lane >> 4) + r), which is
 // also the layout of an operand whose contraction index is visited in that
@@ -262,18 +262,18 @@ __global__ __launch_bounds__(DP * 4, 2) void la_pass_f32(PassArgs a) {
     // round the loop for both cases: a second one, with a continue, kept copies
     // of the state.)
     if (now) {
-    if (FULL) q_r.put(q_s);
-    k_r.put(k_s);
-    v_r.put(v_s);
-    if (X) x_r.put(x_s);
-    if (threadIdx.x < ROWS) {
-      const unsigned own = (now >> (lane & 16)) & 0xffffu;
-      const int n = __popc(own & ((2u << (lane & 15)) - 1)), N = __popc(own);
-      n_s[lane] = (float)n;
-      inter_s[lane] = a.c_inter * lam[REV ? N - n : n];
-      update_s[lane] = a.c_update * lam[REV ? n : N - n];
-    }
-    __syncthreads();
+      if (FULL) q_r.put(q_s);
+      k_r.put(k_s);
+      v_r.put(v_s);
+      if (X) x_r.put(x_s);
+      if (threadIdx.x < ROWS) {
+        const unsigned own = (now >> (lane & 16)) & 0xffffu;
+        const int n = __popc(own & ((2u << (lane & 15)) - 1)), N = __popc(own);
+        n_s[lane] = (float)n;
+        inter_s[lane] = a.c_inter * lam[REV ? N - n : n];
+        update_s[lane] = a.c_update * lam[REV ? n : N - n];
+      }
+      __syncthreads();
     }
     bits = (unsigned)__ballot(ahead);
     fetch(step + 1, bits);
@@ -339,25 +339,25 @@ __global__ __launch_bounds__(DP * 4, 2) void la_pass_f32(PassArgs a) {
         const bool update = want_end || step + 1 < last || half == 0;
         started = true;
         if (update) {
-        const float lN = lam[N];
-#pragma unroll
-        for (int t = 0; t < NT; ++t) {
-          if (DERIV) Sd[t] = lN * (Sd[t] + (float)N * S[t]);
-          S[t] = lN * S[t];
-        }
-        const f32x4 w = *reinterpret_cast<const f32x4*>(update_s + r0 + 4 * g);
-        const f32x4 left = REV ? n_j : (float)N - n_j;
-#pragma unroll
-        for (int r = 0; r < 4; ++r) {
-          if (DERIV) asm volatile("" ::: "memory");
-          const float weighted = vr[r] * w[r];
+          const float lN = lam[N];
 #pragma unroll
           for (int t = 0; t < NT; ++t) {
-            const float kv = k_c[(4 * g + r) * LD + 16 * t + lo];
-            S[t] = mfma4(kv, weighted, S[t]);
-            if (DERIV) Sd[t] = mfma4(kv, weighted * left[r], Sd[t]);
+            if (DERIV) Sd[t] = lN * (Sd[t] + (float)N * S[t]);
+            S[t] = lN * S[t];
           }
-        }
+          const f32x4 w = *reinterpret_cast<const f32x4*>(update_s + r0 + 4 * g);
+          const f32x4 left = REV ? n_j : (float)N - n_j;
+#pragma unroll
+          for (int r = 0; r < 4; ++r) {
+            if (DERIV) asm volatile("" ::: "memory");
+            const float weighted = vr[r] * w[r];
+#pragma unroll
+            for (int t = 0; t < NT; ++t) {
+              const float kv = k_c[(4 * g + r) * LD + 16 * t + lo];
+              S[t] = mfma4(kv, weighted, S[t]);
+              if (DERIV) Sd[t] = mfma4(kv, weighted * left[r], Sd[t]);
+            }
+          }
         }
       }
     }
@@ -691,178 +691,179 @@ __global__ __launch_bounds__(DP * 4, DERIV ? 2 : AHEAD ? 3 : 4) void la_pass_bf1
     // round the loop for both cases: a second one, with a continue, kept copies
     // of the state, 50 registers of it at head size 64.)
     if (N) {
-    if (!AHEAD) fetch(step, now);
-    if (FULL) q_r.put(q_s);
-    k_r.put(k_s);
-    v_r.put(v_s);
-    if (X) x_r.put(x_s);
-    if (wave == 0) {
-      const int n = __popcll(now & ((2ull << lane) - 1));
-      n_s[lane] = (float)n;
-      inter_s[lane] = a.c_inter * lam[REV ? N - n : n];
-      update_s[lane] = a.c_update * lam[REV ? n : N - n];
-    }
-    __syncthreads();
+      if (!AHEAD) fetch(step, now);
+      if (FULL) q_r.put(q_s);
+      k_r.put(k_s);
+      v_r.put(v_s);
+      if (X) x_r.put(x_s);
+      if (wave == 0) {
+        const int n = __popcll(now & ((2ull << lane) - 1));
+        n_s[lane] = (float)n;
+        inter_s[lane] = a.c_inter * lam[REV ? N - n : n];
+        update_s[lane] = a.c_update * lam[REV ? n : N - n];
+      }
+      __syncthreads();
     }
     bits = __ballot(ahead);
     if (AHEAD) fetch(step + 1, bits);
     ahead = look(step + 2);
 
     if (N) {
-    const float all = (float)N;
-    if (FULL) {
-      // valid positions in one run: n_i - n_j = i - j wherever a pair counts
-      const uint64_t run = now >> __builtin_ctzll(now);
-      const bool whole = (run & (run + 1)) == 0;
-#pragma unroll 1
-      for (int unit = wave; unit < 6; unit += WAVES) {
-        const int it = unit_it(unit), s = unit_s(unit), i = 16 * it + lo;
-        const float n_i = n_s[i];
-        bf16x8 qf[NS];
-#pragma unroll
-        for (int c = 0; c < NS; ++c) qf[c] = Ch::rows(q_s, 16 * it, c, lo, g);
-        f32x4 p[2];
-#pragma unroll
-        for (int u = 0; u < 2; ++u) {
-          const int jt = 2 * s + u, apart = REV ? jt - it : it - jt;
-          p[u] = f32x4{0.f, 0.f, 0.f, 0.f};
-          if (apart < 0) continue;
-          f32x4 acc = {0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-          for (int c = 0; c < NS; ++c) acc = mfma32(Ch::rows(k_s, 16 * jt, c, lo, g), qf[c], acc);
-          f32x4 gaps;
-          if (DERIV || !TABLE || !whole) {
-            const f32x4 n_j = *reinterpret_cast<const f32x4*>(n_s + 16 * jt + 4 * g);
-            gaps = REV ? n_j - n_i : n_i - n_j;
-          }
-          if (TABLE && whole) {
-            p[u] = acc * full_s[apart][lane];
-          } else {
-            f32x4 w;
-#pragma unroll
-            for (int r = 0; r < 4; ++r) w[r] = lam[max((int)gaps[r], 0)];
-#pragma unroll
-            for (int r = 0; r < 4; ++r) {
-              const bool seen = apart > 0 || (REV ? 4 * g + r >= lo : 4 * g + r <= lo);
-              p[u][r] = seen ? acc[r] * (a.c_pair * w[r]) : 0.f;
-            }
-          }
-          if (DERIV) {  // sum of gap weight (q_i.k_j) (x_i.v_j)
-            asm volatile("" ::: "memory");
-            f32x4 other = {0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-            for (int c = 0; c < NS; ++c)
-              other = mfma32(Ch::rows(v_s, 16 * jt, c, lo, g), Ch::rows(x_s, 16 * it, c, lo, g), other);
-#pragma unroll
-            for (int r = 0; r < 4; ++r) d_decay += p[u][r] * gaps[r] * other[r];
-          }
-        }
-        p_s[unit][lane] = __builtin_bit_cast(uint4, pack8(p[0], p[1]));
-      }
-    }
-
-    bf16x8 vf[2];
-    f32x4 o[FULL ? 4 : 1];
-    if (busy) {
-#pragma unroll
-      for (int s = 0; s < 2; ++s) vf[s] = Ch::columns(v_s, e0, 4, s, lo, g);
-
+      const float all = (float)N;
       if (FULL) {
-        // the start state's part, a block of the contraction at a time: so the
-        // split state needs registers for one block only
+        // valid positions in one run: n_i - n_j = i - j wherever a pair counts
+        const uint64_t run = now >> __builtin_ctzll(now);
+        const bool whole = (run & (run + 1)) == 0;
+#pragma unroll 1
+        for (int unit = wave; unit < 6; unit += WAVES) {
+          const int it = unit_it(unit), s = unit_s(unit), i = 16 * it + lo;
+          const float n_i = n_s[i];
+          bf16x8 qf[NS];
 #pragma unroll
-        for (int it = 0; it < 4; ++it) o[it] = f32x4{0.f, 0.f, 0.f, 0.f};
-        if (started) {
-          f32x4 od[DERIV ? 4 : 1];
-          if (DERIV) {
+          for (int c = 0; c < NS; ++c) qf[c] = Ch::rows(q_s, 16 * it, c, lo, g);
+          f32x4 p[2];
 #pragma unroll
-            for (int it = 0; it < 4; ++it) od[it] = f32x4{0.f, 0.f, 0.f, 0.f};
-          }
+          for (int u = 0; u < 2; ++u) {
+            const int jt = 2 * s + u, apart = REV ? jt - it : it - jt;
+            p[u] = f32x4{0.f, 0.f, 0.f, 0.f};
+            if (apart < 0) continue;
+            f32x4 acc = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-          for (int s = 0; s < NS; ++s) {
-            asm volatile("" ::: "memory");
-            const Split8<DERIV ? 3 : 2> state(S[2 * s], S[2 * s + 1]);
-            const Split8<3> state_d(Sd[DERIV ? 2 * s : 0], Sd[DERIV ? 2 * s + 1 : 0]);
+            for (int c = 0; c < NS; ++c) acc = mfma32(Ch::rows(k_s, 16 * jt, c, lo, g), qf[c], acc);
+            f32x4 gaps;
+            if (DERIV || !TABLE || !whole) {
+              const f32x4 n_j = *reinterpret_cast<const f32x4*>(n_s + 16 * jt + 4 * g);
+              gaps = REV ? n_j - n_i : n_i - n_j;
+            }
+            if (TABLE && whole) {
+              p[u] = acc * full_s[apart][lane];
+            } else {
+              f32x4 w;
 #pragma unroll
-            for (int it = 0; it < 4; ++it) {
-              if (DERIV) asm volatile("" ::: "memory");
-              const bf16x8 qf = Ch::rows(q_s, 16 * it, s, lo, g);
-              o[it] = state.times(qf, o[it]);
-              if (DERIV) od[it] = state_d.times(qf, od[it]);
+              for (int r = 0; r < 4; ++r) w[r] = lam[max((int)gaps[r], 0)];
+#pragma unroll
+              for (int r = 0; r < 4; ++r) {
+                const bool seen = apart > 0 || (REV ? 4 * g + r >= lo : 4 * g + r <= lo);
+                p[u][r] = seen ? acc[r] * (a.c_pair * w[r]) : 0.f;
+              }
+            }
+            if (DERIV) {  // sum of gap weight (q_i.k_j) (x_i.v_j)
+              asm volatile("" ::: "memory");
+              f32x4 other = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+              for (int c = 0; c < NS; ++c)
+                other = mfma32(Ch::rows(v_s, 16 * jt, c, lo, g), Ch::rows(x_s, 16 * it, c, lo, g), other);
+#pragma unroll
+              for (int r = 0; r < 4; ++r) d_decay += p[u][r] * gaps[r] * other[r];
             }
           }
-#pragma unroll
-          for (int it = 0; it < 4; ++it) {
-            const int i = 16 * it + lo;
-            const float w_i = inter_s[i];
-            if (DERIV) {  // of the decay's gradient, x . (S' + n S) q w
-              od[it] = w_i * (od[it] + n_s[i] * o[it]);
-              const f32x4 xv = widen(*reinterpret_cast<const bf16x4*>(x_s + i * LD + (e0 + 4 * g) * 2));
-#pragma unroll
-              for (int r = 0; r < 4; ++r) d_decay += xv[r] * od[it][r];
-            }
-            o[it] = w_i * o[it];
-          }
+          p_s[unit][lane] = __builtin_bit_cast(uint4, pack8(p[0], p[1]));
         }
       }
-    }
 
-    if (FULL) {
-      __syncthreads();  // the pair weights are there, and v is read
+      bf16x8 vf[2];
+      f32x4 o[FULL ? 4 : 1];
       if (busy) {
 #pragma unroll
-        for (int u = 0; u < 6; ++u) {
-          const int it = unit_it(u), s = unit_s(u);
-          o[it] = mfma32(vf[s], __builtin_bit_cast(bf16x8, p_s[u][lane]), o[it]);
+        for (int s = 0; s < 2; ++s) vf[s] = Ch::columns(v_s, e0, 4, s, lo, g);
+
+        if (FULL) {
+          // the start state's part, a block of the contraction at a time: so the
+          // split state needs registers for one block only
+#pragma unroll
+          for (int it = 0; it < 4; ++it) o[it] = f32x4{0.f, 0.f, 0.f, 0.f};
+          if (started) {
+            f32x4 od[DERIV ? 4 : 1];
+            if (DERIV) {
+#pragma unroll
+              for (int it = 0; it < 4; ++it) od[it] = f32x4{0.f, 0.f, 0.f, 0.f};
+            }
+#pragma unroll
+            for (int s = 0; s < NS; ++s) {
+              asm volatile("" ::: "memory");
+              const Split8<DERIV ? 3 : 2> state(S[2 * s], S[2 * s + 1]);
+              const Split8<3> state_d(Sd[DERIV ? 2 * s : 0], Sd[DERIV ? 2 * s + 1 : 0]);
+#pragma unroll
+              for (int it = 0; it < 4; ++it) {
+                if (DERIV) asm volatile("" ::: "memory");
+                const bf16x8 qf = Ch::rows(q_s, 16 * it, s, lo, g);
+                o[it] = state.times(qf, o[it]);
+                if (DERIV) od[it] = state_d.times(qf, od[it]);
+              }
+            }
+#pragma unroll
+            for (int it = 0; it < 4; ++it) {
+              const int i = 16 * it + lo;
+              const float w_i = inter_s[i];
+              if (DERIV) {  // of the decay's gradient, x . (S' + n S) q w
+                od[it] = w_i * (od[it] + n_s[i] * o[it]);
+                const f32x4 xv = widen(*reinterpret_cast<const bf16x4*>(x_s + i * LD + (e0 + 4 * g) * 2));
+#pragma unroll
+                for (int r = 0; r < 4; ++r) d_decay += xv[r] * od[it][r];
+              }
+              o[it] = w_i * o[it];
+            }
+          }
         }
-#pragma unroll
-        for (int it = 0; it < 4; ++it)
-          *reinterpret_cast<bf16x4*>(v_s + (16 * it + lo) * LD + (e0 + 4 * g) * 2) =
-              __builtin_convertvector(o[it], bf16x4);
       }
-    }
-    if (busy) {
-      const bool update = want_end || step + 1 < last;
-      started = true;
-      if (update) {
-      const float lN = lam[N];
+
+      if (FULL) {
+        __syncthreads();  // the pair weights are there, and v is read
+        if (busy) {
 #pragma unroll
-      for (int t = 0; t < NT; ++t) {
-        if (DERIV) Sd[t] = lN * (Sd[t] + all * S[t]);
-        S[t] = lN * S[t];
+          for (int u = 0; u < 6; ++u) {
+            const int it = unit_it(u), s = unit_s(u);
+            o[it] = mfma32(vf[s], __builtin_bit_cast(bf16x8, p_s[u][lane]), o[it]);
+          }
+#pragma unroll
+          for (int it = 0; it < 4; ++it)
+            *reinterpret_cast<bf16x4*>(v_s + (16 * it + lo) * LD + (e0 + 4 * g) * 2) =
+                __builtin_convertvector(o[it], bf16x4);
+        }
       }
-#pragma unroll
-      for (int s = 0; s < 2; ++s) {
-        asm volatile("" ::: "memory");
-        f32x4 w[2];
-        const uint4 raw = __builtin_bit_cast(uint4, vf[s]);
-#pragma unroll
-        for (int i = 0; i < 2; ++i)
-          w[i] = widen(__builtin_bit_cast(bf16x4, i ? uint2{raw.z, raw.w} : uint2{raw.x, raw.y})) *
-                 *reinterpret_cast<const f32x4*>(update_s + 32 * s + 16 * i + 4 * g);
-        auto add = [&](f32x4* state) {
-          const Split8<3> weighted(w[0], w[1]);
+      if (busy) {
+        const bool update = want_end || step + 1 < last;
+        started = true;
+        if (update) {
+          const float lN = lam[N];
 #pragma unroll
           for (int t = 0; t < NT; ++t) {
-            if (!AHEAD) __builtin_amdgcn_sched_barrier(0);  // in order: fewer registers
-            if (DERIV && t % 2 == 0) asm volatile("" ::: "memory");
-            state[t] = weighted.after(Ch::columns(k_s, state_row<FULL>(t, 0, 0), FULL ? 8 : 4, s, lo, g), state[t]);
+            if (DERIV) Sd[t] = lN * (Sd[t] + all * S[t]);
+            S[t] = lN * S[t];
           }
-        };
-        add(S);
-        if (DERIV) {
-          asm volatile("" ::: "memory");
 #pragma unroll
-          for (int i = 0; i < 2; ++i) {
-            const f32x4 n_j = *reinterpret_cast<const f32x4*>(n_s + 32 * s + 16 * i + 4 * g);
-            w[i] = w[i] * (REV ? n_j : all - n_j);
+          for (int s = 0; s < 2; ++s) {
+            asm volatile("" ::: "memory");
+            f32x4 w[2];
+            const uint4 raw = __builtin_bit_cast(uint4, vf[s]);
+#pragma unroll
+            for (int i = 0; i < 2; ++i)
+              w[i] = widen(__builtin_bit_cast(bf16x4, i ? uint2{raw.z, raw.w} : uint2{raw.x, raw.y})) *
+                     *reinterpret_cast<const f32x4*>(update_s + 32 * s + 16 * i + 4 * g);
+            auto add = [&](f32x4* state) {
+              const Split8<3> weighted(w[0], w[1]);
+#pragma unroll
+              for (int t = 0; t < NT; ++t) {
+                if (!AHEAD) __builtin_amdgcn_sched_barrier(0);  // in order: fewer registers
+                if (DERIV && t % 2 == 0) asm volatile("" ::: "memory");
+                const bf16x8 kf = Ch::columns(k_s, state_row<FULL>(t, 0, 0), FULL ? 8 : 4, s, lo, g);
+                state[t] = weighted.after(kf, state[t]);
+              }
+            };
+            add(S);
+            if (DERIV) {
+              asm volatile("" ::: "memory");
+#pragma unroll
+              for (int i = 0; i < 2; ++i) {
+                const f32x4 n_j = *reinterpret_cast<const f32x4*>(n_s + 32 * s + 16 * i + 4 * g);
+                w[i] = w[i] * (REV ? n_j : all - n_j);
+              }
+              add(Sd);
+            }
           }
-          add(Sd);
         }
       }
-      }
-    }
-    __syncthreads();  // the chunk is read and its outputs are in LDS
+      __syncthreads();  // the chunk is read and its outputs are in LDS
     }
     if (FULL) store(l0, N == 0);
   }
@@ -1085,10 +1086,11 @@ int chunk_of(torch::ScalarType dt) { return dt == torch::kBFloat16 ? 64 : 32; }
 // One workgroup for each (batch, head) where these alone fill the card (two a
 // CU; one, of 8 waves, at head sizes past 64); else the history is cut until
 // there are about that many, in segments of at least 256 positions (64 of the
-// slower float32 pass: 33 x 3 heads of 333, 50 us in two segments of 192, 35 in
-// six of 64), so that the state-only pass and the scan stay small beside the
-// work they split.  2 x 8 heads of 16384 at head size 128, by segments: 16, 146
-// us; 32, 165; 64, 189; 4, 473 (of an earlier step).
+// slower float32 pass), so that the state-only pass and the scan stay small
+// beside the work they split.  Forward, by segments: 2 x 8 heads of 16384 at
+// head size 128 in 4, 380 us, 8, 203, 16 (taken), 124, 32, 117, 64, 135; 8 x 8 of
+// 4096 at 64 in 4, 70, 8 (taken), 54, 16, 60; float32, 33 x 3 of 333 at 48 in 1,
+// 57, 2, 54, 6 (taken), 36, 11, 38.
 Split split_of(int64_t BH, int64_t L, int64_t D, int C) {
   const int64_t chunks = (L + C - 1) / C, want = D > 64 ? 256 : 512;
   int64_t G = BH ? std::min<int64_t>((want + BH - 1) / BH, chunks / (C == 64 ? 4 : 2)) : 1;
@@ -1119,7 +1121,8 @@ void launch_pass(torch::ScalarType dt, const PassArgs& a, hipStream_t stream) {
     if (dp == 32) LA_BF16(32, true);
     else if (dp == 64) LA_BF16(64, true);
     else if (STATE_ONLY || DERIV || edge || blocks <= 256) LA_BF16(128, true);
-    else if constexpr (!STATE_ONLY && !DERIV) LA_LAUNCH(128, la_pass_bf16<128, REV, false, false, false, false>);
+    else if constexpr (!STATE_ONLY && !DERIV)
+      LA_LAUNCH(128, la_pass_bf16<128, REV, false, false, false, false>);
   } else {
     if (dp == 32) LA_F32(32);
     else if (dp == 64) LA_F32(64);
