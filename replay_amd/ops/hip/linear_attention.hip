@@ -46,6 +46,16 @@ struct Rows {  // [B, H, L, D] with unit stride in D
   int64_t b, h, l;
 };
 
+struct ShortArgs {
+  Rows q, k, v, dout, dq, dk, dv;
+  const float* log_decay;  // [H]
+  const bool* mask;        // [B, L] or nullptr, true = valid
+  int64_t mask_b, mask_l;
+  float* decay_part;       // [B, H] or nullptr
+  float scale;
+  int H, L, Dk, Dv;
+};
+
 struct PassArgs {
   Rows q, k, v, x;       // x: the query whose product with dq' is the decay's gradient
   void* out;
@@ -497,10 +507,10 @@ __device__ __forceinline__ void store8(__hip_bfloat16* p, int n, uint4 v) {
 }
 
 // One operand's 64 positions on their way from memory to LDS: 16-byte pieces,
-// DP / 8 of 4 DP threads a row.
-template <int DP, bool EDGE, bool ROWS>
+// DP / 8 threads a row.
+template <int DP, bool EDGE, bool ROWS, int THREADS = DP * 4>
 struct Chunk {
-  static constexpr int C = 64, ACROSS = DP / 8, DOWN = DP * 4 / ACROSS, PIECES = C / DOWN;
+  static constexpr int C = 64, ACROSS = DP / 8, DOWN = THREADS / ACROSS, PIECES = C / DOWN;
   // rows 16 bytes apart from a power of two: the fragment reads of 16 rows
   // then start in banks 4 words apart.  Without such reads, 32 bytes: the
   // transposing reads of 8 rows then fill the banks.
@@ -906,6 +916,156 @@ __global__ __launch_bounds__(DP * 4, DERIV ? 2 : AHEAD ? 3 : 4) void la_pass_bf1
   }
 }
 
+// All gradients of a history of one chunk without a state on either side, each
+// tensor read once and nothing carried: with w_ij = scale l^{n_i-n_j}, j <= i,
+//   A_ij = w_ij q_i.k_j          B_ij = w_ij dO_i.v_j
+//   dq = B k       dk = B^T q       dv = A^T dO
+//   the decay's: sum (n_i - n_j) A_ij (dO_i.v_j)
+// Wave w has 16 positions: as queries for dq, as keys for dk and dv, so that
+// no pair weight is another wave's and the work is about even (w + 1 and 4 - w
+// tiles of pairs).  The products that a transposed operand needs are worked out
+// again, transposed.
+template <int DP, bool EDGE>
+__global__ __launch_bounds__(256, DP == 128 ? 2 : 4) void la_short_bwd(ShortArgs a) {
+  using Ch = Chunk<DP, EDGE, true, 256>;
+  constexpr int C = 64, NS = DP / 32, NT = DP / 16, LD = Ch::LD;
+  // dq, dk and dv take the places of q, k and v
+  __shared__ __attribute__((aligned(16))) char q_s[Ch::BYTES], k_s[Ch::BYTES], v_s[Ch::BYTES], g_s[Ch::BYTES];
+  __shared__ __attribute__((aligned(16))) float n_s[C];
+  __shared__ float lam[C];
+  __shared__ float red[4];
+
+  const int64_t bh = blockIdx.x;
+  const int b = bh / a.H, h = bh % a.H;
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int lo = lane & 15, g = lane >> 4;
+  const uint64_t bits = __ballot(lane < a.L && (!a.mask || a.mask[b * a.mask_b + lane * a.mask_l]));
+  {
+    Ch q_r(a.q, b, h, a.Dk), k_r(a.k, b, h, a.Dk), v_r(a.v, b, h, a.Dv), g_r(a.dout, b, h, a.Dv);
+    q_r.fetch(0, bits);
+    k_r.fetch(0, bits);
+    v_r.fetch(0, bits);
+    g_r.fetch(0, bits);
+    if (wave == 0) {
+      n_s[lane] = (float)__popcll(bits & ((2ull << lane) - 1));
+      lam[lane] = a.scale * (lane ? expf(a.log_decay[h] * lane) : 1.f);
+    }
+    q_r.put(q_s);
+    k_r.put(k_s);
+    v_r.put(v_s);
+    g_r.put(g_s);
+  }
+  __syncthreads();
+
+  const int tiles = (a.L + 15) / 16, own = 16 * wave;
+  bf16x4 dq[NT], dk[NT], dv[NT];
+  float d_decay = 0.f;
+  if (wave < tiles) {
+    const float n_own = n_s[own + lo];
+    {
+      f32x4 o[NT];
+#pragma unroll
+      for (int t = 0; t < NT; ++t) o[t] = f32x4{0.f, 0.f, 0.f, 0.f};
+      bf16x8 gf[NS];
+#pragma unroll
+      for (int c = 0; c < NS; ++c) gf[c] = Ch::rows(g_s, own, c, lo, g);
+#pragma unroll 1
+      for (int s = 0; 2 * s <= wave; ++s) {
+        f32x4 p[2];
+#pragma unroll
+        for (int u = 0; u < 2; ++u) {
+          const int j0 = 16 * (2 * s + u);
+          p[u] = f32x4{0.f, 0.f, 0.f, 0.f};
+          if (j0 > own) continue;
+          f32x4 acc = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+          for (int c = 0; c < NS; ++c) acc = mfma32(Ch::rows(v_s, j0, c, lo, g), gf[c], acc);
+          const f32x4 gaps = n_own - *reinterpret_cast<const f32x4*>(n_s + j0 + 4 * g);
+#pragma unroll
+          for (int r = 0; r < 4; ++r)
+            p[u][r] = j0 < own || 4 * g + r <= lo ? acc[r] * lam[max((int)gaps[r], 0)] : 0.f;
+        }
+        const bf16x8 pf = pack8(p[0], p[1]);
+#pragma unroll
+        for (int t = 0; t < NT; ++t) o[t] = mfma32(Ch::columns(k_s, 16 * t, 4, s, lo, g), pf, o[t]);
+      }
+#pragma unroll
+      for (int t = 0; t < NT; ++t) dq[t] = __builtin_convertvector(o[t], bf16x4);
+    }
+    f32x4 o[NT], o2[NT];
+#pragma unroll
+    for (int t = 0; t < NT; ++t) o[t] = o2[t] = f32x4{0.f, 0.f, 0.f, 0.f};
+    bf16x8 kf[NS], vf[NS];
+#pragma unroll
+    for (int c = 0; c < NS; ++c) {
+      kf[c] = Ch::rows(k_s, own, c, lo, g);
+      vf[c] = Ch::rows(v_s, own, c, lo, g);
+    }
+#pragma unroll 1
+    for (int s = wave / 2; 2 * s < tiles; ++s) {
+      f32x4 p[2], p2[2];
+#pragma unroll
+      for (int u = 0; u < 2; ++u) {
+        const int i0 = 16 * (2 * s + u);
+        p[u] = p2[u] = f32x4{0.f, 0.f, 0.f, 0.f};
+        if (i0 < own) continue;
+        f32x4 acc = {0.f, 0.f, 0.f, 0.f}, acc2 = acc;
+#pragma unroll
+        for (int c = 0; c < NS; ++c) {
+          acc = mfma32(Ch::rows(q_s, i0, c, lo, g), kf[c], acc);
+          acc2 = mfma32(Ch::rows(g_s, i0, c, lo, g), vf[c], acc2);
+        }
+        const f32x4 gaps = *reinterpret_cast<const f32x4*>(n_s + i0 + 4 * g) - n_own;
+#pragma unroll
+        for (int r = 0; r < 4; ++r) {
+          const float w = i0 > own || 4 * g + r >= lo ? lam[max((int)gaps[r], 0)] : 0.f;
+          p[u][r] = acc[r] * w;
+          p2[u][r] = acc2[r] * w;
+          d_decay += p[u][r] * gaps[r] * acc2[r];
+        }
+      }
+      const bf16x8 pf = pack8(p[0], p[1]), pf2 = pack8(p2[0], p2[1]);
+#pragma unroll
+      for (int t = 0; t < NT; ++t) {
+        o[t] = mfma32(Ch::columns(g_s, 16 * t, 4, s, lo, g), pf, o[t]);
+        o2[t] = mfma32(Ch::columns(q_s, 16 * t, 4, s, lo, g), pf2, o2[t]);
+      }
+    }
+#pragma unroll
+    for (int t = 0; t < NT; ++t) {
+      dv[t] = __builtin_convertvector(o[t], bf16x4);
+      dk[t] = __builtin_convertvector(o2[t], bf16x4);
+    }
+  }
+  d_decay = wave_reduce_sum(d_decay);
+  if (lane == 0) red[wave] = d_decay;
+  __syncthreads();  // q, k, v are read
+  if (wave < tiles) {
+#pragma unroll
+    for (int t = 0; t < NT; ++t) {
+      const int at = (own + lo) * LD + (16 * t + 4 * g) * 2;
+      *reinterpret_cast<bf16x4*>(q_s + at) = dq[t];
+      *reinterpret_cast<bf16x4*>(k_s + at) = dk[t];
+      *reinterpret_cast<bf16x4*>(v_s + at) = dv[t];
+    }
+  }
+  __syncthreads();
+  const int row = threadIdx.x / Ch::ACROSS, d = (threadIdx.x % Ch::ACROSS) * 8;
+  auto store = [&](const char* from, const Rows& dst, int D) {
+    __hip_bfloat16* out = reinterpret_cast<__hip_bfloat16*>(const_cast<void*>(dst.p)) + b * dst.b + h * dst.h + d;
+#pragma unroll
+    for (int i = 0; i < Ch::PIECES; ++i) {
+      const int l = row + i * Ch::DOWN;
+      if (l < a.L && d < D)
+        store8<EDGE>(out + l * dst.l, D - d, *reinterpret_cast<const uint4*>(from + l * LD + d * 2));
+    }
+  };
+  store(q_s, a.dq, a.Dk);
+  store(k_s, a.dk, a.Dk);
+  store(v_s, a.dv, a.Dv);
+  if (threadIdx.x == 0 && a.decay_part) a.decay_part[bh] = (red[0] + red[1]) + (red[2] + red[3]);
+}
+
 // Contributions of the segments -> start states, in place, one thread for
 // each element of a state.
 template <bool REV>
@@ -1293,6 +1453,43 @@ std::vector<torch::Tensor> linear_attention_bwd(
   auto ds0 = need_state ? torch::empty({B, H, Dk, Dv}, f32) : torch::empty({0}, f32);
   if (B * H == 0) {
     if (need_decay) ddecay.zero_();
+    return {dq, dk, dv, ddecay, ds0};
+  }
+  // One chunk and no state: three passes read 10 tensors and write 3, this reads
+  // 4 and writes 3 (SHORT).
+  if (dt == torch::kBFloat16 && L <= 64 && !state.has_value() && !dstate.has_value() && !need_state) {
+    TORCH_CHECK(B * H < (int64_t(1) << 31), "linear attention: too many (batch, head)s");
+    ShortArgs a = {rows_of(q), rows_of(k), rows_of(v), rows_of(dout), rows_of(dq), rows_of(dk), rows_of(dv)};
+    a.log_decay = log_decay.data_ptr<float>();
+    if (mask.has_value()) {
+      a.mask = mask->data_ptr<bool>();
+      a.mask_b = mask->stride(0);
+      a.mask_l = mask->stride(1);
+    }
+    auto part = torch::empty({need_decay ? B * H : 0}, f32);
+    a.decay_part = need_decay ? part.data_ptr<float>() : nullptr;
+    a.scale = (float)scale;
+    a.H = H;
+    a.L = L;
+    a.Dk = Dk;
+    a.Dv = Dv;
+    const int dp = padded(std::max(Dk, Dv));
+    const bool edge = Dk % 8 || Dv % 8;
+#define LA_SHORT(DP)                                                                          \
+  do {                                                                                        \
+    if (edge) hipLaunchKernelGGL((la_short_bwd<DP, true>), dim3((unsigned)(B * H)), dim3(256), 0, stream, a); \
+    else hipLaunchKernelGGL((la_short_bwd<DP, false>), dim3((unsigned)(B * H)), dim3(256), 0, stream, a);     \
+  } while (0)
+    if (dp == 32) LA_SHORT(32);
+    else if (dp == 64) LA_SHORT(64);
+    else LA_SHORT(128);
+#undef LA_SHORT
+    HIP_CHECK(hipGetLastError());
+    if (need_decay) {
+      hipLaunchKernelGGL(la_decay_sum, dim3((unsigned)H), dim3(1024), 0, stream, a.decay_part,
+                         ddecay.data_ptr<float>(), (int)B, (int)H, 1);
+      HIP_CHECK(hipGetLastError());
+    }
     return {dq, dk, dv, ddecay, ds0};
   }
   const Split s = split_of(B * H, L, std::max(Dk, Dv), chunk_of(q.scalar_type()));
