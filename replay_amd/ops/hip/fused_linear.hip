@@ -82,6 +82,7 @@ struct Gemm {
   int act;
   float* part;            // [parts, M, N] instead of y
   float* row_part;        // [parts, M] sums of A over the contraction, or nullptr
+  unsigned tiles;         // of one part
 };
 
 __device__ __attribute__((aligned(16))) const unsigned zero_chunk[4] = {0, 0, 0, 0};
@@ -276,7 +277,7 @@ __device__ __forceinline__ void finish_block(const Gemm& p, const float* block, 
     for (int i = 0; i < V; i += 4)
       *reinterpret_cast<f32x4*>(v + i) = *reinterpret_cast<const f32x4*>(block + row * (WN + 4) + col + i);
     if (p.part) {
-      store_row<float, V>(p.part + (int64_t)blockIdx.y * p.M * p.N + at, left, v);
+      store_row<float, V>(p.part + at, left, v);
       continue;
     }
 #pragma unroll
@@ -314,10 +315,13 @@ __global__ __launch_bounds__(WM * WN * 64) void gemm_tile(Gemm p) {
   __shared__ __attribute__((aligned(16))) char stage1[STAGES == 2 ? STAGE : 16];
 
   // Workgroups go round the 8 dies in turn: give each die one run of tiles,
-  // ordered in bands of 8 tile rows, so that its own L2 serves the operands.
-  const unsigned tiles = gridDim.x, id = blockIdx.x;
-  const unsigned die = id & 7, per = tiles >> 3, more = tiles & 7;
-  const unsigned t = die * per + min(die, more) + (id >> 3);
+  // ordered in bands of 8 tile rows, so that its own L2 serves the operands; of
+  // a contraction in parts, the tiles of one part after the other.
+  const unsigned all = gridDim.x, id = blockIdx.x;
+  const unsigned die = id & 7, per = all >> 3, more = all & 7;
+  const unsigned u = die * per + min(die, more) + (id >> 3);
+  const unsigned at_part = u / p.tiles, t = u - at_part * p.tiles;
+  p.part += (int64_t)at_part * p.M * p.N;
   const unsigned tn = (p.N + BN - 1) / BN, tm = (p.M + BM - 1) / BM;
   const unsigned band = t / (8 * tn), rows = min(8u, tm - band * 8), in = t - band * 8 * tn;
   const int m0 = (int)(band * 8 + in % rows) * BM, n0 = (int)(in / rows) * BN;
@@ -328,7 +332,7 @@ __global__ __launch_bounds__(WM * WN * 64) void gemm_tile(Gemm p) {
   const int wm = (wave / WN) * (BM / WM), wn = (wave % WN) * (BN / WN);
   const T* a_src = reinterpret_cast<const T*>(p.a);
   const T* b_src = reinterpret_cast<const T*>(p.b);
-  const int64_t k_begin = blockIdx.y * p.k_part, k_end = min(p.K, k_begin + p.k_part);
+  const int64_t k_begin = at_part * p.k_part, k_end = min(p.K, k_begin + p.k_part);
   const int iters = k_end > k_begin ? (int)((k_end - k_begin + BK - 1) / BK) : 0;
 
   // where this thread's chunks of the first stage lie
@@ -490,7 +494,7 @@ __global__ __launch_bounds__(WM * WN * 64) void gemm_tile(Gemm p) {
         *reinterpret_cast<f32x4*>(block + lo_out * (WNC + 4) + 16 * j + 4 * g_out) = acc[i][j];
       finish_block<T, WNC, decltype(act)::value>(p, block, lane_out, m, n0 + wn, bias);
       if constexpr (SUMS) {
-        if (want_sums && g_out == 0 && m + lo_out < p.M) p.row_part[(int64_t)blockIdx.y * p.M + m + lo_out] = sums[i][0];
+        if (want_sums && g_out == 0 && m + lo_out < p.M) p.row_part[(int64_t)at_part * p.M + m + lo_out] = sums[i][0];
       }
     }
   };
@@ -639,11 +643,12 @@ bool chunks_aligned(const void* p, int64_t ld, int64_t inner) {
 }
 
 template <typename T, bool A_KM, bool B_KM, int BM, int BN, int WM, int WN, bool DIRECT, int STAGES>
-void launch_tile(const Gemm& p, int parts, hipStream_t stream) {
+void launch_tile(Gemm p, int parts, hipStream_t stream) {
   const int64_t tiles = (int64_t)((p.M + BM - 1) / BM) * ((p.N + BN - 1) / BN);
-  TORCH_CHECK(tiles < (int64_t(1) << 31), "fused_linear: too many tiles");
+  TORCH_CHECK(tiles * parts < (int64_t(1) << 31), "fused_linear: too many tiles");
+  p.tiles = (unsigned)tiles;
   hipLaunchKernelGGL((gemm_tile<T, A_KM, B_KM, BM, BN, WM, WN, DIRECT, STAGES>),
-                     dim3((unsigned)tiles, parts), dim3(WM * WN * 64), 0, stream, p);
+                     dim3((unsigned)(tiles * parts)), dim3(WM * WN * 64), 0, stream, p);
   HIP_CHECK(hipGetLastError());
 }
 
@@ -785,8 +790,9 @@ void backward_t(const torch::Tensor& dy, const torch::Tensor& x, const torch::Te
     p.K = M;
     // The rows are cut into parts, of 256 rows at least, until there is a
     // workgroup a CU: more parts are more float partials to write and read back.
-    // us by workgroups 128, 256, 512, 1024: 1024 x 256 by 25601 rows 46, 37, 42,
-    // 56; 64 x 64 by 409600 (T64) 30, 21, 24, 27.  Where the tiles alone fill
+    // us by workgroups 128, 256, 512, 1024, before a part's tiles shared a die:
+    // 1024 x 256 by 25601 rows 46, 37 (now 35), 42, 56; 64 x 64 by 409600 (T64)
+    // 30, 21, 24, 27.  Where the tiles alone fill
     // half the card, two a CU (2048 x 2048 by 8192: 131, 118).  (T256's registers
     // are full already: 849 us against 647 for 4096 x 4096 by 16384.)  Through
     // registers, small tiles and many: 500 x 1000 by 20000, 154 with T128, 89.
