@@ -388,6 +388,26 @@ class TestKernels:
         q, k, v, ld, _, do, _ = inputs(65, 5, 130, Dk, Dv, torch.bfloat16, "cuda")
         check_all(q, k, v, ld, masks("left", 65, 130, "cuda"), None, None, do, None, torch.bfloat16)
 
+    @pytest.mark.parametrize("Dk,Dv", [(32, 32), (64, 64), (128, 128), (20, 52), (9, 128), (40, 33), (1, 1)])
+    @pytest.mark.parametrize("L", [1, 16, 17, 33, 50, 64])
+    def test_short_histories_without_a_state(self, L, Dk, Dv):
+        for mask in ("none", "left", "right", "holes"):
+            q, k, v, ld, _, do, _ = inputs(4, 3, L, Dk, Dv, torch.bfloat16, "cuda")
+            check_all(q, k, v, ld, masks(mask, 4, L, "cuda"), None, None, do, None, torch.bfloat16)
+
+    @pytest.mark.parametrize("L", [1, 40, 64])
+    def test_short_histories_with_extreme_decays_and_masked_values(self, L):
+        q, k, v, _, _, do, _ = inputs(3, 3, L, 32, 32, torch.bfloat16, "cuda")
+        ld = torch.tensor([-math.inf, -60.0, 0.0], device="cuda")
+        mask = masks("holes", 3, L, "cuda")
+        check_all(q, k, v, ld, mask, None, None, do, None, torch.bfloat16)
+        want = run_all(q, k, v, ld, mask, None, None, do, None)
+        for t, bad in ((q, math.nan), (k, math.inf), (v, torch.finfo(torch.bfloat16).min), (do, -math.inf)):
+            t.transpose(1, 2)[~mask] = bad
+        got = run_all(q, k, v, ld, mask, None, None, do, None)
+        for name in want:
+            assert torch.equal(got[name], want[name]), name
+
     @pytest.mark.parametrize("dtype", DTYPES, ids=str)
     def test_strides(self, dtype):
         # one projection's output, heads side by side; odd rows; a transposed last axis
