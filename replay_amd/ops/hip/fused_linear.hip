@@ -57,7 +57,7 @@ __device__ __forceinline__ float act_of(int act, float z) {
 }
 
 __device__ __forceinline__ float act_slope(int act, float z) {
-  if (act == ACT_RELU) return z > 0.f ? 1.f : 0.f;
+  if (act == ACT_RELU) return z <= 0.f ? 0.f : 1.f;  // a NaN lets the gradient pass, as it passes itself
   if (act == ACT_GELU) {
     float bell;
     const float cdf = normal_cdf(z, bell);

@@ -259,6 +259,15 @@ class TestKernels:
         y = fused_linear(x, torch.ones(1, 1, device="cuda"), activation=act)
         assert torch.isnan(y[0]).all() and torch.isinf(y[1]).all() and torch.isfinite(y[2]).all()
 
+    def test_gradient_at_nan_is_torchs(self):
+        x = torch.tensor([[math.nan], [-1.0], [0.0], [2.0]], device="cuda")
+        w = torch.ones(1, 1, device="cuda")
+        grads = []
+        for f in (lambda t: fused_linear(t, w, activation="relu"), lambda t: torch.relu(t @ w.t())):
+            leaf = x.clone().requires_grad_()
+            grads.append(torch.autograd.grad(f(leaf).sum(), leaf)[0])
+        assert torch.equal(*grads)
+
     def test_same_bits_again(self):
         x, w, b, r, dy = make(20000, 64, 64, torch.bfloat16)
         leaves = [t.requires_grad_() for t in (x, w, b)]
