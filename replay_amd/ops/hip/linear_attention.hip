@@ -76,6 +76,18 @@ struct PassArgs {
   float c_pair, c_inter, c_update;   // where the scale goes
 };
 
+// dk's and dv's passes run in one launch, by turns of 8 workgroups, so that the
+// two for the same rows are on one die at about the same time: both read q and
+// dO, and few heads fill the card better.  us, of the whole backward pass, in two
+// launches and in one: 2 x 8 heads of 16384 at 128, 365 and 343; 33 x 3 of 333
+// (float32, 48) 98 and 83; 64 x 8 of 500 (40 and 56) 124 and 113; 1024 x 2 of
+// 200 at 64, 184 and 179.
+template <int N>
+struct Passes {
+  PassArgs a[N];
+};
+constexpr int passes_of(bool rev, bool state_only, bool deriv) { return rev && !state_only && !deriv ? 2 : 1; }
+
 __device__ __forceinline__ f32x4 mfma4(float a, float b, f32x4 c) {
   return __builtin_amdgcn_mfma_f32_16x16x4f32(a, b, c, 0, 0, 0);
 }
@@ -142,7 +154,14 @@ struct Rows32 {
 // order: neither the state nor the pair weights leave the registers between
 // products.  (Launch bounds as in la_pass_bf16: none that need spills.)
 template <typename T, int DP, bool REV, bool STATE_ONLY, bool DERIV>
-__global__ __launch_bounds__(DP * 4, 2) void la_pass_f32(PassArgs a) {
+__global__ __launch_bounds__(DP * 4, 2) void la_pass_f32(Passes<passes_of(REV, STATE_ONLY, DERIV)> all_passes) {
+  constexpr bool PAIR = passes_of(REV, STATE_ONLY, DERIV) == 2;
+  unsigned id = blockIdx.x;
+  const PassArgs& a = all_passes.a[PAIR ? (id >> 3) & 1 : 0];
+  if (PAIR) {
+    id = (id >> 4) * 8 + (id & 7);
+    if (id >= (unsigned)(a.B * a.H * a.G)) return;  // the same for a whole workgroup
+  }
   using Ch = Rows32<T, DP>;
   constexpr int C = 16, ROWS = 32, LD = Ch::LD, NT = DP / 16, WAVES = DP / 16;
   constexpr bool FULL = !STATE_ONLY, X = DERIV && FULL;
@@ -157,8 +176,8 @@ __global__ __launch_bounds__(DP * 4, 2) void la_pass_f32(PassArgs a) {
   __shared__ float lam[C + 1];
   __shared__ float red[WAVES];
 
-  const int seg = blockIdx.x % a.G;
-  const int64_t bh = blockIdx.x / a.G;
+  const int seg = id % (unsigned)a.G;
+  const int64_t bh = id / (unsigned)a.G;
   const int b = bh / a.H, h = bh % a.H;
   // the wave's index is the same for its lanes, which the compiler cannot see:
   // what depends on it alone then needs no vector registers and no masks
@@ -574,7 +593,14 @@ __device__ __forceinline__ int state_row(int t, int g, int r) {
 // 64 x 8 heads of 512, 57 us against 80; 2 x 8 of 16384 in 256 workgroups, 147
 // against 122.
 template <int DP, bool REV, bool STATE_ONLY, bool DERIV, bool EDGE, bool AHEAD>
-__global__ __launch_bounds__(DP * 4, DERIV ? 2 : AHEAD ? 3 : 4) void la_pass_bf16(PassArgs a) {
+__global__ __launch_bounds__(DP * 4, DERIV ? 2 : AHEAD ? 3 : 4) void la_pass_bf16(Passes<passes_of(REV, STATE_ONLY, DERIV)> all_passes) {
+  constexpr bool PAIR = passes_of(REV, STATE_ONLY, DERIV) == 2;
+  unsigned id = blockIdx.x;
+  const PassArgs& a = all_passes.a[PAIR ? (id >> 3) & 1 : 0];
+  if (PAIR) {
+    id = (id >> 4) * 8 + (id & 7);
+    if (id >= (unsigned)(a.B * a.H * a.G)) return;  // the same for a whole workgroup
+  }
   using Ch = Chunk<DP, EDGE, !STATE_ONLY>;
   constexpr int C = 64, NS = DP / 32, NT = DP / 16, LD = Ch::LD, WAVES = DP / 16;
   constexpr bool FULL = !STATE_ONLY, X = DERIV && FULL;
@@ -593,8 +619,8 @@ __global__ __launch_bounds__(DP * 4, DERIV ? 2 : AHEAD ? 3 : 4) void la_pass_bf1
   __shared__ float lam[C + 1];
   __shared__ float red[WAVES];
 
-  const int seg = blockIdx.x % a.G;
-  const int64_t bh = blockIdx.x / a.G;
+  const int seg = id % (unsigned)a.G;
+  const int64_t bh = id / (unsigned)a.G;
   const int b = bh / a.H, h = bh % a.H;
   // the wave's index is the same for its lanes, which the compiler cannot see:
   // what depends on it alone then needs no vector registers and no masks
@@ -1260,13 +1286,15 @@ Split split_of(int64_t BH, int64_t L, int64_t D, int C) {
 }
 
 template <bool REV, bool STATE_ONLY, bool DERIV>
-void launch_pass(torch::ScalarType dt, const PassArgs& a, hipStream_t stream) {
-  const int64_t blocks = (int64_t)a.B * a.H * a.G;
+void launch_pass(torch::ScalarType dt, const Passes<passes_of(REV, STATE_ONLY, DERIV)>& p, hipStream_t stream) {
+  const PassArgs& a = p.a[0];
+  int64_t blocks = (int64_t)a.B * a.H * a.G;
+  if (passes_of(REV, STATE_ONLY, DERIV) == 2) blocks = (blocks + 7) / 8 * 16;
   TORCH_CHECK(blocks < (int64_t(1) << 31), "linear attention: too many (batch, head, segment)s");
   const int dp = padded(std::max(a.Dc, a.De));
   const bool edge = a.Dc % 8 || a.De % 8;
 #define LA_LAUNCH(DP, ...)                                                                     \
-  hipLaunchKernelGGL((__VA_ARGS__), dim3((unsigned)blocks), dim3(DP * 4), 0, stream, a)
+  hipLaunchKernelGGL((__VA_ARGS__), dim3((unsigned)blocks), dim3(DP * 4), 0, stream, p)
 #define LA_BF16(DP, AHEAD)                                                                     \
   do {                                                                                         \
     if (edge) LA_LAUNCH(DP, la_pass_bf16<DP, REV, STATE_ONLY, DERIV, true, AHEAD>);            \
@@ -1419,10 +1447,10 @@ std::vector<torch::Tensor> linear_attention_fwd(torch::Tensor q, torch::Tensor k
     count = torch::empty({B, H, a.G}, q.options().dtype(torch::kInt32));
     a.seg = seg.data_ptr<float>();
     a.seg_count = count.data_ptr<int>();
-    launch_pass<false, true, false>(q.scalar_type(), a, stream);
+    launch_pass<false, true, false>(q.scalar_type(), {{a}}, stream);
     launch_scan<false>(a, a.state_in, stream);
   }
-  launch_pass<false, false, false>(q.scalar_type(), a, stream);
+  launch_pass<false, false, false>(q.scalar_type(), {{a}}, stream);
   return {out, end, seg};
 }
 
@@ -1514,7 +1542,7 @@ std::vector<torch::Tensor> linear_attention_bwd(
     seg_r = torch::empty_like(seg);
     v_args.seg = seg_r.data_ptr<float>();
     v_args.seg_count = count.data_ptr<int>();
-    launch_pass<true, true, false>(dt, v_args, stream);
+    launch_pass<true, true, false>(dt, {{v_args}}, stream);
   }
 
   {  // dq, and the decay's gradient
@@ -1538,7 +1566,7 @@ std::vector<torch::Tensor> linear_attention_bwd(
         seg_d = torch::empty_like(seg);
         a.seg_d = seg_d.data_ptr<float>();
       }
-      launch_pass<false, false, true>(dt, a, stream);
+      launch_pass<false, false, true>(dt, {{a}}, stream);
       if (split) {
         hipLaunchKernelGGL(la_scan_decay, dim3((unsigned)(B * H), (unsigned)blocks), dim3(256), 0, stream,
                            a.seg_d, v_args.seg, v_args.seg_count, dstate_in, a.log_decay, a.decay_part,
@@ -1549,12 +1577,11 @@ std::vector<torch::Tensor> linear_attention_bwd(
                          part.data_ptr<float>(), ddecay.data_ptr<float>(), (int)B, (int)H, a.parts);
       HIP_CHECK(hipGetLastError());
     } else {
-      launch_pass<false, false, false>(dt, a, stream);
+      launch_pass<false, false, false>(dt, {{a}}, stream);
     }
   }
 
   if (split) launch_scan<true>(v_args, dstate_in, stream);
-  launch_pass<true, false, false>(dt, v_args, stream);
   PassArgs c = args_of(v, dout, q, log_decay, mask, true);
   set_out(c, dk);
   c.G = s.G;
@@ -1563,7 +1590,7 @@ std::vector<torch::Tensor> linear_attention_bwd(
   c.seg = v_args.seg;
   c.c_pair = c.c_update = (float)scale;
   c.c_inter = 1.f;
-  launch_pass<true, false, false>(dt, c, stream);
+  launch_pass<true, false, false>(dt, {{v_args, c}}, stream);
   return {dq, dk, dv, ddecay, ds0};
 }
 
