@@ -47,7 +47,8 @@ struct Rows {  // [B, H, L, D] with unit stride in D
 };
 
 struct ShortArgs {
-  Rows q, k, v, dout, dq, dk, dv;
+  Rows q, k, v, out;       // forward: out
+  Rows dout, dq, dk, dv;   // backward
   const float* log_decay;  // [H]
   const bool* mask;        // [B, L] or nullptr, true = valid
   int64_t mask_b, mask_l;
@@ -942,12 +943,102 @@ __global__ __launch_bounds__(DP * 4, DERIV ? 2 : AHEAD ? 3 : 4) void la_pass_bf1
   }
 }
 
-// All gradients of a history of one chunk without a state on either side, each
-// tensor read once and nothing carried: with w_ij = scale l^{n_i-n_j}, j <= i,
+// Histories of at most one chunk without a state on either side, where nothing is
+// carried: with w_ij = scale l^{n_i-n_j}, j <= i.  Wave w has 16 positions.
+//   out_i = sum_j w_ij (x_i.y_j) z_j for the positions of wave w
+template <int DP, class Ch>
+__device__ __forceinline__ void short_rows(const char* x_s, const char* y_s, const char* z_s, const float* n_s,
+                                           const float* lam, int wave, int lo, int g, bf16x4* out) {
+  constexpr int NS = DP / 32, NT = DP / 16;
+  const int own = 16 * wave;
+  const float n_own = n_s[own + lo];
+  f32x4 o[NT];
+#pragma unroll
+  for (int t = 0; t < NT; ++t) o[t] = f32x4{0.f, 0.f, 0.f, 0.f};
+  bf16x8 xf[NS];
+#pragma unroll
+  for (int c = 0; c < NS; ++c) xf[c] = Ch::rows(x_s, own, c, lo, g);
+#pragma unroll 1
+  for (int s = 0; 2 * s <= wave; ++s) {
+    f32x4 p[2];
+#pragma unroll
+    for (int u = 0; u < 2; ++u) {
+      const int j0 = 16 * (2 * s + u);
+      p[u] = f32x4{0.f, 0.f, 0.f, 0.f};
+      if (j0 > own) continue;
+      f32x4 acc = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+      for (int c = 0; c < NS; ++c) acc = mfma32(Ch::rows(y_s, j0, c, lo, g), xf[c], acc);
+      const f32x4 gaps = n_own - *reinterpret_cast<const f32x4*>(n_s + j0 + 4 * g);
+#pragma unroll
+      for (int r = 0; r < 4; ++r)
+        p[u][r] = j0 < own || 4 * g + r <= lo ? acc[r] * lam[max((int)gaps[r], 0)] : 0.f;
+    }
+    const bf16x8 pf = pack8(p[0], p[1]);
+#pragma unroll
+    for (int t = 0; t < NT; ++t) o[t] = mfma32(Ch::columns(z_s, 16 * t, 4, s, lo, g), pf, o[t]);
+  }
+#pragma unroll
+  for (int t = 0; t < NT; ++t) out[t] = __builtin_convertvector(o[t], bf16x4);
+}
+
+// rows [0, L) of an LDS tile to [B, H, L, D] memory, 16 bytes a thread
+template <bool EDGE, class Ch>
+__device__ __forceinline__ void short_store(const char* from, const Rows& dst, int b, int h, int L, int D) {
+  const int row = threadIdx.x / Ch::ACROSS, d = (threadIdx.x % Ch::ACROSS) * 8;
+  __hip_bfloat16* out = reinterpret_cast<__hip_bfloat16*>(const_cast<void*>(dst.p)) + b * dst.b + h * dst.h + d;
+#pragma unroll
+  for (int i = 0; i < Ch::PIECES; ++i) {
+    const int l = row + i * Ch::DOWN;
+    if (l < L && d < D)
+      store8<EDGE>(out + l * dst.l, D - d, *reinterpret_cast<const uint4*>(from + l * Ch::LD + d * 2));
+  }
+}
+
+// The forward pass of them, out = (w o q k^T) v.
+template <int DP, bool EDGE>
+__global__ __launch_bounds__(256, 4) void la_short_fwd(ShortArgs a) {
+  using Ch = Chunk<DP, EDGE, true, 256>;
+  constexpr int NT = DP / 16;
+  // the outputs take the place of q, whose rows a wave reads alone
+  __shared__ __attribute__((aligned(16))) char q_s[Ch::BYTES], k_s[Ch::BYTES], v_s[Ch::BYTES];
+  __shared__ __attribute__((aligned(16))) float n_s[Ch::C];
+  __shared__ float lam[Ch::C];
+  const int64_t bh = blockIdx.x;
+  const int b = bh / a.H, h = bh % a.H;
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int lo = lane & 15, g = lane >> 4;
+  const uint64_t bits = __ballot(lane < a.L && (!a.mask || a.mask[b * a.mask_b + lane * a.mask_l]));
+  {
+    Ch q_r(a.q, b, h, a.Dk), k_r(a.k, b, h, a.Dk), v_r(a.v, b, h, a.Dv);
+    q_r.fetch(0, bits);
+    k_r.fetch(0, bits);
+    v_r.fetch(0, bits);
+    if (wave == 0) {
+      n_s[lane] = (float)__popcll(bits & ((2ull << lane) - 1));
+      lam[lane] = a.scale * (lane ? expf(a.log_decay[h] * lane) : 1.f);
+    }
+    q_r.put(q_s);
+    k_r.put(k_s);
+    v_r.put(v_s);
+  }
+  __syncthreads();
+  if (16 * wave < a.L) {
+    bf16x4 o[NT];
+    short_rows<DP, Ch>(q_s, k_s, v_s, n_s, lam, wave, lo, g, o);
+#pragma unroll
+    for (int t = 0; t < NT; ++t)
+      *reinterpret_cast<bf16x4*>(q_s + (16 * wave + lo) * Ch::LD + (16 * t + 4 * g) * 2) = o[t];
+  }
+  __syncthreads();
+  short_store<EDGE, Ch>(q_s, a.out, b, h, a.L, a.Dv);
+}
+
+// All gradients of them, each tensor read once:
 //   A_ij = w_ij q_i.k_j          B_ij = w_ij dO_i.v_j
 //   dq = B k       dk = B^T q       dv = A^T dO
 //   the decay's: sum (n_i - n_j) A_ij (dO_i.v_j)
-// Wave w has 16 positions: as queries for dq, as keys for dk and dv, so that
+// A wave has its positions as queries for dq and as keys for dk and dv, so that
 // no pair weight is another wave's and the work is about even (w + 1 and 4 - w
 // tiles of pairs).  The products that a transposed operand needs are worked out
 // again, transposed.
@@ -988,36 +1079,7 @@ __global__ __launch_bounds__(256, DP == 128 ? 2 : 4) void la_short_bwd(ShortArgs
   float d_decay = 0.f;
   if (wave < tiles) {
     const float n_own = n_s[own + lo];
-    {
-      f32x4 o[NT];
-#pragma unroll
-      for (int t = 0; t < NT; ++t) o[t] = f32x4{0.f, 0.f, 0.f, 0.f};
-      bf16x8 gf[NS];
-#pragma unroll
-      for (int c = 0; c < NS; ++c) gf[c] = Ch::rows(g_s, own, c, lo, g);
-#pragma unroll 1
-      for (int s = 0; 2 * s <= wave; ++s) {
-        f32x4 p[2];
-#pragma unroll
-        for (int u = 0; u < 2; ++u) {
-          const int j0 = 16 * (2 * s + u);
-          p[u] = f32x4{0.f, 0.f, 0.f, 0.f};
-          if (j0 > own) continue;
-          f32x4 acc = {0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-          for (int c = 0; c < NS; ++c) acc = mfma32(Ch::rows(v_s, j0, c, lo, g), gf[c], acc);
-          const f32x4 gaps = n_own - *reinterpret_cast<const f32x4*>(n_s + j0 + 4 * g);
-#pragma unroll
-          for (int r = 0; r < 4; ++r)
-            p[u][r] = j0 < own || 4 * g + r <= lo ? acc[r] * lam[max((int)gaps[r], 0)] : 0.f;
-        }
-        const bf16x8 pf = pack8(p[0], p[1]);
-#pragma unroll
-        for (int t = 0; t < NT; ++t) o[t] = mfma32(Ch::columns(k_s, 16 * t, 4, s, lo, g), pf, o[t]);
-      }
-#pragma unroll
-      for (int t = 0; t < NT; ++t) dq[t] = __builtin_convertvector(o[t], bf16x4);
-    }
+    short_rows<DP, Ch>(g_s, v_s, k_s, n_s, lam, wave, lo, g, dq);
     f32x4 o[NT], o2[NT];
 #pragma unroll
     for (int t = 0; t < NT; ++t) o[t] = o2[t] = f32x4{0.f, 0.f, 0.f, 0.f};
@@ -1076,19 +1138,9 @@ __global__ __launch_bounds__(256, DP == 128 ? 2 : 4) void la_short_bwd(ShortArgs
     }
   }
   __syncthreads();
-  const int row = threadIdx.x / Ch::ACROSS, d = (threadIdx.x % Ch::ACROSS) * 8;
-  auto store = [&](const char* from, const Rows& dst, int D) {
-    __hip_bfloat16* out = reinterpret_cast<__hip_bfloat16*>(const_cast<void*>(dst.p)) + b * dst.b + h * dst.h + d;
-#pragma unroll
-    for (int i = 0; i < Ch::PIECES; ++i) {
-      const int l = row + i * Ch::DOWN;
-      if (l < a.L && d < D)
-        store8<EDGE>(out + l * dst.l, D - d, *reinterpret_cast<const uint4*>(from + l * LD + d * 2));
-    }
-  };
-  store(q_s, a.dq, a.Dk);
-  store(k_s, a.dk, a.Dk);
-  store(v_s, a.dv, a.Dv);
+  short_store<EDGE, Ch>(q_s, a.dq, b, h, a.L, a.Dk);
+  short_store<EDGE, Ch>(k_s, a.dk, b, h, a.L, a.Dk);
+  short_store<EDGE, Ch>(v_s, a.dv, b, h, a.L, a.Dv);
   if (threadIdx.x == 0 && a.decay_part) a.decay_part[bh] = (red[0] + red[1]) + (red[2] + red[3]);
 }
 
@@ -1409,6 +1461,49 @@ void set_out(PassArgs& a, const torch::Tensor& out) {
   a.out_l = out.stride(2);
 }
 
+// One chunk and no state: nothing to carry.  us, with the general passes and
+// without: 8192 x 2 heads of 50 at head size 32, forward 47 and 33, backward 183 (10
+// tensors read and 3 written in three passes; 4 and 3 here) and 80.
+bool is_short(const torch::Tensor& q, bool states) {
+  return q.scalar_type() == torch::kBFloat16 && q.size(2) <= 64 && !states;
+}
+
+ShortArgs short_args(const torch::Tensor& q, const torch::Tensor& k, const torch::Tensor& v,
+                     const torch::Tensor& log_decay, const c10::optional<torch::Tensor>& mask, double scale) {
+  TORCH_CHECK(q.size(0) * q.size(1) < (int64_t(1) << 31), "linear attention: too many (batch, head)s");
+  ShortArgs a = {};
+  a.q = rows_of(q);
+  a.k = rows_of(k);
+  a.v = rows_of(v);
+  a.log_decay = log_decay.data_ptr<float>();
+  if (mask.has_value()) {
+    a.mask = mask->data_ptr<bool>();
+    a.mask_b = mask->stride(0);
+    a.mask_l = mask->stride(1);
+  }
+  a.scale = (float)scale;
+  a.H = q.size(1);
+  a.L = q.size(2);
+  a.Dk = q.size(3);
+  a.Dv = v.size(3);
+  return a;
+}
+
+#define LA_SHORT_DP(KERNEL, DP)                                                                      \
+  do {                                                                                               \
+    const dim3 grid((unsigned)(B * H));                                                              \
+    if (Dk % 8 || Dv % 8) hipLaunchKernelGGL((KERNEL<DP, true>), grid, dim3(256), 0, stream, a);     \
+    else hipLaunchKernelGGL((KERNEL<DP, false>), grid, dim3(256), 0, stream, a);                     \
+  } while (0)
+#define LA_SHORT(KERNEL)                                   \
+  do {                                                     \
+    const int dp = padded(std::max(Dk, Dv));               \
+    if (dp == 32) LA_SHORT_DP(KERNEL, 32);                 \
+    else if (dp == 64) LA_SHORT_DP(KERNEL, 64);            \
+    else LA_SHORT_DP(KERNEL, 128);                         \
+    HIP_CHECK(hipGetLastError());                          \
+  } while (0)
+
 }  // namespace
 
 // -> {out, state or empty, start states of the segments or empty}
@@ -1431,6 +1526,12 @@ std::vector<torch::Tensor> linear_attention_fwd(torch::Tensor q, torch::Tensor k
   auto end = want_state ? torch::empty({B, H, Dk, Dv}, f32) : torch::empty({0}, f32);
   auto seg = torch::empty({0}, f32);
   if (B * H == 0) return {out, end, seg};
+  if (is_short(q, state.has_value() || want_state)) {
+    ShortArgs a = short_args(q, k, v, log_decay, mask, scale);
+    a.out = rows_of(out);
+    LA_SHORT(la_short_fwd);
+    return {out, end, seg};
+  }
 
   PassArgs a = args_of(q, k, v, log_decay, mask, false);
   set_out(a, out);
@@ -1483,36 +1584,15 @@ std::vector<torch::Tensor> linear_attention_bwd(
     if (need_decay) ddecay.zero_();
     return {dq, dk, dv, ddecay, ds0};
   }
-  // One chunk and no state: three passes read 10 tensors and write 3, this reads
-  // 4 and writes 3 (SHORT).
-  if (dt == torch::kBFloat16 && L <= 64 && !state.has_value() && !dstate.has_value() && !need_state) {
-    TORCH_CHECK(B * H < (int64_t(1) << 31), "linear attention: too many (batch, head)s");
-    ShortArgs a = {rows_of(q), rows_of(k), rows_of(v), rows_of(dout), rows_of(dq), rows_of(dk), rows_of(dv)};
-    a.log_decay = log_decay.data_ptr<float>();
-    if (mask.has_value()) {
-      a.mask = mask->data_ptr<bool>();
-      a.mask_b = mask->stride(0);
-      a.mask_l = mask->stride(1);
-    }
+  if (is_short(q, state.has_value() || dstate.has_value() || need_state)) {
+    ShortArgs a = short_args(q, k, v, log_decay, mask, scale);
+    a.dout = rows_of(dout);
+    a.dq = rows_of(dq);
+    a.dk = rows_of(dk);
+    a.dv = rows_of(dv);
     auto part = torch::empty({need_decay ? B * H : 0}, f32);
     a.decay_part = need_decay ? part.data_ptr<float>() : nullptr;
-    a.scale = (float)scale;
-    a.H = H;
-    a.L = L;
-    a.Dk = Dk;
-    a.Dv = Dv;
-    const int dp = padded(std::max(Dk, Dv));
-    const bool edge = Dk % 8 || Dv % 8;
-#define LA_SHORT(DP)                                                                          \
-  do {                                                                                        \
-    if (edge) hipLaunchKernelGGL((la_short_bwd<DP, true>), dim3((unsigned)(B * H)), dim3(256), 0, stream, a); \
-    else hipLaunchKernelGGL((la_short_bwd<DP, false>), dim3((unsigned)(B * H)), dim3(256), 0, stream, a);     \
-  } while (0)
-    if (dp == 32) LA_SHORT(32);
-    else if (dp == 64) LA_SHORT(64);
-    else LA_SHORT(128);
-#undef LA_SHORT
-    HIP_CHECK(hipGetLastError());
+    LA_SHORT(la_short_bwd);
     if (need_decay) {
       hipLaunchKernelGGL(la_decay_sum, dim3((unsigned)H), dim3(1024), 0, stream, a.decay_part,
                          ddecay.data_ptr<float>(), (int)B, (int)H, 1);

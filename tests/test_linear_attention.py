@@ -395,6 +395,48 @@ class TestKernels:
             q, k, v, ld, _, do, _ = inputs(4, 3, L, Dk, Dv, torch.bfloat16, "cuda")
             check_all(q, k, v, ld, masks(mask, 4, L, "cuda"), None, None, do, None, torch.bfloat16)
 
+    @pytest.mark.parametrize("Dk,Dv", [(32, 32), (64, 64), (128, 128), (20, 52), (9, 128), (40, 33), (1, 1)])
+    @pytest.mark.parametrize("L", [1, 16, 17, 33, 50, 64, 65])
+    def test_outputs_alone(self, L, Dk, Dv):
+        for mask in ("none", "left", "right", "holes"):
+            q, k, v, ld, _, do, _ = inputs(4, 3, L, Dk, Dv, torch.bfloat16, "cuda")
+            ld[0] = -math.inf
+            m = masks(mask, 4, L, "cuda")
+            exact = oracle(q, k, v, ld, m, None, 0.3)
+            tol = bounds(exact, oracle(q.abs(), k.abs(), v.abs(), ld, m, None, 0.3), torch.bfloat16, L, Dk, Dv)
+            if m is not None:
+                q, k, v = (torch.where(m[:, None, :, None], t, math.nan) for t in (q, k, v))
+            out = linear_attention(q, k, v, ld, padding_mask=m, scale=0.3)
+            assert_within(out, exact["out"], tol["out"], "out")
+            if m is not None:
+                assert not out.transpose(1, 2)[~m].any()
+            assert torch.equal(out, linear_attention(q, k, v, ld, padding_mask=m, scale=0.3, return_state=True)[0])
+
+    def test_short_histories_on_another_stream_and_captured(self):
+        q, k, v, ld, _, do, _ = inputs(5, 2, 50, 32, 32, torch.bfloat16, "cuda")
+        mask = masks("left", 5, 50, "cuda")
+        stream, graph = torch.cuda.Stream(), torch.cuda.CUDAGraph()
+
+        def step():
+            leaves = [t.detach().requires_grad_() for t in (q, k, v, ld)]
+            out = linear_attention(*leaves, padding_mask=mask)
+            return (out.detach(), *torch.autograd.grad(out, leaves, do))
+
+        torch.cuda.synchronize()
+        with torch.cuda.stream(stream):
+            step()
+        torch.cuda.synchronize()
+        with torch.cuda.graph(graph, stream=stream):
+            got = step()
+        for seed in range(3):
+            fresh = inputs(5, 2, 50, 32, 32, torch.bfloat16, "cuda", seed=seed)
+            for t, new in zip((q, k, v, do), (*fresh[:3], fresh[5])):
+                t.copy_(new)
+            graph.replay()
+            for a, b in zip(got, step()):
+                assert torch.equal(a, b)
+            torch.cuda.synchronize()
+
     @pytest.mark.parametrize("L", [1, 40, 64])
     def test_short_histories_with_extreme_decays_and_masked_values(self, L):
         q, k, v, _, _, do, _ = inputs(3, 3, L, 32, 32, torch.bfloat16, "cuda")
