@@ -1322,15 +1322,17 @@ struct Split {
 int chunk_of(torch::ScalarType dt) { return dt == torch::kBFloat16 ? 64 : 32; }
 
 // One workgroup for each (batch, head) where these alone fill the card (two a
-// CU; one, of 8 waves, at head sizes past 64); else the history is cut until
-// there are about that many, in segments of at least 256 positions (64 of the
-// slower float32 pass), so that the state-only pass and the scan stay small
-// beside the work they split.  Forward, by segments: 2 x 8 heads of 16384 at
-// head size 128 in 4, 380 us, 8, 203, 16 (taken), 124, 32, 117, 64, 135; 8 x 8 of
-// 4096 at 64 in 4, 70, 8 (taken), 54, 16, 60; float32, 33 x 3 of 333 at 48 in 1,
-// 57, 2, 54, 6 (taken), 36, 11, 38.
+// CU; one, of 8 waves, of bfloat16's at head sizes past 64); else the history is
+// cut until there are about that many, in segments of at least 256 positions (64
+// of the slower float32 pass), so that the state-only pass and the scan stay
+// small beside the work they split.  Forward / backward, by segments: 2 x 8 heads
+// of 16384 at head size 128 in 4, 380 us, 8, 203, 16 (taken), 124 / 360, 32, 117 /
+// 372, 64, 135 / 464; 8 x 8 of 4096 at 64 in 4, 70 / 166, 8 (taken), 53 / 145, 16,
+// 59 / 157; float32, 33 x 3 of 333 at 48 in 1, 57, 2, 54, 4 (taken), 37, 11, 38;
+// float16, 6 x 2 of 12878 at 88 in 22, 375 / 1038, 41 (taken), 216 / 655, 81,
+// 232 / 703.
 Split split_of(int64_t BH, int64_t L, int64_t D, int C) {
-  const int64_t chunks = (L + C - 1) / C, want = D > 64 ? 256 : 512;
+  const int64_t chunks = (L + C - 1) / C, want = D > 64 && C == 64 ? 256 : 512;
   int64_t G = BH ? std::min<int64_t>((want + BH - 1) / BH, chunks / (C == 64 ? 4 : 2)) : 1;
   G = std::max<int64_t>(G, 1);
   const int64_t per = std::max<int64_t>((chunks + G - 1) / G, 1);
