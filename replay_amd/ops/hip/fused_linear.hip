@@ -664,6 +664,12 @@ void launch_gemm(const Gemm& p, Tile tile, int parts, hipStream_t stream) {
     if constexpr (sizeof(T) == 2 && A_KM) {
       if (tile == T256) FL_TILE(256, 256, 2, 4, true, 2);
     }
+    // where dW has one workgroup a CU: in 8 waves, two a SIMD hide each other's
+    // transposing reads (1024 x 256 by 25601: 36 us in 4 waves, 31; all gradients of
+    // 8192 x 8192 by 8192, with db, whose sums weigh more in narrower waves: 2590, 2650)
+    if constexpr (sizeof(T) == 2 && !A_KM) {
+      if (tile == T128 && tile_count(T128, p.M, p.N) < 128) FL_TILE(128, 128, 2, 4, true, 2);
+    }
     if (tile == T256 || tile == T128) FL_TILE(128, 128, 2, 2, true, 2);
     if constexpr (A_KM) {
       if (tile == T128x64 && one) FL_TILE(128, 64, 4, 1, true, 1);
@@ -791,7 +797,7 @@ void backward_t(const torch::Tensor& dy, const torch::Tensor& x, const torch::Te
     // The rows are cut into parts, of 256 rows at least, until there is a
     // workgroup a CU: more parts are more float partials to write and read back.
     // us by workgroups 128, 256, 512, 1024, before a part's tiles shared a die:
-    // 1024 x 256 by 25601 rows 46, 37 (now 35), 42, 56; 64 x 64 by 409600 (T64)
+    // 1024 x 256 by 25601 rows 46, 37 (now 31), 42, 56; 64 x 64 by 409600 (T64)
     // 30, 21, 24, 27.  Where the tiles alone fill
     // half the card, two a CU (2048 x 2048 by 8192: 131, 118).  (T256's registers
     // are full already: 849 us against 647 for 4096 x 4096 by 16384.)  Through
