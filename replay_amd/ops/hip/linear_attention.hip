@@ -1733,5 +1733,9 @@ torch::Tensor linear_attention_step(torch::Tensor q, torch::Tensor k, torch::Ten
 #undef LA_STEP_T
 #undef LA_STEP
   HIP_CHECK(hipGetLastError());
+  // as every operation in place does: a backward pass that saved this state as
+  // its initial_state then raises instead of reading the new one (tensors made in
+  // inference mode have no such count)
+  if (!state.is_inference()) state.unsafeGetTensorImpl()->bump_version();
   return out;
 }

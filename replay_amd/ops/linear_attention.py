@@ -201,7 +201,8 @@ def linear_attention_step(
 
     :param q, k: [B, H, Dk]; v: [B, H, Dv].
     :param state: [B, H, Dk, Dv] float32, UPDATED IN PLACE; each head's
-        [Dk, Dv] block must be contiguous, and no two blocks may overlap.
+        [Dk, Dv] block must be contiguous, and no two blocks may overlap.  A
+        backward pass that still needs it (as ``initial_state``) then raises.
     :param active: [B] bool; a row that is False keeps its state and gets a
         zero output.
     :return: [B, H, Dv] in q's dtype.

@@ -764,3 +764,44 @@ class TestModuleOnGpu:
             for t in range(80, 90):
                 last = layer.step(x[:, t].to(dtype), states, mask[:, t])
         assert (last.float().cpu() - want[:, -1].detach()).norm() <= rel * want[:, -1].norm()
+
+
+def step_before_backward(device):
+    """A state is the start of a differentiable call, and a step changes it
+    before that call's backward pass."""
+    q, k, v, ld, s0, _, _ = inputs(2, 3, 5, 8, 8, torch.float32, device, carry=True)
+    out = linear_attention(q.requires_grad_(), k, v, ld, initial_state=s0)
+    with torch.no_grad():
+        linear_attention_step(q[:, :, 0], k[:, :, 0], v[:, :, 0], ld, s0)
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        out.sum().backward()
+
+
+def step_in_inference_mode(device):
+    q, k, v, ld, s0, _, _ = inputs(2, 3, 1, 8, 8, torch.float32, device, carry=True)
+    q, k, v = (t[:, :, 0] for t in (q, k, v))
+    want = s0.clone()
+    linear_attention_step(q, k, v, ld, want)
+    with torch.inference_mode():
+        made, given = s0.clone(), s0
+        for state in (made, given):
+            linear_attention_step(q, k, v, ld, state)
+    assert torch.equal(made, want) and torch.equal(given, want)
+
+
+class TestStepAndAutograd:
+    def test_step_before_backward(self):
+        step_before_backward("cpu")
+
+    def test_inference_mode(self):
+        step_in_inference_mode("cpu")
+
+
+@pytest.mark.gpu
+@requires_gpu
+class TestStepAndAutogradOnGpu:
+    def test_step_before_backward(self):
+        step_before_backward("cuda")
+
+    def test_inference_mode(self):
+        step_in_inference_mode("cuda")
