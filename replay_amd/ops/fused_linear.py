@@ -102,7 +102,8 @@ def fused_linear(
     :return: [..., N] in the inputs' dtype, accumulated in float32.
 
     All tensors share dtype and device; under CUDA autocast they are cast to
-    its dtype first, as ``torch.nn.Linear``'s are.  Differentiable once.
+    its dtype first, as ``torch.nn.Linear``'s are.  Differentiable once, on the
+    GPU in reverse mode alone (a dual tensor is refused there).
     """
     act = ACTIVATIONS.get(activation)
     if act is None:
@@ -116,7 +117,8 @@ def fused_linear(
         bias = bias.to(dt) if bias is not None else None
         residual = residual.to(dt) if residual is not None else None
     try:
-        if torch.is_grad_enabled() and (
+        # a trace records the autograd function, but not the extension's call
+        if torch.jit.is_tracing() or torch.is_grad_enabled() and (
             x.requires_grad or weight.requires_grad
             or (bias is not None and bias.requires_grad)
             or (residual is not None and residual.requires_grad)

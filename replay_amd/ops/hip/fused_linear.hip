@@ -832,6 +832,10 @@ std::vector<torch::Tensor> fused_linear_fwd(torch::Tensor x_in, torch::Tensor we
   weight = rows_of(weight);
   const int64_t M = x.size(0), N = weight.size(0);
   TORCH_CHECK(act >= 0 && act <= 3, "fused_linear: unknown activation");
+  // a dual tensor's tangent would be lost
+  auto dual = [](const c10::optional<torch::Tensor>& t) { return t.has_value() && t->_fw_grad(0).defined(); };
+  TORCH_CHECK(!dual(x_in) && !dual(weight) && !dual(bias) && !dual(residual),
+              "fused_linear: not differentiable in forward mode on the GPU");
   if (bias.has_value()) {
     TORCH_CHECK(bias->device() == x.device() && bias->scalar_type() == x.scalar_type() &&
                     bias->dim() == 1 && bias->size(0) == N,

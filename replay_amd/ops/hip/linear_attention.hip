@@ -1426,6 +1426,14 @@ void check_inputs(const torch::Tensor& q, const torch::Tensor& k, const torch::T
   }
 }
 
+// The kernels carry no forward-mode tangents: a dual tensor is refused, since its
+// tangent would be lost.
+template <typename... Ts>
+void check_no_tangent(const Ts&... given) {
+  auto has = [](const c10::optional<torch::Tensor>& t) { return t.has_value() && t->_fw_grad(0).defined(); };
+  TORCH_CHECK(!(has(given) || ...), "linear attention: not differentiable in forward mode on the GPU");
+}
+
 // [B, L, H, D] memory behind a [B, H, L, D] view: what the next projection
 // reads needs no copy.
 torch::Tensor heads_last(const torch::Tensor& q, int64_t D) {
@@ -1515,6 +1523,7 @@ std::vector<torch::Tensor> linear_attention_fwd(torch::Tensor q, torch::Tensor k
                                                 c10::optional<torch::Tensor> state, double scale,
                                                 bool want_state) {
   check_inputs(q, k, v, log_decay, mask, state, 4);
+  check_no_tangent(q, k, v, log_decay, state);
   const c10::hip::HIPGuardMasqueradingAsCUDA guard(q.device());
   auto stream = at::cuda::getCurrentHIPStream();
   q = unit_stride(q);
@@ -1680,6 +1689,7 @@ torch::Tensor linear_attention_step(torch::Tensor q, torch::Tensor k, torch::Ten
                                     torch::Tensor log_decay, torch::Tensor state,
                                     c10::optional<torch::Tensor> active, double scale) {
   check_inputs(q, k, v, log_decay, active, state, 3);
+  check_no_tangent(q, k, v, log_decay, state);
   const int64_t B = q.size(0), H = q.size(1), Dk = q.size(2), Dv = v.size(2);
   TORCH_CHECK((Dv <= 1 || state.stride(3) == 1) && (Dk <= 1 || state.stride(2) == Dv),
               "linear attention: each head's state must be contiguous");

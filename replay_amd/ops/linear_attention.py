@@ -165,7 +165,8 @@ def linear_attention(
     :return: [B, H, L, Dv] in q's dtype (its memory is laid out [B, L, H, Dv]),
         and the state if asked for.
 
-    Differentiable once in q, k, v, log_decay and initial_state.
+    Differentiable once in q, k, v, log_decay and initial_state; on the GPU in
+    reverse mode alone (a dual tensor is refused there).
     """
     scale = _scale(q, scale)
     args = (q, k, v, log_decay, padding_mask, initial_state, scale)
@@ -174,7 +175,8 @@ def linear_attention(
         out, state = eager_linear_attention(*args)
         return (out, state) if return_state else out
     try:
-        if torch.is_grad_enabled() and (
+        # a trace records the autograd function, but not the extension's call
+        if torch.jit.is_tracing() or torch.is_grad_enabled() and (
             q.requires_grad or k.requires_grad or v.requires_grad or log_decay.requires_grad
             or (initial_state is not None and initial_state.requires_grad)
         ):
@@ -197,7 +199,8 @@ def linear_attention_step(
     active: Optional[torch.Tensor] = None,
     scale: Optional[float] = None,
 ) -> torch.Tensor:
-    """One new position for each row, for serving (not differentiable).
+    """One new position for each row, for serving (not differentiable, and on
+    the GPU not traceable).
 
     :param q, k: [B, H, Dk]; v: [B, H, Dv].
     :param state: [B, H, Dk, Dv] float32, UPDATED IN PLACE; each head's
@@ -219,6 +222,8 @@ def linear_attention_step(
         _check(q, k, v, log_decay, active, state, scale, 3, "active", "state")
         _check_blocks(state)
         return _eager_step(q, k, v, log_decay, state, active, scale)
+    if torch.jit.is_tracing():
+        raise RuntimeError("linear_attention_step cannot be traced on the GPU: the trace would leave it out")
     try:
         return hip_ext().linear_attention_step(q, k, v, log_decay, state, active, scale)
     except RuntimeError:

@@ -5,6 +5,7 @@ import math
 
 import pytest
 import torch
+import torch.autograd.forward_ad as forward_ad
 
 from replay_amd.ops.fused_linear import fused_linear
 
@@ -334,3 +335,30 @@ class TestKernels:
             torch.cuda.synchronize()
             for a, c in zip(held, want):
                 assert torch.equal(a, c)
+
+
+@pytest.mark.gpu
+@requires_gpu
+class TestForwardModeAndTraces:
+    """What the kernels cannot carry is refused, and a trace holds the call."""
+
+    @pytest.mark.parametrize("which", range(4))
+    @pytest.mark.parametrize("grad", [False, True])
+    def test_tangents(self, which, grad):
+        args = list(make(8, 4, 5, torch.float32)[:4])
+        args[0].requires_grad_(grad)
+        with forward_ad.dual_level():
+            args[which] = forward_ad.make_dual(args[which], torch.ones_like(args[which]))
+            with pytest.raises(RuntimeError):
+                fused_linear(*args[:3], residual=args[3])
+
+    @pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32], ids=str)
+    def test_trace(self, dtype):
+        x, w, b, r, _ = make(70, 40, 24, dtype)
+
+        def call(x, r):
+            return fused_linear(x, w, b, "gelu", r)
+
+        with torch.no_grad():
+            traced = torch.jit.trace(call, (x, r), check_trace=False)
+            assert torch.equal(traced(2 * x, 3 * r), call(2 * x, 3 * r))

@@ -5,6 +5,7 @@ import math
 
 import pytest
 import torch
+import torch.autograd.forward_ad as forward_ad
 
 from replay_amd.ops.linear_attention import (
     eager_linear_attention,
@@ -805,3 +806,55 @@ class TestStepAndAutogradOnGpu:
 
     def test_inference_mode(self):
         step_in_inference_mode("cuda")
+
+
+@pytest.mark.gpu
+@requires_gpu
+class TestForwardModeAndTraces:
+    """What the kernels cannot carry is refused, and a trace holds the call."""
+
+    @pytest.mark.parametrize("which", range(5))
+    @pytest.mark.parametrize("grad", [False, True])
+    @pytest.mark.parametrize("L", [5, 1000])
+    def test_tangents(self, which, grad, L):
+        args = list(inputs(2, 3, L, 8, 8, torch.float32, "cuda", carry=True)[:5])
+        args[0].requires_grad_(grad)
+        with forward_ad.dual_level():
+            args[which] = forward_ad.make_dual(args[which], torch.ones_like(args[which]))
+            with pytest.raises(RuntimeError):
+                linear_attention(*args[:4], initial_state=args[4])
+        out = linear_attention(*args[:4])  # outside of the level there is none
+        assert torch.isfinite(out).all()
+
+    @pytest.mark.parametrize("which", range(5))
+    def test_tangents_of_a_step(self, which):
+        q, k, v, ld, s0, _, _ = inputs(2, 3, 1, 8, 8, torch.float32, "cuda", carry=True)
+        args = [q[:, :, 0], k[:, :, 0], v[:, :, 0], ld, s0]
+        kept = s0.clone()
+        with forward_ad.dual_level():
+            args[which] = forward_ad.make_dual(args[which], torch.ones_like(args[which]))
+            with pytest.raises(RuntimeError, match="forward mode"):
+                linear_attention_step(*args)
+        assert torch.equal(s0, kept)
+
+    @pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32], ids=str)
+    def test_trace(self, dtype):
+        q, k, v, ld, s0, _, _ = inputs(2, 3, 70, 8, 8, dtype, "cuda", carry=True)
+        mask = masks("left", 2, 70, "cuda")
+
+        def call(q, s0):
+            return linear_attention(q, k, v, ld, mask, s0, return_state=True)
+
+        with torch.no_grad():
+            traced = torch.jit.trace(call, (q, s0), check_trace=False)
+            for a, b in zip(traced(2 * q, 3 * s0), call(2 * q, 3 * s0)):
+                assert torch.equal(a, b)
+
+    def test_trace_of_a_step(self):
+        q, k, v, ld, s0, _, _ = inputs(2, 3, 1, 8, 8, torch.float32, "cuda", carry=True)
+
+        def call(q):
+            return linear_attention_step(q, k[:, :, 0], v[:, :, 0], ld, s0)
+
+        with torch.no_grad(), pytest.raises(RuntimeError, match="traced"):
+            torch.jit.trace(call, (q[:, :, 0],), check_trace=False)
