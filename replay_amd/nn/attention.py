@@ -189,10 +189,12 @@ class MultiheadLinearAttention(torch.nn.Module):
         return (t.unflatten(-1, (self.num_heads, self.head_dim)) for t in qkv.chunk(3, dim=-1))
 
     def _project(self, out: torch.Tensor, residual: Optional[torch.Tensor]) -> torch.Tensor:
-        from replay_amd.ops.fused_linear import fused_linear
+        from replay_amd.ops.fused_linear import fused_linear, fused_linear_residual
 
         out = self.head_norm(out.float()).to(out.dtype).flatten(-2)
-        return fused_linear(out, self.out_proj.weight, self.out_proj.bias, residual=residual)
+        if residual is None:
+            return fused_linear(out, self.out_proj.weight, self.out_proj.bias)
+        return fused_linear_residual(out, self.out_proj.weight, self.out_proj.bias, residual)
 
     def forward(
         self,

@@ -40,13 +40,13 @@ class PointWiseFeedForward(torch.nn.Module):
         self.fused = activation if fused else None
 
     def _forward_fused(self, x: torch.Tensor) -> torch.Tensor:
-        from replay_amd.ops.fused_linear import fused_linear
+        from replay_amd.ops.fused_linear import fused_linear, fused_linear_residual
 
         h = self.dropout1(fused_linear(x, self.w1.weight, self.w1.bias, activation=self.fused))
         if self.training and self.dropout2.p > 0.0:
             # the dropout stands between the product and the residual
             return self.dropout2(fused_linear(h, self.w2.weight, self.w2.bias)) + x
-        return fused_linear(h, self.w2.weight, self.w2.bias, residual=x)
+        return fused_linear_residual(h, self.w2.weight, self.w2.bias, x)
 
     def forward(self, x: torch.Tensor) -> torch.Tensor:
         if self.fused is not None:

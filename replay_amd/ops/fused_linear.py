@@ -129,3 +129,16 @@ def fused_linear(
         # the extension refuses what _check does, without the cost of asking twice
         _check(x, weight, bias, residual)
         raise
+
+
+def fused_linear_residual(
+    x: torch.Tensor, weight: torch.Tensor, bias: Optional[torch.Tensor], residual: torch.Tensor
+) -> torch.Tensor:
+    """``x @ weight.T + bias + residual`` for a residual stream: in one product
+    where the residual has the product's type.  A wider one (float32 under
+    autocast) is added in its own type instead, so that a stream of blocks is
+    not rounded to 16 bits by each."""
+    dt = torch.get_autocast_dtype("cuda") if x.is_cuda and torch.is_autocast_enabled("cuda") else x.dtype
+    if torch.promote_types(dt, residual.dtype) != dt:
+        return fused_linear(x, weight, bias) + residual
+    return fused_linear(x, weight, bias, residual=residual)

@@ -858,3 +858,51 @@ class TestForwardModeAndTraces:
 
         with torch.no_grad(), pytest.raises(RuntimeError, match="traced"):
             torch.jit.trace(call, (q[:, :, 0],), check_trace=False)
+
+
+def silent_layer(dropout, device):
+    """Six blocks whose products all add nothing to the residual stream."""
+    from replay_amd.nn.sequential import LinearTransformerLayer
+
+    layer = LinearTransformerLayer(64, 2, 6, dropout=dropout).to(device)
+    for block in layer.blocks:
+        for linear in (block.attention.out_proj, block.ffn.w2):
+            torch.nn.init.zeros_(linear.weight)
+            torch.nn.init.zeros_(linear.bias)
+    return layer
+
+
+def check_stream(dtype, dropout, device):
+    """Under autocast the stream keeps the type it came in, in training as in
+    serving, and is not rounded on its way."""
+    layer = silent_layer(dropout, device)
+    gen = torch.Generator().manual_seed(0)
+    x = torch.randn(2, 9, 64, generator=gen).to(dtype).to(device)
+
+    def through(*args):
+        with torch.autocast(device, dtype=torch.bfloat16):
+            return layer(*args)
+
+    def ffn_input(x):  # what is added to is the normed input, rounded to the norm's own type
+        for block in layer.blocks:
+            x = block.ffn_norm(x)
+        return x
+
+    want = ffn_input(x)
+    for mode in (True, False):
+        layer.train(mode)
+        got = through(x)
+        assert got.dtype == dtype and torch.equal(got, want)
+    with torch.no_grad(), torch.autocast(device, dtype=torch.bfloat16):
+        _, states = layer.prefill(x[:, :5])
+        got = layer.step(x[:, 5], states)
+    assert got.dtype == dtype and torch.equal(got, want[:, 5])
+
+
+@pytest.mark.gpu
+@requires_gpu
+class TestResidualStreamOnGpu:
+    @pytest.mark.parametrize("dropout", [0.0, 0.3])
+    @pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16], ids=str)
+    def test_keeps_its_type(self, dtype, dropout):
+        check_stream(dtype, dropout, "cuda")
