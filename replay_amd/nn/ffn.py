@@ -43,7 +43,7 @@ class PointWiseFeedForward(torch.nn.Module):
         from replay_amd.ops.fused_linear import fused_linear, fused_linear_residual
 
         h = self.dropout1(fused_linear(x, self.w1.weight, self.w1.bias, activation=self.fused))
-        if self.training and self.dropout2.p > 0.0:
+        if self.dropout2.training and self.dropout2.p > 0.0:
             # the dropout stands between the product and the residual
             return self.dropout2(fused_linear(h, self.w2.weight, self.w2.bias)) + x
         return fused_linear_residual(h, self.w2.weight, self.w2.bias, x)
