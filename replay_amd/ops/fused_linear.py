@@ -68,6 +68,13 @@ class FusedLinearFunction(torch.autograd.Function):
         )
 
 
+def _autocast(dtype: torch.dtype, *given: Optional[torch.Tensor]):
+    """What autocast makes of a linear layer's tensors: float64 and integers stay."""
+    return (
+        t.to(dtype) if t is not None and t.is_floating_point() and t.dtype != torch.float64 else t for t in given
+    )
+
+
 def _check(x, weight, bias, residual) -> None:
     given = [t for t in (x, weight, bias, residual) if t is not None]
     if any(t.device != x.device for t in given):
@@ -102,7 +109,7 @@ def fused_linear(
     :return: [..., N] in the inputs' dtype, accumulated in float32.
 
     All tensors share dtype and device; under CUDA autocast they are cast to
-    its dtype first, as ``torch.nn.Linear``'s are.  Differentiable once, on the
+    its dtype first, as ``torch.nn.Linear``'s are (which leaves float64 as it is).  Differentiable once, on the
     GPU in reverse mode alone (a dual tensor is refused there).
     """
     act = ACTIVATIONS.get(activation)
@@ -112,10 +119,7 @@ def fused_linear(
         _check(x, weight, bias, residual)
         return eager_fused_linear(x, weight, bias, activation, residual)
     if torch.is_autocast_enabled("cuda"):
-        dt = torch.get_autocast_dtype("cuda")
-        x, weight = x.to(dt), weight.to(dt)
-        bias = bias.to(dt) if bias is not None else None
-        residual = residual.to(dt) if residual is not None else None
+        x, weight, bias, residual = _autocast(torch.get_autocast_dtype("cuda"), x, weight, bias, residual)
     try:
         # a trace records the autograd function, but not the extension's call
         if torch.jit.is_tracing() or torch.is_grad_enabled() and (

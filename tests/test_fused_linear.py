@@ -382,3 +382,21 @@ class TestFeedForwardOnCpu:
                 torch.manual_seed(1)
                 outs.append(module(x))
             torch.testing.assert_close(*outs)
+
+
+@pytest.mark.gpu
+@requires_gpu
+class TestAutocastOnGpu:
+    @pytest.mark.parametrize("dtype", [torch.float64, torch.int32], ids=str)
+    @pytest.mark.parametrize("grad", [False, True])
+    def test_leaves_other_types_alone(self, dtype, grad):
+        x, w = torch.ones(6, 4, device="cuda"), torch.ones(5, 4, device="cuda", requires_grad=grad)
+        b, r = torch.ones(5, device="cuda"), torch.ones(6, 5, device="cuda")
+        with torch.autocast("cuda", dtype=torch.bfloat16):
+            fused_linear(x, w, b, residual=r)
+            for bad in (
+                (x.to(dtype), w, b, r), (x, w.detach().to(dtype), b, r), (x, w, b.to(dtype), r), (x, w, b, r.to(dtype)),
+                tuple(t.detach().to(dtype) for t in (x, w, b, r)),
+            ):
+                with pytest.raises(ValueError):
+                    fused_linear(*bad[:3], residual=bad[3])
