@@ -108,18 +108,19 @@ def fused_linear(
     :param residual: [..., N], of x's leading dimensions; never broadcast.
     :return: [..., N] in the inputs' dtype, accumulated in float32.
 
-    All tensors share dtype and device; under CUDA autocast they are cast to
+    All tensors share dtype and device; under autocast they are cast to
     its dtype first, as ``torch.nn.Linear``'s are (which leaves float64 as it is).  Differentiable once, on the
     GPU in reverse mode alone (a dual tensor is refused there).
     """
     act = ACTIVATIONS.get(activation)
     if act is None:
         raise ValueError(f"activation must be one of {sorted(ACTIVATIONS)}, got {activation!r}")
+    kind = "cuda" if x.is_cuda else "cpu"
+    if torch.is_autocast_enabled(kind):
+        x, weight, bias, residual = _autocast(torch.get_autocast_dtype(kind), x, weight, bias, residual)
     if not require_hip_on_gpu(x):
         _check(x, weight, bias, residual)
         return eager_fused_linear(x, weight, bias, activation, residual)
-    if torch.is_autocast_enabled("cuda"):
-        x, weight, bias, residual = _autocast(torch.get_autocast_dtype("cuda"), x, weight, bias, residual)
     try:
         # a trace records the autograd function, but not the extension's call
         if torch.jit.is_tracing() or torch.is_grad_enabled() and (
@@ -142,7 +143,8 @@ def fused_linear_residual(
     where the residual has the product's type.  A wider one (float32 under
     autocast) is added in its own type instead, so that a stream of blocks is
     not rounded to 16 bits by each."""
-    dt = torch.get_autocast_dtype("cuda") if x.is_cuda and torch.is_autocast_enabled("cuda") else x.dtype
+    kind = "cuda" if x.is_cuda else "cpu"
+    dt = torch.get_autocast_dtype(kind) if torch.is_autocast_enabled(kind) else x.dtype
     if torch.promote_types(dt, residual.dtype) != dt:
         return fused_linear(x, weight, bias) + residual
     return fused_linear(x, weight, bias, residual=residual)

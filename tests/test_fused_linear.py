@@ -400,3 +400,17 @@ class TestAutocastOnGpu:
             ):
                 with pytest.raises(ValueError):
                     fused_linear(*bad[:3], residual=bad[3])
+
+
+class TestAutocastOnCpu:
+    def test_casts_as_on_the_gpu(self):
+        gen = torch.Generator().manual_seed(0)
+        x, w, b, r = (torch.randn(*s, generator=gen) for s in ((6, 4), (5, 4), (5,), (6, 5)))
+        w.requires_grad_()
+        with torch.autocast("cpu", dtype=torch.bfloat16):
+            y = fused_linear(x.bfloat16(), w, b, "gelu", r)  # mixed types, as a stack of layers has them
+            z = fused_linear(x.double(), w.detach().double(), b.double())
+        assert y.dtype == torch.bfloat16 and z.dtype == torch.float64
+        assert torch.equal(y, fused_linear(*(t.bfloat16() for t in (x, w, b)), "gelu", r.bfloat16()))
+        (dw,) = torch.autograd.grad(y.sum(), [w])
+        assert dw.dtype == torch.float32

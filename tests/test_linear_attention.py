@@ -906,3 +906,10 @@ class TestResidualStreamOnGpu:
     @pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16], ids=str)
     def test_keeps_its_type(self, dtype, dropout):
         check_stream(dtype, dropout, "cuda")
+
+
+class TestResidualStreamOnCpu:
+    @pytest.mark.parametrize("dropout", [0.0, 0.3])
+    @pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16], ids=str)
+    def test_keeps_its_type(self, dtype, dropout):
+        check_stream(dtype, dropout, "cpu")
