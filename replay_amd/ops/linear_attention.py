@@ -23,6 +23,7 @@ replay_amd.ops.require_hip_on_gpu.
 
 from __future__ import annotations
 
+import functools
 import math
 from typing import Optional, Tuple, Union
 
@@ -79,6 +80,18 @@ def _power(log_decay: torch.Tensor, n: torch.Tensor) -> torch.Tensor:
     return torch.where(n > 0, torch.exp(log_decay * n.clamp(min=1)), torch.ones_like(n))
 
 
+def _without_autocast(function):
+    """Autocast would take the float32 products and sums to 16 bits."""
+
+    @functools.wraps(function)
+    def call(q, *args, **kwargs):
+        with torch.autocast(q.device.type, enabled=False):
+            return function(q, *args, **kwargs)
+
+    return call
+
+
+@_without_autocast
 def eager_linear_attention(
     q: torch.Tensor,
     k: torch.Tensor,
@@ -247,6 +260,7 @@ def _check_blocks(state: torch.Tensor) -> None:
         reach += stride * (size - 1)
 
 
+@_without_autocast
 def _eager_step(q, k, v, log_decay, state, active, scale: float) -> torch.Tensor:
     wide = log_decay.dtype
     qw, kw, vw = q.to(wide), k.to(wide), v.to(wide)

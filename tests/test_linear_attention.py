@@ -913,3 +913,21 @@ class TestResidualStreamOnCpu:
     @pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16], ids=str)
     def test_keeps_its_type(self, dtype, dropout):
         check_stream(dtype, dropout, "cpu")
+
+
+class TestAutocastOnCpu:
+    @pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16], ids=str)
+    def test_keeps_32_bits(self, dtype):
+        q, k, v, ld, s0, do, ds = inputs(2, 2, 130, 4, 6, dtype, "cpu", carry=True)
+
+        def call(enabled):
+            leaves = [t.clone().requires_grad_() for t in (q, k, v, ld, s0)]
+            step = s0.clone()
+            with torch.autocast("cpu", dtype=torch.bfloat16, enabled=enabled):
+                out, state = linear_attention(*leaves[:4], initial_state=leaves[4], return_state=True)
+                with torch.no_grad():
+                    o = linear_attention_step(q[:, :, 0], k[:, :, 0], v[:, :, 0], ld, step)
+            return (out, state, o, step, *torch.autograd.grad([out, state], leaves, [do, ds]))
+
+        for a, b in zip(call(True), call(False)):
+            assert a.dtype == b.dtype and torch.equal(a, b)
