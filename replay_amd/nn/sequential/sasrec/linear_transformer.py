@@ -87,7 +87,8 @@ class LinearTransformerLayer(torch.nn.Module):
 
     @staticmethod
     def _blank(x: torch.Tensor, valid: Optional[torch.Tensor]) -> torch.Tensor:
-        return x if valid is None else x * valid.unsqueeze(-1).to(x.dtype)
+        # chosen, not multiplied: what the other rows hold need not be finite
+        return x if valid is None else torch.where(valid.unsqueeze(-1), x, 0.0)
 
     def forward(
         self,
@@ -97,10 +98,12 @@ class LinearTransformerLayer(torch.nn.Module):
     ) -> torch.Tensor:
         """x: [B, L, E]; padding_mask: [B, L] bool, True = VALID.  attn_mask
         (DefaultAttentionMask's MaskSpec) must be causal; without a
-        padding_mask its own is used."""
+        padding_mask its own is used.  What masked rows of x hold is not used;
+        they give zeros."""
         self._check_mask(attn_mask)
         if padding_mask is None and attn_mask is not None:
             padding_mask = attn_mask.padding_mask
+        x = self._blank(x, padding_mask)
         for block in self.blocks:
             x = self._blank(block(x, padding_mask), padding_mask)
         return x
@@ -117,6 +120,7 @@ class LinearTransformerLayer(torch.nn.Module):
         if states is not None and len(states) != len(self.blocks):
             raise ValueError(f"expected {len(self.blocks)} states, got {len(states)}")
         new = []
+        x = self._blank(x, padding_mask)
         for i, block in enumerate(self.blocks):
             x, state = block(x, padding_mask, None if states is None else states[i], return_state=True)
             x = self._blank(x, padding_mask)
@@ -134,6 +138,7 @@ class LinearTransformerLayer(torch.nn.Module):
         place.  Rows that ``active`` [B] leaves out keep theirs and give zeros."""
         if len(states) != len(self.blocks):
             raise ValueError(f"expected {len(self.blocks)} states, got {len(states)}")
+        x = self._blank(x, active)
         for block, state in zip(self.blocks, states):
             x = self._blank(block.step(x, state, active), active)
         return x

@@ -931,3 +931,49 @@ class TestAutocastOnCpu:
 
         for a, b in zip(call(True), call(False)):
             assert a.dtype == b.dtype and torch.equal(a, b)
+
+
+def check_layer_ignores(device, bad):
+    """Masked rows of a layer's input may hold anything: outputs, states and
+    every gradient are those of rows that hold zeros."""
+    from replay_amd.nn.sequential import LinearTransformerLayer
+
+    torch.manual_seed(0)
+    layer = LinearTransformerLayer(16, 2, 2, learn_decay=True).to(device)
+    mask = masks("left", 3, 7, device)
+    gen = torch.Generator().manual_seed(0)
+    x = torch.randn(3, 7, 16, generator=gen).to(device)
+    x[~mask] = 0.0
+
+    def results(x):
+        leaf = x.clone().requires_grad_()
+        out = layer(leaf, padding_mask=mask)
+        grads = torch.autograd.grad(out.square().sum(), [leaf, *layer.parameters()])
+        with torch.no_grad():
+            first, states = layer.prefill(x[:, :6], mask[:, :6])
+            last = layer.step(x[:, 6], states, mask[:, 6])
+        return out, *grads, first, last, *states
+
+    want = results(x)
+    x[~mask] = bad
+    summed = [False, False, *("_norm." in n and "head" not in n for n, _ in layer.named_parameters())]
+    for i, (a, b) in enumerate(zip(results(x), want)):
+        if device == "cuda" and i < len(summed) and summed[i]:
+            # the layer norms' gradients are sums of 21 terms in no fixed order: they
+            # differ by at most 40 2^-24 of the sum S of the absolute values, which is
+            # within 2^-10 of the largest unless S is 400 times that
+            assert (a - b).abs().max() <= 2.0**-10 * b.abs().max()
+        else:
+            assert torch.equal(a, b), i
+
+
+class TestMaskedRowsOfALayer:
+    @pytest.mark.parametrize("bad", [math.nan, math.inf, 3.0e38])
+    def test_on_cpu(self, bad):
+        check_layer_ignores("cpu", bad)
+
+    @pytest.mark.gpu
+    @requires_gpu
+    @pytest.mark.parametrize("bad", [math.nan, -math.inf, 3.0e38])
+    def test_on_gpu(self, bad):
+        check_layer_ignores("cuda", bad)
