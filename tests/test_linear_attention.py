@@ -977,3 +977,26 @@ class TestMaskedRowsOfALayer:
     @pytest.mark.parametrize("bad", [math.nan, -math.inf, 3.0e38])
     def test_on_gpu(self, bad):
         check_layer_ignores("cuda", bad)
+
+
+def check_states_are_new(device):
+    """Steps on a returned state leave the one it started from alone, also where
+    the history between had no position."""
+    for L in (0, 1, 70):
+        q, k, v, ld, s0, _, _ = inputs(2, 3, L, 4, 6, torch.float32, device, carry=True)
+        kept = s0.clone()
+        _, state = linear_attention(q, k, v, ld, initial_state=s0, return_state=True)
+        assert L or torch.equal(state, s0)
+        one = torch.ones(2, 3, 6, device=device)
+        linear_attention_step(one[..., :4], one[..., :4], one, ld, state)
+        assert torch.equal(s0, kept)
+
+
+class TestStatesAreNew:
+    def test_on_cpu(self):
+        check_states_are_new("cpu")
+
+    @pytest.mark.gpu
+    @requires_gpu
+    def test_on_gpu(self):
+        check_states_are_new("cuda")
