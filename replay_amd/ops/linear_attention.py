@@ -109,8 +109,9 @@ def eager_linear_attention(
     zero = torch.zeros((), dtype=wide, device=q.device)
     q, k, v = (torch.where(valid[:, None, :, None], t.to(wide), zero) for t in (q, k, v))
     ld = log_decay.view(1, H, 1)
-    # a copy also where no position changes it: the state after is never the one before
-    state = initial_state.clone() if initial_state is not None else q.new_zeros(B, H, Dk, v.shape[-1])
+    state = initial_state if initial_state is not None else q.new_zeros(B, H, Dk, v.shape[-1])
+    if not L:  # a copy where no position changes it: the state after is never the one before
+        state = state.clone()
     outs = []
     for s in range(0, L, chunk):
         qc, kc, vc = (t[:, :, s : s + chunk] for t in (q, k, v))
