@@ -173,14 +173,18 @@ class MultiheadLinearAttention(torch.nn.Module):
         # decay 1 - 1/horizon, as a logit
         self.decay_logit = torch.nn.Parameter(torch.log(horizon - 1.0), requires_grad=learn_decay)
 
+    def _wide(self, t: torch.Tensor) -> torch.Tensor:
+        # decays, states and norms are held in 32 bits, in 64 in a float64 module
+        return t.to(torch.promote_types(t.dtype, torch.float32))
+
     def log_decay(self) -> torch.Tensor:
-        return torch.nn.functional.logsigmoid(self.decay_logit.float())
+        return torch.nn.functional.logsigmoid(self._wide(self.decay_logit))
 
     def new_state(self, batch_size: int) -> torch.Tensor:
-        """The state before the first position: [B, H, Dh, Dh] float32 zeros."""
-        return torch.zeros(
-            batch_size, self.num_heads, self.head_dim, self.head_dim, device=self.decay_logit.device
-        )
+        """The state before the first position: [B, H, Dh, Dh] zeros, float32
+        (float64 in a float64 module)."""
+        shape = (batch_size, self.num_heads, self.head_dim, self.head_dim)
+        return self._wide(self.decay_logit.detach()).new_zeros(shape)
 
     def _heads(self, x: torch.Tensor):
         from replay_amd.ops.fused_linear import fused_linear
@@ -191,7 +195,7 @@ class MultiheadLinearAttention(torch.nn.Module):
     def _project(self, out: torch.Tensor, residual: Optional[torch.Tensor]) -> torch.Tensor:
         from replay_amd.ops.fused_linear import fused_linear, fused_linear_residual
 
-        out = self.head_norm(out.float()).to(out.dtype).flatten(-2)
+        out = self.head_norm(self._wide(out)).to(out.dtype).flatten(-2)
         if residual is None:
             return fused_linear(out, self.out_proj.weight, self.out_proj.bias)
         return fused_linear_residual(out, self.out_proj.weight, self.out_proj.bias, residual)

@@ -1000,3 +1000,26 @@ class TestStatesAreNew:
     @requires_gpu
     def test_on_gpu(self):
         check_states_are_new("cuda")
+
+
+class TestFloat64Module:
+    def test_layer(self):
+        from replay_amd.nn.sequential import LinearTransformerLayer
+
+        torch.manual_seed(0)
+        layer = LinearTransformerLayer(16, 2, 2, learn_decay=True)
+        x = torch.randn(2, 7, 16)
+        want = layer(x)
+        wide = LinearTransformerLayer(16, 2, 2, learn_decay=True)
+        wide.load_state_dict(layer.state_dict())
+        wide.double()
+        got = wide(x.double())
+        assert got.dtype == torch.float64
+        torch.testing.assert_close(got.float(), want, rtol=1e-4, atol=1e-5)
+        states = [block.attention.new_state(2) for block in wide.blocks]
+        steps = torch.stack([wide.step(x[:, t].double(), states) for t in range(7)], 1)
+        # two orders of the same float64 sums
+        torch.testing.assert_close(steps, got, rtol=1e-10, atol=1e-12)
+        states = [block.attention.new_state(2) for block in layer.blocks]
+        assert all(s.dtype == torch.float32 and not s.requires_grad for s in states)
+        layer.step(x[:, 0], states)
