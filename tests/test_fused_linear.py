@@ -414,3 +414,53 @@ class TestAutocastOnCpu:
         assert torch.equal(y, fused_linear(*(t.bfloat16() for t in (x, w, b)), "gelu", r.bfloat16()))
         (dw,) = torch.autograd.grad(y.sum(), [w])
         assert dw.dtype == torch.float32
+
+
+@pytest.mark.gpu
+@requires_gpu
+class TestTiles:
+    """Each tile of each product, with ragged edges: (rows, K, N), and what the
+    forward product, dx and dW (in how many parts of the rows) run on."""
+
+    @pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16], ids=str)
+    @pytest.mark.parametrize("act", ["none", "gelu"])
+    @pytest.mark.parametrize(
+        "M,K,N",
+        [
+            (4097, 1032, 4104),  # 256x256; 128x128; 128x128 in 4 waves, 1 part
+            (4097, 4104, 1032),  # 128x128; 256x256; as above
+            (33000, 136, 72),    # 128x64, two stages; the same; 128x128 in 8 waves, 104 parts
+            (33001, 56, 48),     # 128x64, one stage; the same; 64x64, 104 parts
+            (4097, 1031, 4103),  # 128x128 through registers; 64x64 so; 64x64 so, 1 part
+            (4097, 4103, 1031),  # 64x64 so; 128x128 so; as above
+            (2001, 1416, 1504),  # 128x64, two stages; the same; 128x128 in 4 waves, 3 parts
+            (2000, 136, 72),     # 64x64; the same; 128x128 in 8 waves, 7 parts
+        ],
+    )
+    def test_16_bits(self, M, K, N, act, dtype):
+        check(*make(M, K, N, dtype, residual=act != "none"), act, dtype)
+
+    @pytest.mark.parametrize(
+        "M,K,N",
+        [
+            (4097, 516, 4100),  # 128x128; 128x64, two stages; 128x128, 3 parts
+            (4097, 4100, 516),  # 128x64, two stages; 128x128; 128x128, 3 parts
+            (33000, 68, 72),    # 128x64, two stages; the same; 128x128, 104 parts
+            (33001, 32, 64),    # 128x64, one stage; two stages; 64x64, 104 parts
+            (4097, 515, 4099),  # 64x64 through registers
+        ],
+    )
+    def test_float32(self, M, K, N):
+        check(*make(M, K, N, torch.float32), "silu", torch.float32)
+
+    @pytest.mark.parametrize("off", [8, 3])
+    def test_rows_of_a_wider_buffer(self, off):
+        # 256x256 with whole chunks, and through registers off 16 bytes
+        gen = torch.Generator().manual_seed(0)
+        M, K, N = 4097, 1032, 4104
+        x = torch.randn(M, K + 16, generator=gen).bfloat16().cuda()[:, off : off + K]
+        w = (torch.randn(N, K + 8, generator=gen) / 32).bfloat16().cuda()[:, :K]
+        r = torch.randn(M, N + 24, generator=gen).bfloat16().cuda()[:, off : off + N]
+        b = torch.randn(N, generator=gen).bfloat16().cuda()
+        dy = torch.randn(M, N + 8, generator=gen).bfloat16().cuda()[:, :N]
+        check(x, w, b, r, dy, "relu", torch.bfloat16)
