@@ -17,6 +17,7 @@ from __future__ import annotations
 from typing import Optional
 
 import torch
+from torch._C import _is_tracing  # torch.jit.is_tracing() without its 0.4 us
 from torch.autograd.function import once_differentiable
 
 from replay_amd.ops import hip_ext, require_hip_on_gpu
@@ -123,7 +124,7 @@ def fused_linear(
         return eager_fused_linear(x, weight, bias, activation, residual)
     try:
         # a trace records the autograd function, but not the extension's call
-        if torch.jit.is_tracing() or torch.is_grad_enabled() and (
+        if _is_tracing() or torch.is_grad_enabled() and (
             x.requires_grad or weight.requires_grad
             or (bias is not None and bias.requires_grad)
             or (residual is not None and residual.requires_grad)
