@@ -11,6 +11,12 @@ state, its output and its gradients are zero, and what its rows of q, k, v hold
 is not read.  A left-padded, a right-padded and an unpadded batch of the same
 histories therefore give the same states.
 
+An infinity or a NaN at a valid position, or in a state, stays with its (batch,
+head): the outputs and states that depend on it are not finite, NaN where the
+formula gives an infinity too (the kernels split operands into sums, where it
+becomes inf - inf), and so may the outputs of up to 63 positions before it be
+(they share a product with it, with a weight of zero).
+
 The state [B, H, Dk, Dv] (float32) is all that a history leaves behind:
 ``linear_attention(..., return_state=True)`` gives it, ``initial_state``
 continues from it, and :func:`linear_attention_step` adds one position to it in

@@ -1023,3 +1023,48 @@ class TestFloat64Module:
         states = [block.attention.new_state(2) for block in layer.blocks]
         assert all(s.dtype == torch.float32 and not s.requires_grad for s in states)
         layer.step(x[:, 0], states)
+
+
+def check_not_finite(device, dtype, L, D, bad, which):
+    """A value that is not finite is never lost, and reaches nothing but its own
+    (batch, head) from 63 positions before it on."""
+    args = dict(zip(("q", "k", "v", "log_decay", "initial_state"), inputs(2, 2, L, D, D, dtype, device, carry=True)[:5]))
+
+    def call():
+        return linear_attention(**args, return_state=True)
+
+    want = call()
+    at = L // 2
+    if which == "initial_state":
+        at = 0
+        args[which][1, 1, 0, 0] = bad
+    else:
+        args[which][1, 1, at, 0] = bad
+    out, state = call()
+    for a, b in zip((out, state), want):
+        assert torch.equal(a[0], b[0]) and torch.equal(a[1, 0], b[1, 0])
+    first = max(at - 63, 0)
+    assert torch.equal(out[1, 1, :first], want[0][1, 1, :first])
+    if which == "q":
+        assert not torch.isfinite(out[1, 1, at]).any() and torch.equal(state[1, 1], want[1][1, 1])
+    else:
+        columns = slice(0, 1) if which in ("v", "initial_state") else slice(0, D)  # what k touches, all values see
+        assert not torch.isfinite(out[1, 1, at:, columns]).any()
+        rows = slice(0, 1) if which in ("k", "initial_state") else slice(0, D)
+        assert not torch.isfinite(state[1, 1, rows, columns]).any()
+    if which in ("v", "initial_state"):
+        assert torch.equal(out[1, 1, :, 1:], want[0][1, 1, :, 1:])
+
+
+@pytest.mark.parametrize("bad", [math.nan, math.inf, -math.inf])
+@pytest.mark.parametrize("which", ["q", "k", "v", "initial_state"])
+class TestNotFinite:
+    def test_on_cpu(self, which, bad):
+        check_not_finite("cpu", torch.float32, 150, 8, bad, which)
+
+    @pytest.mark.gpu
+    @requires_gpu
+    @pytest.mark.parametrize("dtype", DTYPES, ids=str)
+    @pytest.mark.parametrize("L,D", [(150, 8), (60, 32), (200, 64), (140, 128), (1500, 64)])
+    def test_on_gpu(self, which, bad, dtype, L, D):
+        check_not_finite("cuda", dtype, L, D, bad, which)
