@@ -7,6 +7,11 @@ a backward pass whose products are the framework's own kernels too
 (``hip/fused_linear.hip``).  CPU path: explicit torch math; GPU path: falls
 back loudly per replay_amd.ops.require_hip_on_gpu.
 
+Products and sums are float32 with one rounding of the result.  Two more in the
+backward pass of an activation, both to the inputs' type: the slope is taken at
+``x W^T + bias`` as kept from the forward pass, and dy times the slope is what the
+products for dx and dW read (the bias gradient sums it before that rounding).
+
 Beside :class:`replay_amd.ops.fast_linear.ChunkedWgradLinear` this is the form
 for layers whose activation or residual follows at once
 (:class:`replay_amd.nn.ffn.PointWiseFeedForward` with ``fused=True``).
@@ -109,9 +114,10 @@ def fused_linear(
     :param residual: [..., N], of x's leading dimensions; never broadcast.
     :return: [..., N] in the inputs' dtype, accumulated in float32.
 
-    All tensors share dtype and device; under autocast they are cast to
-    its dtype first, as ``torch.nn.Linear``'s are (which leaves float64 as it is).  Differentiable once, on the
-    GPU in reverse mode alone (a dual tensor is refused there).
+    All tensors share dtype and device; under autocast they are cast to its
+    dtype first, as ``torch.nn.Linear``'s are (which leaves float64 as it is).
+    Differentiable once, on the GPU in reverse mode alone (a dual tensor is
+    refused there).
     """
     act = ACTIVATIONS.get(activation)
     if act is None:

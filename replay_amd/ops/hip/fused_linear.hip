@@ -7,7 +7,9 @@
 // index is contiguous in memory, and in where the contraction runs (over the
 // rows, M, for dW: it is split over workgroups and joined in a fixed order).
 // z is kept for the backward pass in the input's type, rounded once: act' is
-// as exact as the gradient's own rounding needs.
+// as exact as the gradient's own rounding needs.  dz is rounded to it too, since
+// the matrix instructions take it so (db sums it before): gradients of bfloat16
+// inputs with gelu are then off by 2.4e-3 of their norm, 1.7e-3 with one rounding.
 
 #include <torch/extension.h>
 #include <ATen/hip/HIPContext.h>

@@ -1321,8 +1321,8 @@ struct Split {
   int G, seg_chunks;
 };
 
-// Positions of one load: bfloat16's pass takes 64; float16 shares float32's (its
-// range does not hold a state that long histories add up to).
+// Positions of one load: bfloat16's pass takes 64; float16 shares float32's, which
+// holds everything in float32 (a state is past float16's own range).
 int chunk_of(torch::ScalarType dt) { return dt == torch::kBFloat16 ? 64 : 32; }
 
 // One workgroup for each (batch, head) where these alone fill the card (two a

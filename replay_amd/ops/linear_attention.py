@@ -22,6 +22,12 @@ The state [B, H, Dk, Dv] (float32) is all that a history leaves behind:
 continues from it, and :func:`linear_attention_step` adds one position to it in
 time that does not depend on the history's length.
 
+What the kernels hold in fewer than 32 bits: with bfloat16 inputs the weights of
+the position pairs within 64 positions, rounded once to bfloat16 (2^-8 of each
+term), and the state's part of an output, taken as two bfloat16 numbers (2^-17;
+three in the decay's gradient).  States, their updates and every sum are float32,
+and float16 and float32 inputs meet float32 products alone.
+
 CPU path: explicit torch math (the numerics reference).  GPU path: the gfx950
 kernels of ``hip/linear_attention.hip``; falls back loudly per
 replay_amd.ops.require_hip_on_gpu.
