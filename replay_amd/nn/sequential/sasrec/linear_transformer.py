@@ -87,8 +87,12 @@ class LinearTransformerLayer(torch.nn.Module):
 
     @staticmethod
     def _blank(x: torch.Tensor, valid: Optional[torch.Tensor]) -> torch.Tensor:
+        if valid is None:
+            return x
+        if valid.dtype != torch.bool or valid.shape != x.shape[:-1]:
+            raise ValueError(f"the mask must be bool of shape {tuple(x.shape[:-1])}")
         # chosen, not multiplied: what the other rows hold need not be finite
-        return x if valid is None else torch.where(valid.unsqueeze(-1), x, 0.0)
+        return torch.where(valid.unsqueeze(-1), x, 0.0)
 
     def forward(
         self,

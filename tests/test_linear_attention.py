@@ -1068,3 +1068,21 @@ class TestNotFinite:
     @pytest.mark.parametrize("L,D", [(150, 8), (60, 32), (200, 64), (140, 128), (1500, 64)])
     def test_on_gpu(self, which, bad, dtype, L, D):
         check_not_finite("cuda", dtype, L, D, bad, which)
+
+
+class TestLayerRefusals:
+    @pytest.mark.parametrize("change", [lambda m: m.float(), lambda m: m.long(), lambda m: m[:, :4], lambda m: m[:1], lambda m: m[0]])
+    def test_masks(self, change):
+        from replay_amd.nn.sequential import LinearTransformerLayer
+
+        layer = LinearTransformerLayer(16, 2, 1)
+        x, mask = torch.randn(2, 5, 16), torch.ones(2, 5, dtype=torch.bool)
+        for call in (lambda m: layer(x, padding_mask=m), lambda m: layer.prefill(x, m)):
+            call(mask)
+            with pytest.raises(ValueError, match="mask"):
+                call(change(mask))
+        states = [block.attention.new_state(2) for block in layer.blocks]
+        for active in (torch.ones(2), torch.ones(3, dtype=torch.bool), torch.ones(2, 1, dtype=torch.bool)):
+            with pytest.raises(ValueError, match="mask"):
+                layer.step(x[:, 0], states, active)
+        assert not states[0].any()
