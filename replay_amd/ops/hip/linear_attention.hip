@@ -590,13 +590,13 @@ __device__ __forceinline__ int state_row(int t, int g, int r) {
 // launch bounds are the tightest that spill no vector registers, and the build
 // refuses kernels here that do: an earlier form of this pass with 53 spilled
 // registers at head size 128 gave wrong first chunks now and then.  Why is not
-// known.  Read in full, its assembly waits for every load before its use; a load is
-// there before younger stores, to scratch memory too (0 of 168 million early); and
-// no two waves share LDS without a barrier between.  AHEAD: a chunk's rows are loaded while the one
-// before is worked on.  At head size 128 two workgroups a CU (128 registers)
-// without that hide the loads better than one with it, where there are as many:
-// 64 x 8 heads of 512, 57 us against 80; 2 x 8 of 16384 in 256 workgroups, 147
-// against 122.
+// known.  Read in full, its assembly waits for every load before its use; a load
+// is there before younger stores, to scratch memory too (0 of 168 million early);
+// and no two waves share LDS without a barrier between.
+// AHEAD: a chunk's rows are loaded while the one before is worked on.  At head
+// size 128 two workgroups a CU (128 registers) without that hide the loads better
+// than one with it, where there are as many: 64 x 8 heads of 512, 57 us against
+// 80; 2 x 8 of 16384 in 256 workgroups, 147 against 122.
 template <int DP, bool REV, bool STATE_ONLY, bool DERIV, bool EDGE, bool AHEAD>
 __global__ __launch_bounds__(DP * 4, DERIV ? 2 : AHEAD ? 3 : 4) void la_pass_bf16(Passes<passes_of(REV, STATE_ONLY, DERIV)> all_passes) {
   constexpr bool PAIR = passes_of(REV, STATE_ONLY, DERIV) == 2;
